@@ -108,6 +108,21 @@ int r3d_unrelayout_head(const RadParam* p, int n_p, int operand, const RadEncodi
                         const int* sel, const void* src, int64_t src_bytes,
                         const RadTensor* planes, int n);
 
+/* ---- extension rows: ops the reference does not have. They stand in a table of their own
+ * (r3d_b200_ext_kernel_count / _at), so that an engine's row table stays the reference's; with R3D_EXT_ROWS set the
+ * loader's table (rad_kernel_at) carries them too. Their schemas are in the schema list always. */
+int                  r3d_b200_ext_kernel_count(void);
+const RadKernelInfo* r3d_b200_ext_kernel_at(int i);
+/* gemm_nt_q @ i8a8 (a, a_scale, b, b_scale, y): int8 codes, one scale a token and one a channel. */
+int r3d_rad_gemm_nt_q_i8(const RadArgs* a, RadStream s);
+/* its activation producers, one scale a token: quant_token_i8 (x, q, scale), gated_quant_token_i8 (gate_up, q, scale,
+ * out?), rmsnorm_quant_token_i8 (x, residual?, w, q, scale, out?). */
+int r3d_rad_quant_token_i8(const RadArgs* a, RadStream s);
+int r3d_rad_gated_quant_token_i8(const RadArgs* a, RadStream s);
+int r3d_rad_rmsnorm_quant_token_i8(const RadArgs* a, RadStream s);
+/* sample_nucleus (logits, u, temperature?, top_k?, top_p?, min_p?, token, logprob?, kept?). */
+int r3d_rad_sample_nucleus(const RadArgs* a, RadStream s);
+
 /* ------------------------------------------------------------------ (2) launch layer */
 
 /* Which kernel serves a call. AUTO picks by shape and alignment the way the entries do.
@@ -211,6 +226,56 @@ int r3d_b200_gemm_fp8a8_gated(const R3dGemmQ* q, void* codes, int64_t q_pitch, f
  * mma.sync over byte-quads cut from the 2-bit plane; anything else: one thread per weight row with dp4a.
  * Both apply the oracle's flush per 128 of K; exact, bit-identical to each other. */
 int r3d_b200_gemm_w2a8(const R3dW2A8* q, void* stream);
+
+/* Operands of one gemm_nt_q @ i8a8 call: y[m, n] = (float(sum_k a[m, k] b[n, k]) * a_scale[m]) * b_scale[n], the sum
+ * exact in 32-bit integers, the result rounded once to y's type. Every arm gives the same bits. */
+typedef struct R3dGemmI8 {
+    const void*  a;         /* int8 codes [M, K] */
+    const float* a_scale;   /* f32, one a token */
+    const void*  b;         /* int8 codes [N, K] */
+    const void*  b_scale;   /* f32 or bf16, one a channel */
+    void*        y;         /* bf16 or f32 [M, N] */
+    int32_t      m, n, k;   /* k <= 131071: the sum of k products of two codes stays inside 32 bits */
+    int32_t      bs_dtype, y_dtype;
+    int32_t      arm;       /* R3D_ARM_AUTO, _EXACT (any alignment), _TILE (tcgen05) */
+    int64_t      a_pitch, b_pitch, y_pitch, as_pitch, bs_pitch;   /* elements */
+} R3dGemmI8;
+int r3d_b200_gemm_i8a8(const R3dGemmI8* q, void* stream);
+
+/* One call of an int8 activation producer: h as `kind` says, then per token scale = max|h| / 127 and
+ * q = rint(h * (127 / max|h|)); a row below 2^-100 has scale 1 and codes 0. h is held in f32. */
+enum { R3D_TOKEN_QUANT = 0, R3D_TOKEN_SILU = 1, R3D_TOKEN_SIGMOID = 2, R3D_TOKEN_RMSNORM = 3 };
+typedef struct R3dTokenI8 {
+    const void* x;          /* [rows, n], [rows, 2n] for the gated kinds (gate half first); x_dtype RAD_BF16 or RAD_F32 */
+    void*       residual;   /* RMSNORM: optional [rows, n] of x's type, updated with x + residual */
+    const void* w;          /* RMSNORM: [n], w_dtype RAD_BF16 or RAD_F32 */
+    void*       q;          /* int8 [rows, n] */
+    float*      scale;      /* f32, one a row */
+    void*       out;        /* optional [rows, n]: h, narrowed to out_dtype (RAD_BF16 or RAD_F32) */
+    int32_t     kind, x_dtype, w_dtype, out_dtype;
+    int32_t     rows, n;
+    float       eps, wadd;
+    int64_t     x_pitch, r_pitch, q_pitch, s_pitch, out_pitch;   /* elements */
+} R3dTokenI8;
+int r3d_b200_token_i8(const R3dTokenI8* q, void* stream);
+
+/* One call of sample_nucleus (kern_nucleus.cu states the rule). A null parameter plane switches its filter off
+ * (temperature: 1); per-row planes have a stride, 0 for one value for all rows. */
+typedef struct R3dNucleus {
+    const void*    logits;  /* [rows, n_vocab], x_dtype RAD_F32 or RAD_BF16 */
+    const float*   u;       /* [rows], in [0, 1) */
+    const float*   temperature;
+    const int32_t* top_k;
+    const float*   top_p;
+    const float*   min_p;
+    int32_t*       token;
+    float*         logprob; /* optional: log of the token's share of what the filters kept */
+    int32_t*       kept;    /* optional: how many tokens the filters kept */
+    int32_t        rows, n_vocab, x_dtype;
+    int32_t        shift;   /* set by the library */
+    int64_t        x_pitch, u_pitch, t_pitch, k_pitch, p_pitch, mp_pitch, token_pitch, lp_pitch, kept_pitch;
+} R3dNucleus;
+int r3d_b200_sample_nucleus(const R3dNucleus* q, void* stream);
 
 typedef struct R3dLogits {
     const void* x;          /* bf16 [M, K] */

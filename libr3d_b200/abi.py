@@ -129,6 +129,34 @@ class R3dW2A8(C.Structure):
                 ("b_pitch", C.c_int64), ("zp_pitch", C.c_int64), ("sc_pitch", C.c_int64)]
 
 
+class R3dGemmI8(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("a_scale", C.c_void_p), ("b", C.c_void_p), ("b_scale", C.c_void_p),
+                ("y", C.c_void_p), ("m", C.c_int32), ("n", C.c_int32), ("k", C.c_int32),
+                ("bs_dtype", C.c_int32), ("y_dtype", C.c_int32), ("arm", C.c_int32),
+                ("a_pitch", C.c_int64), ("b_pitch", C.c_int64), ("y_pitch", C.c_int64),
+                ("as_pitch", C.c_int64), ("bs_pitch", C.c_int64)]
+
+
+R3D_TOKEN_QUANT, R3D_TOKEN_SILU, R3D_TOKEN_SIGMOID, R3D_TOKEN_RMSNORM = range(4)
+
+
+class R3dTokenI8(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("residual", C.c_void_p), ("w", C.c_void_p), ("q", C.c_void_p),
+                ("scale", C.c_void_p), ("out", C.c_void_p),
+                ("kind", C.c_int32), ("x_dtype", C.c_int32), ("w_dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("rows", C.c_int32), ("n", C.c_int32), ("eps", C.c_float), ("wadd", C.c_float),
+                ("x_pitch", C.c_int64), ("r_pitch", C.c_int64), ("q_pitch", C.c_int64), ("s_pitch", C.c_int64),
+                ("out_pitch", C.c_int64)]
+
+
+class R3dNucleus(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p),
+                ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("token", C.c_void_p), ("logprob", C.c_void_p),
+                ("kept", C.c_void_p), ("rows", C.c_int32), ("n_vocab", C.c_int32), ("x_dtype", C.c_int32),
+                ("shift", C.c_int32)] + [(f + "_pitch", C.c_int64) for f in
+                                         ("x", "u", "t", "k", "p", "mp", "token", "lp", "kept")]
+
+
 class R3dLogits(C.Structure):
     _fields_ = [("x", C.c_void_p), ("codes", C.c_void_p), ("scale", C.c_void_p),
                 ("y", C.c_void_p),

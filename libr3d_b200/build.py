@@ -27,6 +27,7 @@ SOURCES = [
     "entries_band.cpp",
     "entries_logits.cpp",
     "entries_w2a8.cpp",
+    "entries_i8.cpp",
     "planes_cache.cpp",
     "launch.cu",
     "kern_exact.cu",
@@ -34,6 +35,7 @@ SOURCES = [
     "kern_rerank.cu",
     "kern_w2a8.cu",
     "kern_q8x.cu",
+    "kern_i8.cu", "kern_token_i8.cu", "kern_nucleus.cu",
     "q8x_static.cu",
     "kern_stream.cu",
     "kern_tc.cu", "kern_tc_mxf4.cu", "kern_tc_q8x.cu", "kern_tc_gemm.cu", "kern_tc_gemm2.cu", "gather.cu",

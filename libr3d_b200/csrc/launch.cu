@@ -332,3 +332,28 @@ extern "C" int r3d_b200_gated_quant_fp8(const void* gu, int64_t gu_pitch, void* 
     return launch_gated_quant_fp8(gu, gu_pitch, q, q_pitch, scale, s_pitch, ob, ob_dtype, ob_pitch, rows, n,
                                   group, silu, (cudaStream_t)stream);
 }
+
+/* gemm_nt_q @ i8a8. AUTO: the dp4a tile kernel. */
+extern "C" int r3d_b200_gemm_i8a8(const R3dGemmI8* q, void* stream) {
+    if (!q) return RAD_E_INVAL;
+    if (q->m <= 0 || q->n <= 0 || q->k <= 0 || q->k > 131071) return RAD_E_SHAPE;
+    if ((q->bs_dtype != RAD_F32 && q->bs_dtype != RAD_BF16) || (q->y_dtype != RAD_F32 && q->y_dtype != RAD_BF16)) return RAD_E_DTYPE;
+    if (!device_is_sm100()) return RAD_E_UNSUPPORTED;
+    if (q->arm != R3D_ARM_AUTO && q->arm != R3D_ARM_EXACT) return RAD_E_UNSUPPORTED;
+    debug_arm("i8a8", "dp4a tiles", q->m);
+    return i8_tile(*q, (cudaStream_t)stream);
+}
+
+extern "C" int r3d_b200_token_i8(const R3dTokenI8* q, void* stream) {
+    if (!q || !q->x || !q->q || !q->scale || (q->kind == R3D_TOKEN_RMSNORM && !q->w)) return RAD_E_INVAL;
+    if (q->rows <= 0 || q->n <= 0) return RAD_E_SHAPE;
+    if (!device_is_sm100()) return RAD_E_UNSUPPORTED;
+    return launch_token_i8(*q, (cudaStream_t)stream);
+}
+
+extern "C" int r3d_b200_sample_nucleus(const R3dNucleus* q, void* stream) {
+    if (!q || !q->logits || !q->u || !q->token) return RAD_E_INVAL;
+    if (q->rows <= 0 || q->n_vocab <= 0) return RAD_E_SHAPE;
+    if (!device_is_sm100()) return RAD_E_UNSUPPORTED;
+    return launch_nucleus(*q, (cudaStream_t)stream);
+}

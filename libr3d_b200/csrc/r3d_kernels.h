@@ -47,6 +47,12 @@ int launch_logit_rerank_e4m3(const void* x, int xdt, int64_t x_rs, const void* c
 /* gemm_nt_q @ w2a8 (kern_w2a8.cu) */
 int launch_gemm_w2a8(const R3dW2A8& q, cudaStream_t st);
 
+/* the int8 band: gemm_nt_q @ i8a8 on dp4a (kern_i8.cu, any shape), its producers (kern_token_i8.cu), and the
+ * sampler behind the logits (kern_nucleus.cu) */
+int i8_tile(const R3dGemmI8& p, cudaStream_t st);
+int launch_token_i8(const R3dTokenI8& p, cudaStream_t st);
+int launch_nucleus(const R3dNucleus& p, cudaStream_t st);
+
 /* weight-streaming tensor-core arm (kern_stream.cu); *_ok say whether the arm can take
  * the call's shape and alignment */
 bool stream_fp8a8_ok(const R3dGemmQ& p);

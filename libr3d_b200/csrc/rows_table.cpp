@@ -114,6 +114,38 @@ const RadOperandSpec kArgmaxOperands[] = {
     { "logits", RAD_OPD_IN, 0 }, { "params", RAD_OPD_IN, 0 }, { "token", RAD_OPD_OUT, 0 },
 };
 
+/* ---- ops the reference does not have: the int8 band's producers and the sampler ---- */
+const RadParamSpec kTokenI8Params[] = {
+    { "M", RAD_P_INT, RAD_REQUIRED, 0 }, { "n", RAD_P_INT, RAD_REQUIRED, 0 }, { "dtype", RAD_P_STR, RAD_REQUIRED, 0 },
+};
+const RadOperandSpec kTokenI8Operands[] = {
+    { "x", RAD_OPD_IN, 0 }, { "q", RAD_OPD_OUT, 0 }, { "scale", RAD_OPD_OUT, 0 },
+};
+const RadParamSpec kGatedTokenI8Params[] = {
+    { "M", RAD_P_INT, RAD_REQUIRED, 0 },     { "n", RAD_P_INT, RAD_REQUIRED, 0 },
+    { "dtype", RAD_P_STR, RAD_REQUIRED, 0 }, { "act", RAD_P_STR, RAD_OPTIONAL, 0 },
+};
+const RadOperandSpec kGatedTokenI8Operands[] = {
+    { "gate_up", RAD_OPD_IN, 0 }, { "q", RAD_OPD_OUT, 0 }, { "scale", RAD_OPD_OUT, 0 }, { "out", RAD_OPD_OUT, 1 },
+};
+const RadParamSpec kRmsTokenI8Params[] = {
+    { "M", RAD_P_INT, RAD_REQUIRED, 0 },     { "n", RAD_P_INT, RAD_REQUIRED, 0 },
+    { "eps", RAD_P_F64, RAD_REQUIRED, 0 },   { "dtype", RAD_P_STR, RAD_REQUIRED, 0 },
+    { "wadd", RAD_P_F64, RAD_OPTIONAL, 0 },
+};
+const RadOperandSpec kRmsTokenI8Operands[] = {
+    { "x", RAD_OPD_IN, 0 },  { "residual", RAD_OPD_INOUT, 1 }, { "w", RAD_OPD_WEIGHT, 0 },
+    { "q", RAD_OPD_OUT, 0 }, { "scale", RAD_OPD_OUT, 0 },      { "out", RAD_OPD_OUT, 1 },
+};
+const RadParamSpec kNucleusParams[] = {
+    { "M", RAD_P_INT, RAD_REQUIRED, 0 }, { "n_vocab", RAD_P_INT, RAD_REQUIRED, 0 }, { "dtype", RAD_P_STR, RAD_REQUIRED, 0 },
+};
+const RadOperandSpec kNucleusOperands[] = {
+    { "logits", RAD_OPD_IN, 0 }, { "u", RAD_OPD_IN, 0 },       { "temperature", RAD_OPD_IN, 1 },
+    { "top_k", RAD_OPD_IN, 1 },  { "top_p", RAD_OPD_IN, 1 },   { "min_p", RAD_OPD_IN, 1 },
+    { "token", RAD_OPD_OUT, 0 }, { "logprob", RAD_OPD_OUT, 1 }, { "kept", RAD_OPD_OUT, 1 },
+};
+
 const RadOpSchema kSchemas[] = {
     { "logit_rerank", kRerankParams, COUNT_OF(kRerankParams), kRerankOperands, COUNT_OF(kRerankOperands),
       "R candidate ids a row rescored exactly against the full-precision head and re-sorted on those "
@@ -147,6 +179,18 @@ const RadOpSchema kSchemas[] = {
       COUNT_OF(kGemmQGatedOperands),
       "gemm_nt_q over a [2n, K] gate_up plane with the gated activation quantiser folded into "
       "the epilogue; outputs are [M, N/2]." },
+    { "quant_token_i8", kTokenI8Params, COUNT_OF(kTokenI8Params), kTokenI8Operands, COUNT_OF(kTokenI8Operands),
+      "symmetric int8 quantisation of a token-major activation, one scale a token: scale = amax / 127, a "
+      "dequantisation multiplier." },
+    { "gated_quant_token_i8", kGatedTokenI8Params, COUNT_OF(kGatedTokenI8Params), kGatedTokenI8Operands,
+      COUNT_OF(kGatedTokenI8Operands),
+      "silu(gate)*up or sigmoid(gate)*up over a [M, 2n] gate_up plane, held in f32, then the same quantiser." },
+    { "rmsnorm_quant_token_i8", kRmsTokenI8Params, COUNT_OF(kRmsTokenI8Params), kRmsTokenI8Operands,
+      COUNT_OF(kRmsTokenI8Operands),
+      "RMS norm (optionally after a residual add that is stored back), held in f32, then the same quantiser." },
+    { "sample_nucleus", kNucleusParams, COUNT_OF(kNucleusParams), kNucleusOperands, COUNT_OF(kNucleusOperands),
+      "one token a row by temperature, top-k, top-p and min-p from a given number in [0, 1); a temperature of 0 is "
+      "greedy; -inf and NaN logits are masked, a row with nothing left reports -1." },
 };
 
 /* ------------------------------------------------------------------ constraints */
@@ -352,6 +396,36 @@ const RadKernelInfo kRows[] = {
         kPrioPlain, kCArgmax, r3d_rad_sample_argmax, r3d_rad_sample_argmax_scratch),
 };
 
+/* ------------------------------------------------------------------ extension rows */
+const RadConstraint kCI8[] = {
+    { "dtype", RAD_C_IN, 0, "i8a8" }, { "K", RAD_C_GE, 1, nullptr }, { "K", RAD_C_LE, 131071, nullptr },
+};
+const RadConstraint kCNucleus[] = { { "n_vocab", RAD_C_GE, 1, nullptr }, { "dtype", RAD_C_IN, 0, "f32 bf16" } };
+
+const RadKernelInfo kExtRows[] = {
+    ROW("gemm_nt_q_i8a8", "gemm_nt_q", "gemm",
+        "i8a8, any M: int8 codes into exact 32-bit sums over the whole of K, one scale a token and one a channel",
+        "K at most 131071; any N; M from numel(y)/N",
+        "int8 a + f32 a_scale [M], int8 b + f32/bf16 b_scale [N], bf16/f32 y; a_sum and b_ref refused",
+        kPrioPlain, kCI8, r3d_rad_gemm_nt_q_i8),
+    ROW("quant_token_i8_act", "quant_token_i8", "band",
+        "per-token symmetric int8 quantisation, one block a row",
+        "f32/bf16 input, any width", "activation in, int8 codes and f32 scales out",
+        kPrioPlain, kCBand, r3d_rad_quant_token_i8),
+    ROW("gated_quant_token_i8_act", "gated_quant_token_i8", "band",
+        "silu(gate)*up (or sigmoid(gate)*up) in f32 and the per-token quantiser in one pass",
+        "f32/bf16 gate_up [M, 2n], gate half first, any width", "gate_up in, int8 codes, f32 scales, optional bf16/f32 product",
+        kPrioPlain, kCBand, r3d_rad_gated_quant_token_i8),
+    ROW("rmsnorm_quant_token_i8", "rmsnorm_quant_token_i8", "quant",
+        "residual add, RMS norm and the per-token quantiser in one pass; the norm's output stays in f32",
+        "any width", "f32/bf16 x (+ residual of x's type), f32/bf16 w, int8 codes, f32 scales, optional bf16/f32 norm output",
+        kPrioPlain, kCBand, r3d_rad_rmsnorm_quant_token_i8),
+    ROW("sample_nucleus_row", "sample_nucleus", "sample",
+        "temperature, top-k, top-p and min-p over exact fixed-point weights, then the given number's token in id order",
+        "any vocabulary", "f32/bf16 logits, f32/i32 per-row parameters, i32 token, optional f32 logprob and i32 count",
+        kPrioPlain, kCNucleus, r3d_rad_sample_nucleus),
+};
+
 /* ------------------------------------------------------------------ registration gate */
 bool row_hidden(const RadKernelInfo& k) {
     static const bool no_fp8 = getenv("R3D_NO_FP8A8") != nullptr;
@@ -369,7 +443,16 @@ bool row_hidden(const RadKernelInfo& k) {
     if (!strcmp(k.name, "gemm_nt_q_mxfp4_decode")) return no_mx || no_mx_dec;
     /* the q8x sibling rides every lever of its band, plus its own */
     if (!strcmp(k.name, "gemm_nt_q_mxfp4_decode_q8x")) return no_mx || no_mx_dec || q8x_off;
+    static const bool no_i8 = getenv("R3D_NO_I8A8") != nullptr;
+    static const bool no_nucleus = getenv("R3D_NO_NUCLEUS") != nullptr;
+    if (!strcmp(k.op, "sample_nucleus")) return no_nucleus;
+    if (!strcmp(k.name, "gemm_nt_q_i8a8") || strstr(k.op, "token_i8")) return no_i8;
     return false;
+}
+/* R3D_EXT_ROWS: the loader's table carries the extension rows behind the reference's */
+bool ext_in_table() {
+    static const bool on = getenv("R3D_EXT_ROWS") != nullptr;
+    return on;
 }
 
 } /* namespace */
@@ -393,8 +476,20 @@ const RadOpSchema* rad_kernel_schema_at(int i) {
     return (i >= 0 && i < COUNT_OF(kSchemas)) ? &kSchemas[i] : nullptr;
 }
 
-int rad_kernel_count(void) {
+int r3d_b200_ext_kernel_count(void) {
     int n = 0;
+    for (const RadKernelInfo& k : kExtRows) if (!row_hidden(k)) ++n;
+    return n;
+}
+const RadKernelInfo* r3d_b200_ext_kernel_at(int i) {
+    if (i < 0) return nullptr;
+    for (const RadKernelInfo& k : kExtRows)
+        if (!row_hidden(k) && i-- == 0) return &k;
+    return nullptr;
+}
+
+int rad_kernel_count(void) {
+    int n = ext_in_table() ? r3d_b200_ext_kernel_count() : 0;
     for (const RadKernelInfo& k : kRows) if (!row_hidden(k)) ++n;
     return n;
 }
@@ -402,7 +497,7 @@ const RadKernelInfo* rad_kernel_at(int i) {
     if (i < 0) return nullptr;
     for (const RadKernelInfo& k : kRows)
         if (!row_hidden(k) && i-- == 0) return &k;
-    return nullptr;
+    return ext_in_table() ? r3d_b200_ext_kernel_at(i) : nullptr;
 }
 
 } /* extern "C" */

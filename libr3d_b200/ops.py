@@ -7,6 +7,8 @@ current CUDA stream. Nothing is computed here.
 """
 from __future__ import annotations
 
+import ctypes as C
+import threading
 from typing import Any
 
 import torch
@@ -270,6 +272,147 @@ def sample_argmax(logits: torch.Tensor, token: torch.Tensor, params: torch.Tenso
     return _issue("sample_argmax", query, [_desc(logits, abi.RAD_F32), _desc(params, abi.RAD_U8),
                                            _desc(token, abi.RAD_I32)],
                   plugin().lib.r3d_rad_sample_argmax_scratch, logits.device)
+
+
+# ---------------------------------------------------------------------- the int8 band and its sampler
+_RAD_OF = {torch.float32: abi.RAD_F32, torch.bfloat16: abi.RAD_BF16, torch.int8: abi.RAD_I8, torch.int32: abi.RAD_I32}
+_NAME_OF = {torch.float32: "f32", torch.bfloat16: "bf16"}
+_tls = threading.local()
+
+
+class _Declared:
+    """An op declared for one set of shapes, strides, types and parameters: the resolved row and its RadArgs, in
+    which a call only writes its operands' addresses. One per thread, as a call fills it in."""
+
+    def __init__(self, op: str, query: dict, tensors: tuple):
+        P = plugin()
+        self.row = P.resolve(op, query)
+        if self.row is None:
+            raise RuntimeError(f"no row serves {op} {query}")
+        self.pack = ArgPack([_desc(t, abi.RAD_F32 if t is None else _RAD_OF[t.dtype]) for t in tensors], query)
+        self.slots = [self.pack.t[i] for i in range(len(tensors))]
+        self.argp = C.byref(self.pack.args)
+        self.fn = P._launch_t(self.row.launch)
+
+
+def _run(op: str, params: tuple, tensors: tuple) -> Row:
+    """One call of `op` on the operands' device, on that device's current stream. `params`: (key, value) pairs;
+    `tensors`: by schema position, None where an optional one is absent."""
+    key = (op, params, *[None if t is None else (t.dtype, t.shape, t.stride(), t.get_device()) for t in tensors])
+    try:
+        declared = _tls.declared
+    except AttributeError:
+        declared = _tls.declared = {}
+    d = declared.get(key)
+    if d is None:
+        for t in tensors:
+            if t is not None and t.dtype not in _RAD_OF:
+                raise TypeError(f"{op}: no {t.dtype} operands")
+        if len({t.get_device() for t in tensors if t is not None}) > 1 or not tensors[0].is_cuda:
+            raise ValueError(f"{op}: operands on one CUDA device are needed, got {[t.device for t in tensors if t is not None]}")
+        if len(declared) >= 1024:                   # shapes that keep changing: start over
+            declared.clear()
+        d = declared[key] = _Declared(op, dict(params), tensors)
+    for slot, t in zip(d.slots, tensors):
+        if t is not None:
+            slot.data = t.data_ptr()
+    dev = tensors[0].get_device()
+    if dev == torch.cuda.current_device():
+        rc = d.fn(d.argp, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = d.fn(d.argp, torch.cuda.current_stream(dev).cuda_stream)
+    if rc != abi.RAD_OK:
+        raise RowRefused(d.row.name, rc)
+    return d.row
+
+
+def gemm_i8a8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+              y: torch.Tensor | None = None, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """y[..., N] = (sum_k a[..., k] * b[n, k]) * a_scale[...] * b_scale[n]: int8 codes [..., K] and [N, K], one f32
+    scale a token ([...] or [..., 1]) and one f32 or bf16 scale a channel ([N] or [N, 1]). The sum is exact (K at
+    most 131071), the result is rounded once, to `out_dtype` (bf16 or f32), or to y's type where y is given."""
+    K, N = a.shape[-1], b.shape[0]
+    if y is None:
+        y = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=a.device)
+    if a.dim() > 0 and a.numel() == 0 and K and y.numel() == 0:
+        return y                                    # no tokens
+    _run("gemm_nt_q", (("M", y.numel() // max(N, 1)), ("N", N), ("K", K), ("group", K), ("dtype", "i8a8")),
+         (a, a_scale, b, b_scale, y, None, None))
+    return y
+
+
+def _codes_for(x: torch.Tensor, n: int, q: torch.Tensor | None, scale: torch.Tensor | None):
+    if q is None:
+        q = torch.empty((*x.shape[:-1], n), dtype=torch.int8, device=x.device)
+    if scale is None:
+        scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
+    return q, scale
+
+
+def _act_name(op: str, x: torch.Tensor) -> str:
+    if x.dtype not in _NAME_OF:
+        raise TypeError(f"{op}: bf16 or f32 activations, got {x.dtype}")
+    return _NAME_OF[x.dtype]
+
+
+def quant_token_i8(x: torch.Tensor, q: torch.Tensor | None = None,
+                   scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16/f32 activations [..., n] -> int8 codes [..., n] and one f32 scale a token [..., 1]:
+    scale = max|x| / 127, q = rint(x * (127 / max|x|)); a row of zeros has scale 1."""
+    n = x.shape[-1]
+    q, scale = _codes_for(x, n, q, scale)
+    if x.numel() or not n:
+        _run("quant_token_i8", (("M", x.numel() // max(n, 1)), ("n", n), ("dtype", _act_name("quant_token_i8", x))), (x, q, scale))
+    return q, scale
+
+
+def gated_quant_token_i8(gate_up: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                         out: torch.Tensor | None = None, *, act: str = "silu") -> tuple[torch.Tensor, torch.Tensor]:
+    """silu(gate) * up (act "sigmoid": sigmoid(gate) * up) of gate_up [..., 2n], gate half first, quantised per token
+    as by quant_token_i8 from its f32 values; `out` (bf16 or f32 [..., n]) receives the product itself."""
+    n = gate_up.shape[-1] // 2
+    q, scale = _codes_for(gate_up, n, q, scale)
+    if gate_up.numel() or not n:
+        _run("gated_quant_token_i8", (("M", gate_up.numel() // max(2 * n, 1)), ("n", n),
+                                      ("dtype", _act_name("gated_quant_token_i8", gate_up)), ("act", act)), (gate_up, q, scale, out))
+    return q, scale
+
+
+def rmsnorm_quant_token_i8(x: torch.Tensor, w: torch.Tensor, q: torch.Tensor | None = None,
+                           scale: torch.Tensor | None = None, *, eps: float, residual: torch.Tensor | None = None,
+                           out: torch.Tensor | None = None, wadd: float = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """x / sqrt(mean(x^2) + eps) * (w + wadd) over [..., n], quantised per token as by quant_token_i8 from its f32
+    values. `residual` (x's type, updated in place with x + residual) selects the fused-add form, whose norm reads
+    the stored sum; `out` (bf16 or f32) receives the norm itself."""
+    n = x.shape[-1]
+    q, scale = _codes_for(x, n, q, scale)
+    if x.numel() or not n:
+        _run("rmsnorm_quant_token_i8",
+             (("M", x.numel() // max(n, 1)), ("n", n), ("eps", float(eps)), ("wadd", float(wadd)),
+              ("dtype", _act_name("rmsnorm_quant_token_i8", x))), (x, residual, w, q, scale, out))
+    return q, scale
+
+
+def sample_nucleus(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor | None = None,
+                   top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+                   min_p: torch.Tensor | None = None, token: torch.Tensor | None = None,
+                   logprob: torch.Tensor | None = None, kept: torch.Tensor | None = None) -> torch.Tensor:
+    """One token a row of logits (f32 or bf16 [..., n_vocab]) from the row's number u in [0, 1) -> int32 [...].
+
+    Tokens are ordered by logit, ties to the lower id. top_k (int32) keeps the first k (k <= 0: all), top_p the
+    shortest first part that holds p of what top_k left (p >= 1: all), min_p those at least min_p times as likely as
+    the first; the first always stays. The answer is the first kept id, ascending, at which the running share of the
+    kept probability exceeds u. temperature <= 0 is greedy. Every parameter is a plane with one value a row (f32
+    but for top_k), or None. -inf and NaN logits are masked; a row with nothing left reports -1.
+    `logprob` (f32) receives the log of the token's share of what was kept, `kept` (int32) how many tokens were."""
+    V = logits.shape[-1]
+    if token is None:
+        token = torch.empty(logits.shape[:-1], dtype=torch.int32, device=logits.device)
+    if logits.numel() or not V:
+        _run("sample_nucleus", (("M", logits.numel() // max(V, 1)), ("n_vocab", V), ("dtype", _act_name("sample_nucleus", logits))),
+             (logits, u, temperature, top_k, top_p, min_p, token, logprob, kept))
+    return token
 
 
 class BoundGemm:

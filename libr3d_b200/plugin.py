@@ -39,6 +39,9 @@ EXPORTS = [
     "r3d_b200_gather_create", "r3d_b200_gather_connect", "r3d_b200_gather_buffer", "r3d_b200_gather_wait",
     "r3d_b200_gather_status", "r3d_b200_gather_destroy", "r3d_b200_gather_connect_ptr", "r3d_b200_gather_base", "r3d_b200_gemm_mxfp4a8_push",
     "r3d_b200_gemm_fp8a8_push", "r3d_b200_logits_push",
+    "r3d_b200_ext_kernel_count", "r3d_b200_ext_kernel_at", "r3d_rad_gemm_nt_q_i8", "r3d_rad_quant_token_i8",
+    "r3d_rad_gated_quant_token_i8", "r3d_rad_rmsnorm_quant_token_i8", "r3d_rad_sample_nucleus",
+    "r3d_b200_gemm_i8a8", "r3d_b200_token_i8", "r3d_b200_sample_nucleus",
 ]
 
 
@@ -121,6 +124,11 @@ class Plugin:
         L.r3d_b200_gather_connect_ptr.argtypes = [C.c_void_p, C.c_int, C.c_void_p]
         L.r3d_b200_gather_base.argtypes = [C.c_void_p]
         L.r3d_b200_gather_base.restype = C.c_void_p
+        L.r3d_b200_ext_kernel_at.restype = C.POINTER(abi.RadKernelInfo)
+        L.r3d_b200_ext_kernel_at.argtypes = [C.c_int]
+        L.r3d_b200_gemm_i8a8.argtypes = [C.POINTER(abi.R3dGemmI8), C.c_void_p]
+        L.r3d_b200_token_i8.argtypes = [C.POINTER(abi.R3dTokenI8), C.c_void_p]
+        L.r3d_b200_sample_nucleus.argtypes = [C.POINTER(abi.R3dNucleus), C.c_void_p]
         for f in ("r3d_b200_gemm_mxfp4a8_push", "r3d_b200_gemm_fp8a8_push"):
             getattr(L, f).argtypes = [C.POINTER(abi.R3dGemmQ), C.c_void_p, C.c_int, C.c_int64, C.c_void_p]
         L.r3d_b200_logits_push.argtypes = [C.POINTER(abi.R3dLogits), C.c_void_p, C.c_int, C.c_int64, C.c_void_p]
@@ -149,9 +157,18 @@ class Plugin:
         return out
 
     def rows(self) -> list[Row]:
+        """The loader's table: the reference's rows (and the extension rows under R3D_EXT_ROWS)."""
+        return self._rows(self.lib.rad_kernel_count(), self.lib.rad_kernel_at)
+
+    def ext_rows(self) -> list[Row]:
+        """The rows of ops the reference does not have."""
+        return self._rows(self.lib.r3d_b200_ext_kernel_count(), self.lib.r3d_b200_ext_kernel_at)
+
+    @staticmethod
+    def _rows(count: int, at) -> list[Row]:
         out = []
-        for k in range(self.lib.rad_kernel_count()):
-            r = self.lib.rad_kernel_at(k).contents
+        for k in range(count):
+            r = at(k).contents
             cons = [(r.constraints[j].key.decode(), r.constraints[j].op, r.constraints[j].ival,
                      r.constraints[j].sval.decode() if r.constraints[j].sval else None)
                     for j in range(r.n_constraints)]
@@ -161,9 +178,9 @@ class Plugin:
 
     def resolve(self, op: str, query: dict[str, Any]) -> Row | None:
         """The row a band with these parameters lands on: all constraints hold, highest
-        priority wins, first declared breaks ties."""
+        priority wins, first declared breaks ties. Extension rows stand behind the loader's."""
         best = None
-        for r in self.rows():
+        for r in self.rows() + self.ext_rows():
             if r.op != op or not all(_holds(c, query) for c in r.constraints):
                 continue
             if best is None or r.priority > best.priority:
