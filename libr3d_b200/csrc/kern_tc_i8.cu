@@ -1,0 +1,578 @@
+/* kern_tc_i8.cu -- gemm_nt_q @ i8a8 on the tensor core (tcgen05 kind::i8, 32-bit integer accumulators in tensor
+ * memory): y[m, n] = (float(sum_k a[m, k] b[n, k]) * sa[m]) * sb[n]. The sum over the whole of K is one exact
+ * accumulation, so the result does not depend on tiles, splits or order, and the scales are two multiplies at the end.
+ *
+ * Tokens lie on the MMA's M axis (tensor-memory lanes), channels on its N axis (columns): a thread of the epilogue
+ * owns a token, whose channels lie next to each other in registers as they do in y, and the channel tile can be any
+ * multiple of 16, which is what balances a wave over 148 SMs.
+ *
+ * k_i8_stream (M <= 128): bound by the weights' bytes. One CTA a channel tile, the channel tile chosen so that the
+ *   tiles fill the device's slots (27648 channels: 288 tiles of 96 on 296 slots), a deep TMA ring; rows of the token
+ *   tile past M are whatever shared memory holds, their lanes are never read. Where channels alone do not fill the
+ *   device, the CTAs of a cluster split K and add their 32-bit sums through distributed shared memory.
+ *
+ * k_i8_pair (M > 128): bound by the tensor pipe and by the operands' way from L2 into shared memory. CTA pairs
+ *   (cta_group::2), 256 tokens x 512 channels a pair: 96 KiB of operands for 2 x 256 x 512 x 128 operations, two
+ *   thirds of what 256 x 256 tiles fetch. The 512 accumulator columns fill tensor memory, so its two halves run
+ *   `kLag` K steps apart: while one half is drained, the other half's MMAs still run. Persistent, 74 pairs.
+ *
+ * Every wait is bounded; on expiry a status word is set and the CTA drains and leaves.
+ */
+#include <cstdio>
+#include <cstdlib>
+#include <cstring>
+#define R3D_TC_STATUS_WORD ::r3d::g_tci8_status
+namespace r3d { __device__ int g_tci8_status = 0; }
+#include "tc_common.cuh"
+
+namespace r3d {
+
+namespace {
+using namespace tcdev;
+
+constexpr int kStageK = 128;                       /* K bytes of a stage: one 128-byte swizzle row */
+
+struct I8Params {
+    const float* as; int64_t as_pitch;
+    const void* ws; int64_t ws_pitch; int ws_dtype;
+    void* y; int64_t y_pitch; int y_f32;
+    int m, n, nk;                                  /* nk: K stages */
+    int nt;                                        /* channels of a tile */
+    int tok_tiles, ch_tiles, tiles, workers, group;
+    int mb, stages, shares, tma_store;
+};
+
+/* kind::i8: s32 accumulators (2 at bit 4), a and b signed (1 at bits 7 and 10), N >> 3 at bit 17, M >> 4 at bit 24 */
+__device__ __forceinline__ uint32_t i8_idesc(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+template <int CG>
+__device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if (CG == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ uint32_t mapa_u32(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void umma2_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+/* pins uses of the loaded registers behind tcgen05.wait::ld */
+template <int N>
+__device__ __forceinline__ void pin_u32(uint32_t* r) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+__device__ __forceinline__ float scaled(uint32_t sum, float sa, float sb) { return __fmul_rn(__fmul_rn((float)(int)sum, sa), sb); }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float channel_scale(const I8Params& P, int n) {
+    return n < P.n ? ld_scale((const uint8_t*)P.ws, (int64_t)n * P.ws_pitch, P.ws_dtype) : 0.0f;
+}
+
+/* barrier `id` of 128 threads; true where all of them came with true */
+__device__ __forceinline__ bool group_and(int id, bool v) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\t"
+                 "barrier.cta.red.and.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(id), "r"((uint32_t)v) : "memory");
+    return r != 0;
+}
+
+/* ------------------------------------------------------------------ M > 128: CTA pairs */
+constexpr int kTokC = 128;                         /* tokens of a CTA; a pair has 256 */
+constexpr int kHalf = 256;                         /* accumulator columns of a half */
+constexpr int kLag = 2;                            /* K stages between the halves of a 512-channel tile */
+constexpr int kOpBytes = 128 * kStageK;            /* one operand tile of a stage: 128 rows, 16 KiB */
+constexpr int kPairThreads = 32 * 10;
+constexpr int kStoreBytes = 32 * 128;              /* a warp's staging tile: 32 tokens x 128 bytes */
+
+template <int NH> struct Pair {
+    static constexpr int stages = NH == 2 ? 4 : 6, stage = (1 + NH) * kOpBytes;
+    static constexpr size_t smem = (size_t)stages * stage + 8 * kStoreBytes + 2 * kHalf * sizeof(float) + 256;
+};
+static_assert(Pair<1>::smem <= 232448 && Pair<2>::smem <= 232448, "shared memory of a CTA");
+
+/* tile -> (token tile, channel tile): blocks of `group` token tiles walk the channels, so that the tiles in flight
+ * share both operands in L2 */
+__device__ __forceinline__ void place(const I8Params& P, int tile, int* tt, int* ct) {
+    const int block = P.group * P.ch_tiles, b = tile / block, r = tile - b * block;
+    const int here = min(P.group, P.tok_tiles - b * P.group);
+    *ct = r / here;
+    *tt = b * P.group + r % here;
+}
+
+template <int NH>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+          const __grid_constant__ CUtensorMap tmY, const I8Params P) {
+    constexpr int kStages = Pair<NH>::stages, kStage = Pair<NH>::stage;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* staging = smem + kStages * kStage;
+    float* sb_s = (float*)(staging + 8 * kStoreBytes);            /* [2][kHalf] channel scales of the half in each buffer */
+    uint64_t* full = (uint64_t*)(sb_s + 2 * kHalf);
+    uint64_t* empty = full + kStages;
+    uint64_t* acc_full = empty + kStages;
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t crank = cluster_rank();
+    const bool leader = crank == 0;
+    const int pair = blockIdx.x >> 1;
+    const int nk = P.nk, bc = P.nt / 2;                           /* bc: channels of a half that this CTA loads */
+    bool alive = (smem_u32(smem) & 1023u) == 0;                   /* the operand tiles' swizzle needs it */
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 8); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (!alive) atomicExch(&R3D_TC_STATUS_WORD, 90);
+    }
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    dep_launch();
+    dep_wait();
+
+    if (warp == 0) {
+        /* ---------------- TMA producer: this CTA's half of both operands ---------------- */
+        if (elect_one()) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&tmB) : "memory");
+            const uint32_t bytes = 2u * (uint32_t)(kTokC + NH * bc) * kStageK;
+            int s = 0; uint32_t ph = 0;
+            for (int tile = pair; tile < P.tiles && alive; tile += P.workers) {
+                int tt, ct;
+                place(P, tile, &tt, &ct);
+                const int t0 = tt * 2 * kTokC + (int)crank * kTokC, n0 = ct * NH * P.nt + (int)crank * bc;
+                for (int it = 0; it < nk; ++it) {
+                    if (!mbar_wait(&empty[s], ph ^ 1u, 91)) { alive = false; break; }
+                    const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0u);
+                    if (leader) mbar_expect_tx(&full[s], bytes);
+                    const uint32_t st = smem_u32(smem + s * kStage);
+                    tma_load_2d_pair(st, &tmA, it * kStageK, t0, bar);
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) tma_load_2d_pair(st + (1 + h) * kOpBytes, &tmB, it * kStageK, n0 + h * P.nt, bar);
+                    if (++s == kStages) { s = 0; ph ^= 1u; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        /* ---------------- MMA issuer (the pair's leader only) ---------------- */
+        if (leader && elect_one()) {
+            const uint32_t idesc = i8_idesc(2 * kTokC, P.nt);
+            const auto mma = [&](int s, int h, int buf, bool first) {
+                const uint32_t a0 = smem_u32(smem + s * kStage), b0 = a0 + (1 + h) * kOpBytes;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_i8<2>(tmem_base + buf * kHalf, smem_desc_sw128(a0 + k * 32), smem_desc_sw128(b0 + k * 32), idesc, first && !k ? 0u : 1u);
+            };
+            const auto release = [&](uint64_t* bar) {
+                umma2_commit(smem_u32(bar));
+                umma2_commit(mapa_u32(smem_u32(bar), 1u));
+            };
+            int s = 0; uint32_t ph = 0;                           /* the stage half 0 (or the tile) reads next */
+            int s1 = 0;                                           /* the stage half 1 reads next */
+            int job = 0;                                          /* NH 1: tile count of this pair */
+            uint32_t aph = 0;
+            for (int tile = pair; tile < P.tiles && alive; tile += P.workers) {
+                if (NH == 1) {
+                    const int buf = job & 1;
+                    if (!mbar_wait(&acc_empty[buf], ((uint32_t)(job >> 1) & 1u) ^ 1u, 92)) { alive = false; break; }
+                    tc_fence_after();
+                    for (int it = 0; it < nk; ++it) {
+                        if (!mbar_wait(&full[s], ph, 93)) { alive = false; break; }
+                        tc_fence_after();
+                        mma(s, 0, buf, it == 0);
+                        release(&empty[s]);
+                        if (++s == kStages) { s = 0; ph ^= 1u; }
+                    }
+                    if (alive) release(&acc_full[buf]);
+                    ++job;
+                } else {
+                    for (int it = 0; it < nk + kLag && alive; ++it) {
+                        if (it < nk) {
+                            if (it == 0 && !mbar_wait(&acc_empty[0], aph ^ 1u, 94)) { alive = false; break; }
+                            if (!mbar_wait(&full[s], ph, 95)) { alive = false; break; }
+                            tc_fence_after();
+                            mma(s, 0, 0, it == 0);
+                            if (it == nk - 1) release(&acc_full[0]);
+                            if (++s == kStages) { s = 0; ph ^= 1u; }
+                        }
+                        if (it >= kLag) {
+                            if (it == kLag) {
+                                if (!mbar_wait(&acc_empty[1], aph ^ 1u, 96)) { alive = false; break; }
+                                tc_fence_after();
+                            }
+                            mma(s1, 1, 1, it == kLag);
+                            release(&empty[s1]);
+                            if (it == nk + kLag - 1) release(&acc_full[1]);
+                            if (++s1 == kStages) s1 = 0;
+                        }
+                    }
+                    aph ^= 1u;
+                }
+            }
+        }
+    } else {
+        /* ---------------- epilogue: thread = token; warps 2-5 drain buffer 0, warps 6-9 buffer 1 ---------------- */
+        const int q = warp & 3, g = (warp - 2) >> 2, et = threadIdx.x - 64 - 128 * g;
+        const uint32_t ta = tmem_base + ((uint32_t)(q * 32) << 16) + g * kHalf;
+        const uint32_t acc_empty_leader = mapa_u32(smem_u32(&acc_empty[g]), 0u);
+        uint8_t* const out = staging + (warp - 2) * kStoreBytes;
+        float* const sb = sb_s + g * kHalf;
+        const int esz = P.y_f32 ? 4 : 2, cols = 128 / esz;        /* channels of a 128-byte staging row */
+        uint32_t aph = 0;
+        int job = 0;
+        for (int tile = pair; tile < P.tiles && alive; tile += P.workers, ++job) {
+            if (NH == 1 && (job & 1) != g) continue;
+            int tt, ct;
+            place(P, tile, &tt, &ct);
+            const int tw = tt * 2 * kTokC + (int)crank * kTokC + q * 32, t = tw + lane;
+            const int n0 = (ct * NH + (NH == 2 ? g : 0)) * P.nt;
+            for (int i = et; i < P.nt; i += 128) sb[i] = channel_scale(P, n0 + i);
+            const float sa = t < P.m ? __ldg(P.as + (int64_t)t * P.as_pitch) : 0.0f;
+            /* one answer for the four warps: they meet at a barrier again below */
+            alive = group_and(1 + g, mbar_wait(&acc_full[g], aph, 97));
+            if (!alive) break;
+            tc_fence_after();
+            aph ^= 1u;
+            const bool live = tw < P.m;                           /* the warp has tokens at all */
+#pragma unroll 1
+            for (int c = 0; c < P.nt && live; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(ta + c, r);
+                tmem_ld_wait();
+                pin_u32<32>(r);
+                if (c % cols == 0) {                              /* the staging tile's last store has read it */
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    __syncwarp();
+                }
+                uint4* row = (uint4*)(out + lane * 128);
+                if (P.y_f32) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float4 w = *(const float4*)(sb + c + 4 * j);
+                        row[j ^ (lane & 7)] = make_uint4(__float_as_uint(scaled(r[4 * j], sa, w.x)), __float_as_uint(scaled(r[4 * j + 1], sa, w.y)),
+                                                         __float_as_uint(scaled(r[4 * j + 2], sa, w.z)), __float_as_uint(scaled(r[4 * j + 3], sa, w.w)));
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float4 w = *(const float4*)(sb + c + 8 * j), v = *(const float4*)(sb + c + 8 * j + 4);
+                        row[(((c >> 5) & 1) * 4 + j) ^ (lane & 7)] = make_uint4(
+                            pack_bf16(scaled(r[8 * j], sa, w.x), scaled(r[8 * j + 1], sa, w.y)), pack_bf16(scaled(r[8 * j + 2], sa, w.z), scaled(r[8 * j + 3], sa, w.w)),
+                            pack_bf16(scaled(r[8 * j + 4], sa, v.x), scaled(r[8 * j + 5], sa, v.y)), pack_bf16(scaled(r[8 * j + 6], sa, v.z), scaled(r[8 * j + 7], sa, v.w)));
+                    }
+                }
+                if ((c + 32) % cols && c + 32 < P.nt) continue;
+                const int cb = c / cols * cols, have = min(c + 32 - cb, P.n - n0 - cb);   /* channels staged and inside y */
+                if (P.tma_store) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0 && have > 0) {
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                                     ::"l"(&tmY), "r"(smem_u32(out)), "r"(n0 + cb), "r"(tw) : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                } else {
+                    __syncwarp();
+                    const int rows = min(32, P.m - tw);
+                    for (int rr = 0; rr < rows; ++rr)
+                        for (int cc = lane; cc < have; cc += 32) {
+                            const int b = cc * esz, at = rr * 128 + ((((b >> 4) ^ (rr & 7)) << 4) | (b & 15));
+                            const int64_t to = (int64_t)(tw + rr) * P.y_pitch + n0 + cb + cc;
+                            if (P.y_f32) ((float*)P.y)[to] = *(const float*)(out + at);
+                            else ((uint16_t*)P.y)[to] = *(const uint16_t*)(out + at);
+                        }
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty_leader);
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");   /* sb is read before the next tile's scales */
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncwarp();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    }
+}
+
+/* ------------------------------------------------------------------ M <= 128: the weights' stream */
+constexpr int kStreamThreads = 32 * 6;
+
+__global__ void __launch_bounds__(kStreamThreads, 1)
+k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const I8Params P) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ uint64_t full[32], empty[32], done;
+    __shared__ uint32_t tmem_slot;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int shares = P.shares, crank = shares > 1 ? (int)cluster_rank() : 0;
+    const int n0 = (int)(blockIdx.x / shares) * P.nt;
+    const int it0 = (int)((int64_t)P.nk * crank / shares), nk = (int)((int64_t)P.nk * (crank + 1) / shares) - it0;
+    const int abytes = P.mb * kStageK, stage = abytes + P.nt * kStageK;
+    const uint32_t cols = P.nt <= 32 ? 32u : P.nt <= 64 ? 64u : P.nt <= 128 ? 128u : 256u;
+    uint8_t* const ring = (uint8_t*)(((uintptr_t)smem + 1023) & ~(uintptr_t)1023);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < P.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_init(&done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_slot;
+    dep_launch();
+    dep_wait();
+
+    bool ok = true;
+    if (warp == 0) {
+        if (elect_one()) {
+            int s = 0; uint32_t ph = 0;
+            for (int it = 0; it < nk; ++it) {
+                if (!mbar_wait(&empty[s], ph ^ 1u, 81)) break;
+                mbar_expect_tx(&full[s], (uint32_t)stage);
+                tma_load_2d(ring + s * stage + abytes, &tmB, (it0 + it) * kStageK, n0, &full[s]);
+                tma_load_2d(ring + s * stage, &tmA, (it0 + it) * kStageK, 0, &full[s]);
+                if (++s == P.stages) { s = 0; ph ^= 1u; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t idesc = i8_idesc(128, P.nt);
+            int s = 0; uint32_t ph = 0;
+            for (int it = 0; it < nk; ++it) {
+                if (!mbar_wait(&full[s], ph, 82)) break;
+                tc_fence_after();
+                const uint32_t a0 = smem_u32(ring + s * stage), b0 = a0 + abytes;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_i8<1>(tmem_base, smem_desc_sw128(a0 + k * 32), smem_desc_sw128(b0 + k * 32), idesc, (it | k) ? 1u : 0u);
+                umma_commit(&empty[s]);
+                if (++s == P.stages) { s = 0; ph ^= 1u; }
+            }
+            umma_commit(&done);
+        }
+        __syncwarp();
+    }
+    /* the sums of the CTA's K share as [token][channel] words over the ring, whose stages are all consumed */
+    ok = mbar_wait(&done, 0, 83);
+    __syncthreads();
+    const int pitch = P.nt + 4;                                   /* 16 bytes on: the lanes' rows fall into different banks */
+    int* const sums = (int*)ring;
+    if (warp >= 2 && ok) {
+        const int q = warp & 3, t = q * 32 + lane;
+        tc_fence_after();
+        if (q * 32 < P.m)
+            for (int c = 0; c < P.nt; c += 16) {
+                float v[16];
+                tmem_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + c, v);
+                tmem_ld_wait();
+                tmem_pin16(v);
+                if (t < P.m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) *(float4*)(sums + t * pitch + c + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            }
+        tc_fence_before();
+    }
+    if (shares > 1) cluster_sync_all(); else __syncthreads();
+    if (ok) {
+        const int all = P.m * P.nt;
+        for (int i = crank * kStreamThreads + (int)threadIdx.x; i < all; i += kStreamThreads * shares) {
+            const int t = i / P.nt, c = i - t * P.nt, n = n0 + c;
+            if (n >= P.n) continue;
+            int sum = 0;
+            if (shares == 1) sum = sums[t * pitch + c];
+            else
+                for (int r = 0; r < shares; ++r) {
+                    int v;
+                    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_u32(smem_u32(sums + t * pitch + c), (uint32_t)r)) : "memory");
+                    sum += v;
+                }
+            const float y = scaled((uint32_t)sum, __ldg(P.as + (int64_t)t * P.as_pitch), channel_scale(P, n));
+            if (P.y_f32) ((float*)P.y)[(int64_t)t * P.y_pitch + n] = y;
+            else ((uint16_t*)P.y)[(int64_t)t * P.y_pitch + n] = f32_to_bf16(y);
+        }
+    }
+    if (shares > 1) cluster_sync_all(); else __syncthreads();    /* peers have read this CTA's sums */
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(cols) : "memory");
+    }
+}
+
+/* ------------------------------------------------------------------ host */
+bool grid16(const void* p, int64_t pitch_bytes) { return (((uintptr_t)p | (uintptr_t)pitch_bytes) & 15) == 0; }
+
+/* made for the call: encoding takes less than a microsecond and nothing outlives the launch */
+bool make_map(CUtensorMap* m, const void* p, uint64_t d0, uint64_t d1, uint64_t pitch, CUtensorMapDataType dt, uint32_t box0, uint32_t box1) {
+    return tc_encode_map(m, p, d0, d1, pitch, dt, box0, box1);
+}
+
+template <typename K, typename... A>
+int launch(K kernel, int grid, int threads, size_t smem, int cluster, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (tc_pdl_on()) { at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; at[n++].val.programmaticStreamSerializationAllowed = 1; }
+    if (cluster > 1) { at[n].id = cudaLaunchAttributeClusterDimension; at[n].val.clusterDim.x = (unsigned)cluster; at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1; ++n; }
+    cfg.attrs = at; cfg.numAttrs = (unsigned)n;
+    count_launch();
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
+}
+
+template <typename K>
+bool allow_smem(K kernel, size_t smem, bool (&set)[kTcMaxDevices]) {
+    const int dev = tc_device();
+    if (dev < 0) return false;
+    if (!set[dev]) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
+        set[dev] = true;
+    }
+    return true;
+}
+
+I8Params params_of(const R3dGemmI8& p) {
+    I8Params P{};
+    P.as = p.a_scale; P.as_pitch = p.as_pitch;
+    P.ws = p.b_scale; P.ws_pitch = p.bs_pitch; P.ws_dtype = p.bs_dtype;
+    P.y = p.y; P.y_pitch = p.y_pitch; P.y_f32 = p.y_dtype == RAD_F32;
+    P.m = p.m; P.n = p.n; P.nk = (p.k + kStageK - 1) / kStageK;
+    return P;
+}
+
+template <int NH>
+int run_pair(const R3dGemmI8& p, I8Params P, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ty, cudaStream_t st) {
+    static bool set[kTcMaxDevices] = {};
+    if (!allow_smem(k_i8_pair<NH>, Pair<NH>::smem, set)) return RAD_E_DEVICE;
+    return launch(k_i8_pair<NH>, 2 * P.workers, kPairThreads, Pair<NH>::smem, 1, st, ta, tb, ty, P);
+}
+
+int tc_i8_pair(const R3dGemmI8& p, cudaStream_t st) {
+    I8Params P = params_of(p);
+    const int pairs = tc_sm_count() / 2;
+    P.tok_tiles = (p.m + 255) / 256;
+    /* 512 channels a tile, or one half of 256 down to 64 (a staging row of bf16 is 64 channels): what ends first when
+     * every pair works through its tiles. */
+    long best = -1; int best_nh = 1, best_nt = 256;
+    for (int nt = 512; nt >= 64; nt -= nt > 256 ? 256 : 64) {
+        const long tiles = (long)P.tok_tiles * ((p.n + nt - 1) / nt), waves = (tiles + pairs - 1) / pairs;
+        const long cost = waves * (nt == 512 ? 512 : 24 + (nt * 9) / 8);
+        if (best < 0 || cost < best) { best = cost; best_nh = nt == 512 ? 2 : 1; best_nt = nt == 512 ? 256 : nt; }
+    }
+    P.nt = best_nt;
+    P.ch_tiles = (p.n + best_nh * best_nt - 1) / (best_nh * best_nt);
+    P.tiles = P.tok_tiles * P.ch_tiles;
+    P.workers = P.tiles < pairs ? P.tiles : pairs;
+    P.group = 8;
+    const int esz = P.y_f32 ? 4 : 2;
+    P.tma_store = grid16(p.y, p.y_pitch * esz);
+    CUtensorMap ta, tb, ty;
+    memset(&ty, 0, sizeof ty);
+    if (!make_map(&ta, p.a, (uint64_t)p.k, (uint64_t)p.m, (uint64_t)p.a_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, kStageK, kTokC) ||
+        !make_map(&tb, p.b, (uint64_t)p.k, (uint64_t)p.n, (uint64_t)p.b_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, kStageK, (uint32_t)(P.nt / 2)) ||
+        (P.tma_store && !make_map(&ty, p.y, (uint64_t)p.n, (uint64_t)p.m, (uint64_t)p.y_pitch * esz,
+                                  P.y_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (uint32_t)(128 / esz), 32)))
+        return RAD_E_UNSUPPORTED;
+    return best_nh == 2 ? run_pair<2>(p, P, ta, tb, ty, st) : run_pair<1>(p, P, ta, tb, ty, st);
+}
+
+int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
+    I8Params P = params_of(p);
+    const int sms = tc_sm_count();
+    P.mb = (p.m + 7) / 8 * 8;
+    /* channels a tile: the multiple of 16 with which the busiest slot streams the fewest bytes, the token tile's
+     * among them (it comes from L2, and counts a quarter). Two CTAs an SM where both rings fit. */
+    long best = -1;
+    for (int nt = 16; nt <= 256; nt += 16) {
+        const int stage = (P.mb + nt) * kStageK, per_sm = P.mb <= 64 && nt <= 128 ? 2 : 1;
+        const long tiles = (p.n + nt - 1) / nt, slots = (long)sms * per_sm, waves = (tiles + slots - 1) / slots;
+        const long cost = waves * (nt + P.mb / 4 + 4) * per_sm;
+        if (best < 0 || cost < best || (cost == best && nt > P.nt)) {
+            best = cost; P.nt = nt;
+            P.stages = (per_sm == 2 ? 88 * 1024 : 190 * 1024) / stage;
+        }
+    }
+    if (P.stages > 32) P.stages = 32;
+    const int tiles = (p.n + P.nt - 1) / P.nt;
+    P.shares = 1;
+    while (P.shares < 8 && tiles * P.shares * 2 <= sms && P.nk >= 4 * P.shares) P.shares *= 2;
+    /* the MMA reads 128 token rows from wherever the token tile starts: the last stage's reach 16 KiB on */
+    const size_t ring = (size_t)P.stages * (P.mb + P.nt) * kStageK + 128 * kStageK;
+    const size_t sums = (size_t)p.m * (P.nt + 4) * 4;
+    const size_t smem = 1024 + (ring > sums ? ring : sums);
+    static bool set[kTcMaxDevices] = {};
+    if (!allow_smem(k_i8_stream, 220 * 1024, set)) return RAD_E_DEVICE;
+    if (smem > 220 * 1024) return RAD_E_UNSUPPORTED;
+    CUtensorMap ta, tb;
+    if (!make_map(&ta, p.a, (uint64_t)p.k, (uint64_t)p.m, (uint64_t)p.a_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, kStageK, (uint32_t)P.mb) ||
+        !make_map(&tb, p.b, (uint64_t)p.k, (uint64_t)p.n, (uint64_t)p.b_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, kStageK, (uint32_t)P.nt))
+        return RAD_E_UNSUPPORTED;
+    return launch(k_i8_stream, tiles * P.shares, kStreamThreads, smem, P.shares, st, ta, tb, P);
+}
+
+} /* namespace */
+
+bool tc_i8_ok(const R3dGemmI8& p) {
+    return grid16(p.a, p.a_pitch) && grid16(p.b, p.b_pitch) && p.a_pitch >= p.k && p.b_pitch >= p.k && tc_have_encoder();
+}
+int tc_i8(const R3dGemmI8& p, cudaStream_t st) { return p.m <= 128 ? tc_i8_stream(p, st) : tc_i8_pair(p, st); }
+
+int tc_i8_status() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_tci8_status, sizeof(int)) != cudaSuccess) return -1;
+    return v;
+}
+
+} /* namespace r3d */

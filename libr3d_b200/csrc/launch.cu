@@ -333,13 +333,18 @@ extern "C" int r3d_b200_gated_quant_fp8(const void* gu, int64_t gu_pitch, void* 
                                   group, silu, (cudaStream_t)stream);
 }
 
-/* gemm_nt_q @ i8a8. AUTO: the dp4a tile kernel. */
+/* gemm_nt_q @ i8a8. AUTO: the tcgen05 kernels where TMA can take the operands, else the dp4a tile kernel. */
 extern "C" int r3d_b200_gemm_i8a8(const R3dGemmI8* q, void* stream) {
     if (!q) return RAD_E_INVAL;
     if (q->m <= 0 || q->n <= 0 || q->k <= 0 || q->k > 131071) return RAD_E_SHAPE;
     if ((q->bs_dtype != RAD_F32 && q->bs_dtype != RAD_BF16) || (q->y_dtype != RAD_F32 && q->y_dtype != RAD_BF16)) return RAD_E_DTYPE;
     if (!device_is_sm100()) return RAD_E_UNSUPPORTED;
-    if (q->arm != R3D_ARM_AUTO && q->arm != R3D_ARM_EXACT) return RAD_E_UNSUPPORTED;
+    if (q->arm != R3D_ARM_AUTO && q->arm != R3D_ARM_EXACT && q->arm != R3D_ARM_TILE) return RAD_E_UNSUPPORTED;
+    if (q->arm != R3D_ARM_EXACT && tc_i8_ok(*q)) {
+        debug_arm("i8a8", q->m <= 128 ? "tcgen05 weight stream" : "tcgen05 pair tiles", q->m);
+        return tc_i8(*q, (cudaStream_t)stream);
+    }
+    if (q->arm == R3D_ARM_TILE) return RAD_E_UNSUPPORTED;
     debug_arm("i8a8", "dp4a tiles", q->m);
     return i8_tile(*q, (cudaStream_t)stream);
 }

@@ -50,6 +50,10 @@ int launch_gemm_w2a8(const R3dW2A8& q, cudaStream_t st);
 /* the int8 band: gemm_nt_q @ i8a8 on dp4a (kern_i8.cu, any shape), its producers (kern_token_i8.cu), and the
  * sampler behind the logits (kern_nucleus.cu) */
 int i8_tile(const R3dGemmI8& p, cudaStream_t st);
+/* ... and on tcgen05 (kern_tc_i8.cu): operands on the 16-byte grid */
+bool tc_i8_ok(const R3dGemmI8& p);
+int  tc_i8(const R3dGemmI8& p, cudaStream_t st);
+int  tc_i8_status();
 int launch_token_i8(const R3dTokenI8& p, cudaStream_t st);
 int launch_nucleus(const R3dNucleus& p, cudaStream_t st);
 
