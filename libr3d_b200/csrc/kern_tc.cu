@@ -846,15 +846,12 @@ const CUtensorMap* tc_tensor_map(const void* ptr, uint64_t d0, uint64_t d1, uint
                                  CUtensorMapDataType dt, uint32_t box1, uint32_t box0, int promo128) {
     return tensor_map(ptr, d0, d1, pitch_bytes, dt, box1, box0, promo128);
 }
-bool tc_encode_map(CUtensorMap* m, const void* ptr, uint64_t d0, uint64_t d1, uint64_t pitch_bytes,
-                   CUtensorMapDataType dt, uint32_t box0, uint32_t box1) {
+bool tc_encode_map(CUtensorMap* m, const void* ptr, CUtensorMapDataType dt, int rank, const cuuint64_t* dims,
+                   const cuuint64_t* strides, const cuuint32_t* box) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
-    const cuuint64_t dims[2] = {d0, d1};
-    const cuuint64_t strides[1] = {pitch_bytes};
-    const cuuint32_t box[2] = {box0, box1};
-    const cuuint32_t estr[2] = {1u, 1u};
-    return fn(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const cuuint32_t estr[3] = {1u, 1u, 1u};
+    return fn(m, dt, (cuuint32_t)rank, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 int tc_device() {

@@ -38,8 +38,10 @@ struct I8Params {
     void* y; int64_t y_pitch; int y_f32;
     int m, n, nk;                                  /* nk: K stages */
     int nt;                                        /* channels of a tile */
-    int tok_tiles, ch_tiles, tiles, workers, group;
-    int mb, stages, shares, tma_store;
+    int tok_tiles, ch_tiles, workers, group;
+    int whole, split, jobs;                        /* pair: jobs below `whole` are tiles, those above halves of one if `split` */
+    int mb, stages, shares;                        /* stream: token rows of a box, ring, K shares */
+    int tma_store, y_quads;                        /* y on the 16-byte grid; y's rows on that of four elements */
 };
 
 /* kind::i8: s32 accumulators (2 at bit 4), a and b signed (1 at bits 7 and 10), N >> 3 at bit 17, M >> 4 at bit 24 */
@@ -82,6 +84,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16u(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
 /* pins uses of the loaded registers behind tcgen05.wait::ld */
 template <int N>
 __device__ __forceinline__ void pin_u32(uint32_t* r) {
@@ -108,6 +116,12 @@ __device__ __forceinline__ bool group_and(int id, bool v) {
     return r != 0;
 }
 
+/* a place in a ring of N slots, and its phase */
+template <int N> struct Ring {
+    int s = 0; uint32_t ph = 0;
+    __device__ __forceinline__ void next() { if (++s == N) { s = 0; ph ^= 1u; } }
+};
+
 /* ------------------------------------------------------------------ M > 128: CTA pairs */
 constexpr int kTokC = 128;                         /* tokens of a CTA; a pair has 256 */
 constexpr int kHalf = 256;                         /* accumulator columns of a half */
@@ -116,32 +130,37 @@ constexpr int kOpBytes = 128 * kStageK;            /* one operand tile of a stag
 constexpr int kPairThreads = 32 * 10;
 constexpr int kStoreBytes = 32 * 128;              /* a warp's staging tile: 32 tokens x 128 bytes */
 
-template <int NH> struct Pair {
-    static constexpr int stages = NH == 2 ? 4 : 6, stage = (1 + NH) * kOpBytes;
-    static constexpr size_t smem = (size_t)stages * stage + 8 * kStoreBytes + 2 * kHalf * sizeof(float) + 256;
-};
-static_assert(Pair<1>::smem <= 232448 && Pair<2>::smem <= 232448, "shared memory of a CTA");
+/* slots of the token ring and of the channel ring: a token tile is held until both halves have read it, a channel tile
+ * for one half only */
+constexpr int kSA = 6, kSB = 6;
+constexpr size_t kPairSmem = (kSA + kSB) * (size_t)kOpBytes + 8 * kStoreBytes + 2 * kHalf * sizeof(float) + 256;
+static_assert(kPairSmem <= 232448, "shared memory of a CTA");
 
-/* tile -> (token tile, channel tile): blocks of `group` token tiles walk the channels, so that the tiles in flight
+/* job -> tile: blocks of `group` token tiles walk the channels, so that the tiles in flight
  * share both operands in L2 */
-__device__ __forceinline__ void place(const I8Params& P, int tile, int* tt, int* ct) {
+struct Job { int t0, n0, halves; };                /* first token and channel; how many halves of nt channels */
+template <int NH>
+__device__ __forceinline__ Job place(const I8Params& P, int job) {
+    const bool half = P.split && job >= P.whole;
+    const int tile = half ? P.whole + (job - P.whole) / 2 : job;
     const int block = P.group * P.ch_tiles, b = tile / block, r = tile - b * block;
     const int here = min(P.group, P.tok_tiles - b * P.group);
-    *ct = r / here;
-    *tt = b * P.group + r % here;
+    const int first = half ? (job - P.whole) & 1 : 0;
+    return Job{(b * P.group + r % here) * 2 * kTokC, (r / here * NH + first) * P.nt, half ? 1 : NH};
 }
 
 template <int NH>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
           const __grid_constant__ CUtensorMap tmY, const I8Params P) {
-    constexpr int kStages = Pair<NH>::stages, kStage = Pair<NH>::stage;
-    extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* staging = smem + kStages * kStage;
+    extern __shared__ __align__(1024) uint8_t smem[];             /* kSA token tiles, kSB channel tiles */
+    uint8_t* staging = smem + (kSA + kSB) * kOpBytes;
     float* sb_s = (float*)(staging + 8 * kStoreBytes);            /* [2][kHalf] channel scales of the half in each buffer */
-    uint64_t* full = (uint64_t*)(sb_s + 2 * kHalf);
-    uint64_t* empty = full + kStages;
-    uint64_t* acc_full = empty + kStages;
+    uint64_t* full_a = (uint64_t*)(sb_s + 2 * kHalf);
+    uint64_t* empty_a = full_a + kSA;
+    uint64_t* full_b = empty_a + kSA;
+    uint64_t* empty_b = full_b + kSB;
+    uint64_t* acc_full = empty_b + kSB;
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
 
@@ -153,7 +172,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
     bool alive = (smem_u32(smem) & 1023u) == 0;                   /* the operand tiles' swizzle needs it */
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2 * (kSA + kSB); ++s) mbar_init(&full_a[s], 1);
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (!alive) atomicExch(&R3D_TC_STATUS_WORD, 90);
@@ -175,21 +194,24 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         if (elect_one()) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(&tmB) : "memory");
-            const uint32_t bytes = 2u * (uint32_t)(kTokC + NH * bc) * kStageK;
-            int s = 0; uint32_t ph = 0;
-            for (int tile = pair; tile < P.tiles && alive; tile += P.workers) {
-                int tt, ct;
-                place(P, tile, &tt, &ct);
-                const int t0 = tt * 2 * kTokC + (int)crank * kTokC, n0 = ct * NH * P.nt + (int)crank * bc;
-                for (int it = 0; it < nk; ++it) {
-                    if (!mbar_wait(&empty[s], ph ^ 1u, 91)) { alive = false; break; }
-                    const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0u);
-                    if (leader) mbar_expect_tx(&full[s], bytes);
-                    const uint32_t st = smem_u32(smem + s * kStage);
-                    tma_load_2d_pair(st, &tmA, it * kStageK, t0, bar);
-#pragma unroll
-                    for (int h = 0; h < NH; ++h) tma_load_2d_pair(st + (1 + h) * kOpBytes, &tmB, it * kStageK, n0 + h * P.nt, bar);
-                    if (++s == kStages) { s = 0; ph ^= 1u; }
+            Ring<kSA> ra; Ring<kSB> rb;
+            const auto load = [&](uint64_t* full, uint64_t* empty, int s, uint32_t ph, int slot, const CUtensorMap* map, int rows, int x, int y) {
+                if (!mbar_wait(&empty[s], ph ^ 1u, 91)) return false;
+                if (leader) mbar_expect_tx(&full[s], 2u * (uint32_t)rows * kStageK);
+                tma_load_2d_pair(smem_u32(smem + slot * kOpBytes), map, x, y, mapa_u32(smem_u32(&full[s]), 0u));
+                return true;
+            };
+            for (int job = pair; job < P.jobs && alive; job += P.workers) {
+                const Job J = place<NH>(P, job);
+                const int t0 = J.t0 + (int)crank * kTokC, n0 = J.n0 + (int)crank * bc;
+                for (int it = 0; it < nk + (J.halves - 1) * kLag && alive; ++it) {     /* the order in which the MMAs read */
+                    if (it < nk) {
+                        alive = load(full_a, empty_a, ra.s, ra.ph, ra.s, &tmA, kTokC, it * kStageK, t0); ra.next();
+                        alive = alive && load(full_b, empty_b, rb.s, rb.ph, kSA + rb.s, &tmB, bc, it * kStageK, n0); rb.next();
+                    }
+                    if (NH == 2 && J.halves == 2 && it >= kLag && alive) {
+                        alive = load(full_b, empty_b, rb.s, rb.ph, kSA + rb.s, &tmB, bc, (it - kLag) * kStageK, n0 + P.nt); rb.next();
+                    }
                 }
             }
         }
@@ -197,57 +219,45 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         /* ---------------- MMA issuer (the pair's leader only) ---------------- */
         if (leader && elect_one()) {
             const uint32_t idesc = i8_idesc(2 * kTokC, P.nt);
-            const auto mma = [&](int s, int h, int buf, bool first) {
-                const uint32_t a0 = smem_u32(smem + s * kStage), b0 = a0 + (1 + h) * kOpBytes;
+            const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
+            const auto mma = [&](int a, int b, int buf, bool first) {
+                const uint64_t a0 = desc0 + a * (kOpBytes >> 4), b0 = desc0 + (kSA + b) * (kOpBytes >> 4);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_i8<2>(tmem_base + buf * kHalf, smem_desc_sw128(a0 + k * 32), smem_desc_sw128(b0 + k * 32), idesc, first && !k ? 0u : 1u);
+                for (int k = 0; k < 4; ++k)                       /* 32 bytes of K on: two units of the descriptor's address */
+                    umma_i8<2>(tmem_base + buf * kHalf, a0 + 2 * k, b0 + 2 * k, idesc, first && !k ? 0u : 1u);
             };
             const auto release = [&](uint64_t* bar) {
                 umma2_commit(smem_u32(bar));
                 umma2_commit(mapa_u32(smem_u32(bar), 1u));
             };
-            int s = 0; uint32_t ph = 0;                           /* the stage half 0 (or the tile) reads next */
-            int s1 = 0;                                           /* the stage half 1 reads next */
-            int job = 0;                                          /* NH 1: tile count of this pair */
-            uint32_t aph = 0;
-            for (int tile = pair; tile < P.tiles && alive; tile += P.workers) {
-                if (NH == 1) {
-                    const int buf = job & 1;
-                    if (!mbar_wait(&acc_empty[buf], ((uint32_t)(job >> 1) & 1u) ^ 1u, 92)) { alive = false; break; }
-                    tc_fence_after();
-                    for (int it = 0; it < nk; ++it) {
-                        if (!mbar_wait(&full[s], ph, 93)) { alive = false; break; }
+            Ring<kSA> ra, ra1; Ring<kSB> rb;                        /* ra1: the token tile half 1 reads next */
+            int buf = 0; uint32_t aph = 0;
+            for (int job = pair; job < P.jobs && alive; job += P.workers) {
+                const int halves = place<NH>(P, job).halves;
+                for (int it = 0; it < nk + (halves - 1) * kLag; ++it) {
+                    if (it < nk) {
+                        if (it == 0 && !mbar_wait(&acc_empty[buf], aph ^ 1u, 92)) { alive = false; break; }
+                        if (!mbar_wait(&full_a[ra.s], ra.ph, 93) || !mbar_wait(&full_b[rb.s], rb.ph, 94)) { alive = false; break; }
                         tc_fence_after();
-                        mma(s, 0, buf, it == 0);
-                        release(&empty[s]);
-                        if (++s == kStages) { s = 0; ph ^= 1u; }
+                        mma(ra.s, rb.s, buf, it == 0);
+                        release(&empty_b[rb.s]);
+                        if (halves == 1) release(&empty_a[ra.s]);
+                        if (it == nk - 1) release(&acc_full[buf]);
+                        ra.next(); rb.next();
                     }
-                    if (alive) release(&acc_full[buf]);
-                    ++job;
-                } else {
-                    for (int it = 0; it < nk + kLag && alive; ++it) {
-                        if (it < nk) {
-                            if (it == 0 && !mbar_wait(&acc_empty[0], aph ^ 1u, 94)) { alive = false; break; }
-                            if (!mbar_wait(&full[s], ph, 95)) { alive = false; break; }
-                            tc_fence_after();
-                            mma(s, 0, 0, it == 0);
-                            if (it == nk - 1) release(&acc_full[0]);
-                            if (++s == kStages) { s = 0; ph ^= 1u; }
-                        }
-                        if (it >= kLag) {
-                            if (it == kLag) {
-                                if (!mbar_wait(&acc_empty[1], aph ^ 1u, 96)) { alive = false; break; }
-                                tc_fence_after();
-                            }
-                            mma(s1, 1, 1, it == kLag);
-                            release(&empty[s1]);
-                            if (it == nk + kLag - 1) release(&acc_full[1]);
-                            if (++s1 == kStages) s1 = 0;
-                        }
+                    if (NH == 2 && halves == 2 && it >= kLag) {
+                        if (it == kLag && !mbar_wait(&acc_empty[1], aph ^ 1u, 95)) { alive = false; break; }
+                        if (!mbar_wait(&full_b[rb.s], rb.ph, 96)) { alive = false; break; }
+                        tc_fence_after();
+                        mma(ra1.s, rb.s, 1, it == kLag);
+                        release(&empty_b[rb.s]);
+                        release(&empty_a[ra1.s]);
+                        if (it == nk + kLag - 1) release(&acc_full[1]);
+                        ra1.next(); rb.next();
                     }
-                    aph ^= 1u;
                 }
+                if (NH == 2 || buf) aph ^= 1u;
+                if (NH == 1) buf ^= 1;
             }
         }
     } else {
@@ -259,13 +269,12 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         float* const sb = sb_s + g * kHalf;
         const int esz = P.y_f32 ? 4 : 2, cols = 128 / esz;        /* channels of a 128-byte staging row */
         uint32_t aph = 0;
-        int job = 0;
-        for (int tile = pair; tile < P.tiles && alive; tile += P.workers, ++job) {
-            if (NH == 1 && (job & 1) != g) continue;
-            int tt, ct;
-            place(P, tile, &tt, &ct);
-            const int tw = tt * 2 * kTokC + (int)crank * kTokC + q * 32, t = tw + lane;
-            const int n0 = (ct * NH + (NH == 2 ? g : 0)) * P.nt;
+        int count = 0;
+        for (int job = pair; job < P.jobs && alive; job += P.workers, ++count) {
+            const Job J = place<NH>(P, job);
+            if (NH == 1 ? (count & 1) != g : g >= J.halves) continue;
+            const int tw = J.t0 + (int)crank * kTokC + q * 32, t = tw + lane;
+            const int n0 = J.n0 + (NH == 2 ? g * P.nt : 0);
             for (int i = et; i < P.nt; i += 128) sb[i] = channel_scale(P, n0 + i);
             const float sa = t < P.m ? __ldg(P.as + (int64_t)t * P.as_pitch) : 0.0f;
             /* one answer for the four warps: they meet at a barrier again below */
@@ -274,12 +283,22 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
             tc_fence_after();
             aph ^= 1u;
             const bool live = tw < P.m;                           /* the warp has tokens at all */
+            uint32_t bufs[2][32];
+            if (live) tmem_ld32(ta, bufs[0]);
 #pragma unroll 1
-            for (int c = 0; c < P.nt && live; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(ta + c, r);
+            for (int c2 = 0; c2 < P.nt && live; c2 += 64)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int c = c2 + 32 * h;
+                uint32_t* const r = bufs[h];
                 tmem_ld_wait();
                 pin_u32<32>(r);
+                if (c + 32 < P.nt) tmem_ld32(ta + c + 32, bufs[h ^ 1]);
+                else {                                            /* the last columns are in registers: the MMAs may go on */
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(acc_empty_leader);
+                }
                 if (c % cols == 0) {                              /* the staging tile's last store has read it */
                     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                     __syncwarp();
@@ -324,9 +343,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
                     __syncwarp();
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty_leader);
+            if (!live && lane == 0) mbar_arrive_cluster(acc_empty_leader);
             asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");   /* sb is read before the next tile's scales */
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -342,17 +359,20 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
 
 /* ------------------------------------------------------------------ M <= 128: the weights' stream */
 constexpr int kStreamThreads = 32 * 6;
+constexpr size_t kStreamSmem = 220 * 1024;
 
 __global__ void __launch_bounds__(kStreamThreads, 1)
 k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const I8Params P) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint64_t full[32], empty[32], done;
+    __shared__ uint64_t full[16], empty[16], done;       /* at most 88 KiB / 7 KiB or 190 KiB / 21 KiB stages */
     __shared__ uint32_t tmem_slot;
+    __shared__ float sa_s[128];
+    __shared__ __align__(16) float sb_s[256];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int shares = P.shares, crank = shares > 1 ? (int)cluster_rank() : 0;
     const int n0 = (int)(blockIdx.x / shares) * P.nt;
     const int it0 = (int)((int64_t)P.nk * crank / shares), nk = (int)((int64_t)P.nk * (crank + 1) / shares) - it0;
-    const int abytes = P.mb * kStageK, stage = abytes + P.nt * kStageK;
+    const int ablock = P.mb * kStageK, stage = ablock + P.nt * kStageK;
     const uint32_t cols = P.nt <= 32 ? 32u : P.nt <= 64 ? 64u : P.nt <= 128 ? 128u : 256u;
     uint8_t* const ring = (uint8_t*)(((uintptr_t)smem + 1023) & ~(uintptr_t)1023);
 
@@ -372,15 +392,16 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     dep_launch();
     dep_wait();
 
-    bool ok = true;
     if (warp == 0) {
         if (elect_one()) {
             int s = 0; uint32_t ph = 0;
             for (int it = 0; it < nk; ++it) {
                 if (!mbar_wait(&empty[s], ph ^ 1u, 81)) break;
+                uint8_t* const st = ring + s * stage;
+                const int at = it0 + it;
                 mbar_expect_tx(&full[s], (uint32_t)stage);
-                tma_load_2d(ring + s * stage + abytes, &tmB, (it0 + it) * kStageK, n0, &full[s]);
-                tma_load_2d(ring + s * stage, &tmA, (it0 + it) * kStageK, 0, &full[s]);
+                tma_load_2d(st + ablock, &tmB, at * kStageK, n0, &full[s]);
+                tma_load_2d(st, &tmA, at * kStageK, 0, &full[s]);
                 if (++s == P.stages) { s = 0; ph ^= 1u; }
             }
         }
@@ -388,23 +409,26 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     } else if (warp == 1) {
         if (elect_one()) {
             const uint32_t idesc = i8_idesc(128, P.nt);
+            const uint64_t desc0 = smem_desc_sw128(smem_u32(ring));
             int s = 0; uint32_t ph = 0;
             for (int it = 0; it < nk; ++it) {
                 if (!mbar_wait(&full[s], ph, 82)) break;
                 tc_fence_after();
-                const uint32_t a0 = smem_u32(ring + s * stage), b0 = a0 + abytes;
+                const uint64_t a = desc0 + s * (stage >> 4), b = a + (ablock >> 4);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_i8<1>(tmem_base, smem_desc_sw128(a0 + k * 32), smem_desc_sw128(b0 + k * 32), idesc, (it | k) ? 1u : 0u);
+                for (int k = 0; k < 4; ++k) umma_i8<1>(tmem_base, a + 2 * k, b + 2 * k, idesc, (it | k) ? 1u : 0u);
                 umma_commit(&empty[s]);
                 if (++s == P.stages) { s = 0; ph ^= 1u; }
             }
             umma_commit(&done);
         }
         __syncwarp();
+    } else {
+        for (int i = threadIdx.x - 64; i < P.m; i += 128) sa_s[i] = __ldg(P.as + (int64_t)i * P.as_pitch);
+        for (int i = threadIdx.x - 64; i < P.nt; i += 128) sb_s[i] = channel_scale(P, n0 + i);
     }
     /* the sums of the CTA's K share as [token][channel] words over the ring, whose stages are all consumed */
-    ok = mbar_wait(&done, 0, 83);
+    const bool ok = mbar_wait(&done, 0, 83);
     __syncthreads();
     const int pitch = P.nt + 4;                                   /* 16 bytes on: the lanes' rows fall into different banks */
     int* const sums = (int*)ring;
@@ -413,33 +437,52 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         tc_fence_after();
         if (q * 32 < P.m)
             for (int c = 0; c < P.nt; c += 16) {
-                float v[16];
-                tmem_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + c, v);
+                uint32_t v[16];
+                tmem_ld16u(tmem_base + ((uint32_t)(q * 32) << 16) + c, v);
                 tmem_ld_wait();
-                tmem_pin16(v);
+                pin_u32<16>(v);
                 if (t < P.m)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) *(float4*)(sums + t * pitch + c + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    for (int j = 0; j < 4; ++j) *(uint4*)(sums + t * pitch + c + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             }
         tc_fence_before();
     }
     if (shares > 1) cluster_sync_all(); else __syncthreads();
     if (ok) {
-        const int all = P.m * P.nt;
-        for (int i = crank * kStreamThreads + (int)threadIdx.x; i < all; i += kStreamThreads * shares) {
-            const int t = i / P.nt, c = i - t * P.nt, n = n0 + c;
-            if (n >= P.n) continue;
-            int sum = 0;
-            if (shares == 1) sum = sums[t * pitch + c];
-            else
-                for (int r = 0; r < shares; ++r) {
-                    int v;
-                    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_u32(smem_u32(sums + t * pitch + c), (uint32_t)r)) : "memory");
-                    sum += v;
+        /* a warp takes a token, its lanes four channels each; the tokens go round the warps of the cluster */
+        const int warps = kStreamThreads / 32 * shares;
+        for (int c = 4 * lane; c < P.nt; c += 128) {
+            const float4 sb = *(const float4*)(sb_s + c);
+            const int live = P.n - n0 - c;
+            for (int t = crank * (kStreamThreads / 32) + warp; t < P.m && live > 0; t += warps) {
+                int4 v = *(const int4*)(sums + t * pitch + c);
+                if (shares > 1) {
+                    const uint32_t mine = smem_u32(sums + t * pitch + c);
+                    for (int r = 0; r < shares; ++r) {
+                        if (r == crank) continue;
+                        int4 w;
+                        asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(mapa_u32(mine, (uint32_t)r)) : "memory");
+                        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+                    }
                 }
-            const float y = scaled((uint32_t)sum, __ldg(P.as + (int64_t)t * P.as_pitch), channel_scale(P, n));
-            if (P.y_f32) ((float*)P.y)[(int64_t)t * P.y_pitch + n] = y;
-            else ((uint16_t*)P.y)[(int64_t)t * P.y_pitch + n] = f32_to_bf16(y);
+                const float sa = sa_s[t];
+                const float y[4] = {scaled((uint32_t)v.x, sa, sb.x), scaled((uint32_t)v.y, sa, sb.y), scaled((uint32_t)v.z, sa, sb.z), scaled((uint32_t)v.w, sa, sb.w)};
+                const int64_t at = (int64_t)t * P.y_pitch + n0 + c;
+                if (P.y_f32) {
+                    float* const o = (float*)P.y + at;
+                    if (P.y_quads && live >= 4) *(float4*)o = make_float4(y[0], y[1], y[2], y[3]);
+                    else
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) if (j < live) o[j] = y[j];
+                } else {
+                    uint16_t* const o = (uint16_t*)P.y + at;
+                    if (P.y_quads && live >= 4) *(uint2*)o = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+                    else
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) if (j < live) o[j] = f32_to_bf16(y[j]);
+                }
+            }
         }
     }
     if (shares > 1) cluster_sync_all(); else __syncthreads();    /* peers have read this CTA's sums */
@@ -452,9 +495,14 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 /* ------------------------------------------------------------------ host */
 bool grid16(const void* p, int64_t pitch_bytes) { return (((uintptr_t)p | (uintptr_t)pitch_bytes) & 15) == 0; }
 
-/* made for the call: encoding takes less than a microsecond and nothing outlives the launch */
-bool make_map(CUtensorMap* m, const void* p, uint64_t d0, uint64_t d1, uint64_t pitch, CUtensorMapDataType dt, uint32_t box0, uint32_t box1) {
-    return tc_encode_map(m, p, d0, d1, pitch, dt, box0, box1);
+/* maps are made for the call: encoding takes less than a microsecond and nothing outlives the launch */
+bool rows_map(CUtensorMap* m, const void* p, int d0, int d1, int64_t pitch_bytes, CUtensorMapDataType dt, int box0, int box1) {
+    const cuuint64_t dims[2] = {(cuuint64_t)d0, (cuuint64_t)d1}, strides[1] = {(cuuint64_t)pitch_bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)box0, (cuuint32_t)box1};
+    return tc_encode_map(m, p, dt, 2, dims, strides, box);
+}
+bool codes_map(CUtensorMap* m, const void* p, int k, int rows, int64_t pitch, int box) {
+    return rows_map(m, p, k, rows, pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, kStageK, box);
 }
 
 template <typename K, typename... A>
@@ -493,10 +541,10 @@ I8Params params_of(const R3dGemmI8& p) {
 }
 
 template <int NH>
-int run_pair(const R3dGemmI8& p, I8Params P, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ty, cudaStream_t st) {
+int run_pair(const I8Params& P, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ty, cudaStream_t st) {
     static bool set[kTcMaxDevices] = {};
-    if (!allow_smem(k_i8_pair<NH>, Pair<NH>::smem, set)) return RAD_E_DEVICE;
-    return launch(k_i8_pair<NH>, 2 * P.workers, kPairThreads, Pair<NH>::smem, 1, st, ta, tb, ty, P);
+    if (!allow_smem(k_i8_pair<NH>, kPairSmem, set)) return RAD_E_DEVICE;
+    return launch(k_i8_pair<NH>, 2 * P.workers, kPairThreads, kPairSmem, 1, st, ta, tb, ty, P);
 }
 
 int tc_i8_pair(const R3dGemmI8& p, cudaStream_t st) {
@@ -504,61 +552,69 @@ int tc_i8_pair(const R3dGemmI8& p, cudaStream_t st) {
     const int pairs = tc_sm_count() / 2;
     P.tok_tiles = (p.m + 255) / 256;
     /* 512 channels a tile, or one half of 256 down to 64 (a staging row of bf16 is 64 channels): what ends first when
-     * every pair works through its tiles. */
-    long best = -1; int best_nh = 1, best_nt = 256;
-    for (int nt = 512; nt >= 64; nt -= nt > 256 ? 256 : 64) {
-        const long tiles = (long)P.tok_tiles * ((p.n + nt - 1) / nt), waves = (tiles + pairs - 1) / pairs;
-        const long cost = waves * (nt == 512 ? 512 : 24 + (nt * 9) / 8);
-        if (best < 0 || cost < best) { best = cost; best_nh = nt == 512 ? 2 : 1; best_nt = nt == 512 ? 256 : nt; }
+     * every pair works through its tiles. Where the last wave of 512-channel tiles fills no more than half the pairs, its
+     * halves go to pairs of their own. */
+    long best = -1; int nh = 1, nt = 256;
+    for (int c = 512; c >= 64; c -= c > 256 ? 256 : 64) {
+        const long tiles = (long)P.tok_tiles * ((p.n + c - 1) / c), rest = tiles % pairs;
+        const long cost = c == 512 ? tiles / pairs * 512 + (rest == 0 ? 0 : 2 * rest <= pairs ? 300 : 512)
+                                   : (tiles + pairs - 1) / pairs * (24 + (c * 9) / 8);
+        if (best < 0 || cost < best) { best = cost; nh = c == 512 ? 2 : 1; nt = c == 512 ? 256 : c; }
     }
-    P.nt = best_nt;
-    P.ch_tiles = (p.n + best_nh * best_nt - 1) / (best_nh * best_nt);
-    P.tiles = P.tok_tiles * P.ch_tiles;
-    P.workers = P.tiles < pairs ? P.tiles : pairs;
-    P.group = 8;
+    P.nt = nt;
+    P.ch_tiles = (p.n + nh * nt - 1) / (nh * nt);
+    const int tiles = P.tok_tiles * P.ch_tiles;
+    P.whole = tiles / pairs * pairs;
+    P.split = nh == 2 && 2 * (tiles - P.whole) <= pairs;
+    P.jobs = P.whole + (tiles - P.whole) * (P.split ? 2 : 1);
+    P.workers = P.jobs < pairs ? P.jobs : pairs;
+    P.group = 16;
     const int esz = P.y_f32 ? 4 : 2;
     P.tma_store = grid16(p.y, p.y_pitch * esz);
     CUtensorMap ta, tb, ty;
     memset(&ty, 0, sizeof ty);
-    if (!make_map(&ta, p.a, (uint64_t)p.k, (uint64_t)p.m, (uint64_t)p.a_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, kStageK, kTokC) ||
-        !make_map(&tb, p.b, (uint64_t)p.k, (uint64_t)p.n, (uint64_t)p.b_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, kStageK, (uint32_t)(P.nt / 2)) ||
-        (P.tma_store && !make_map(&ty, p.y, (uint64_t)p.n, (uint64_t)p.m, (uint64_t)p.y_pitch * esz,
-                                  P.y_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (uint32_t)(128 / esz), 32)))
+    if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, kTokC) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt / 2) ||
+        (P.tma_store && !rows_map(&ty, p.y, p.n, p.m, p.y_pitch * esz,
+                                  P.y_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 128 / esz, 32)))
         return RAD_E_UNSUPPORTED;
-    return best_nh == 2 ? run_pair<2>(p, P, ta, tb, ty, st) : run_pair<1>(p, P, ta, tb, ty, st);
+    return nh == 2 ? run_pair<2>(P, ta, tb, ty, st) : run_pair<1>(P, ta, tb, ty, st);
 }
 
 int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     I8Params P = params_of(p);
-    const int sms = tc_sm_count();
     P.mb = (p.m + 7) / 8 * 8;
-    /* channels a tile: the multiple of 16 with which the busiest slot streams the fewest bytes, the token tile's
-     * among them (it comes from L2, and counts a quarter). Two CTAs an SM where both rings fit. */
-    long best = -1;
-    for (int nt = 16; nt <= 256; nt += 16) {
-        const int stage = (P.mb + nt) * kStageK, per_sm = P.mb <= 64 && nt <= 128 ? 2 : 1;
-        const long tiles = (p.n + nt - 1) / nt, slots = (long)sms * per_sm, waves = (tiles + slots - 1) / slots;
-        const long cost = waves * (nt + P.mb / 4 + 4) * per_sm;
-        if (best < 0 || cost < best || (cost == best && nt > P.nt)) {
-            best = cost; P.nt = nt;
-            P.stages = (per_sm == 2 ? 88 * 1024 : 190 * 1024) / stage;
+    /* Up to 64 tokens two CTAs an SM with 96 channels each, above one with 192. A K block costs a CTA about 145 ns
+     * however few channels it has (measured from 16 to 64), so where those tiles leave slots idle, the CTAs of a
+     * cluster share K instead of taking fewer channels each: 5120 channels, K = 13824, 16 tokens take 15.0 us with 54
+     * tiles x 4 shares, 22.4 us with 160 tiles of 32. A share is at least eight K blocks (4096 x 4096: 4 shares 6.6 us,
+     * 8 shares 6.9 us). Where they do not, the tile is the multiple of 16 with which the last wave is fullest. */
+    const int per_sm = P.mb <= 64 ? 2 : 1, base = per_sm == 2 ? 96 : 192, slots = tc_sm_count() * per_sm;
+    const int tiles0 = (p.n + base - 1) / base;
+    P.nt = base;
+    P.shares = slots / tiles0;
+    if (P.shares > 8) P.shares = 8;
+    if (P.shares > P.nk / 8) P.shares = P.nk / 8;
+    if (P.shares < 2) {
+        P.shares = 1;
+        long best = -1;
+        for (int nt = base / 2; nt <= base * 4 / 3; nt += 16) {
+            const long tiles = (p.n + nt - 1) / nt, cost = (tiles + slots - 1) / slots * (nt + 16 + P.mb / 4);
+            if (best < 0 || cost <= best) { best = cost; P.nt = nt; }
         }
     }
-    if (P.stages > 32) P.stages = 32;
-    const int tiles = (p.n + P.nt - 1) / P.nt;
-    P.shares = 1;
-    while (P.shares < 8 && tiles * P.shares * 2 <= sms && P.nk >= 4 * P.shares) P.shares *= 2;
+    const int tiles = (p.n + P.nt - 1) / P.nt, stage = (P.mb + P.nt) * kStageK;
+    P.stages = (per_sm == 2 ? 88 * 1024 : 190 * 1024) / stage;
+    const int esz = P.y_f32 ? 4 : 2;
+    P.y_quads = (((uintptr_t)p.y | (uintptr_t)(p.y_pitch * esz)) & (uintptr_t)(4 * esz - 1)) == 0;
     /* the MMA reads 128 token rows from wherever the token tile starts: the last stage's reach 16 KiB on */
-    const size_t ring = (size_t)P.stages * (P.mb + P.nt) * kStageK + 128 * kStageK;
+    const size_t ring = (size_t)P.stages * stage + 128 * kStageK;
     const size_t sums = (size_t)p.m * (P.nt + 4) * 4;
     const size_t smem = 1024 + (ring > sums ? ring : sums);
     static bool set[kTcMaxDevices] = {};
-    if (!allow_smem(k_i8_stream, 220 * 1024, set)) return RAD_E_DEVICE;
-    if (smem > 220 * 1024) return RAD_E_UNSUPPORTED;
+    if (!allow_smem(k_i8_stream, kStreamSmem, set)) return RAD_E_DEVICE;
+    if (smem > kStreamSmem) return RAD_E_UNSUPPORTED;
     CUtensorMap ta, tb;
-    if (!make_map(&ta, p.a, (uint64_t)p.k, (uint64_t)p.m, (uint64_t)p.a_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, kStageK, (uint32_t)P.mb) ||
-        !make_map(&tb, p.b, (uint64_t)p.k, (uint64_t)p.n, (uint64_t)p.b_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, kStageK, (uint32_t)P.nt))
-        return RAD_E_UNSUPPORTED;
+    if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, P.mb) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt)) return RAD_E_UNSUPPORTED;
     return launch(k_i8_stream, tiles * P.shares, kStreamThreads, smem, P.shares, st, ta, tb, P);
 }
 

@@ -217,9 +217,9 @@ bool tc_pdl_on();
  * elements gets the 128-byte swizzle, any other none */
 const CUtensorMap* tc_tensor_map(const void* ptr, uint64_t d0, uint64_t d1, uint64_t pitch_bytes,
                                  CUtensorMapDataType dt, uint32_t box1, uint32_t box0 = 128u, int promo128 = 0);
-/* the same map, encoded for one call (rows of the box are 128 bytes, swizzled): nothing is remembered */
-bool tc_encode_map(CUtensorMap* m, const void* ptr, uint64_t d0, uint64_t d1, uint64_t pitch_bytes,
-                   CUtensorMapDataType dt, uint32_t box0, uint32_t box1);
+/* a map of two or three dimensions, encoded for one call (rows of the box are 128 bytes, swizzled): nothing is remembered */
+bool tc_encode_map(CUtensorMap* m, const void* ptr, CUtensorMapDataType dt, int rank, const cuuint64_t* dims,
+                   const cuuint64_t* strides, const cuuint32_t* box);
 /* the current device's ordinal, or -1 (no device, or beyond kTcMaxDevices): function attributes and
  * device properties are remembered per device, one process may drive several GPUs */
 constexpr int kTcMaxDevices = 64;
