@@ -18,6 +18,7 @@
  *
  * Every wait is bounded; on expiry a status word is set and the CTA drains and leaves.
  */
+#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -359,9 +360,10 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
 
 /* ------------------------------------------------------------------ M <= 128: the weights' stream */
 constexpr int kStreamThreads = 32 * 6;
+constexpr int kMaxShares = 8;                      /* a portable cluster */
 constexpr size_t kStreamSmem = 220 * 1024;
 
-__global__ void __launch_bounds__(kStreamThreads, 1)
+__global__ void __launch_bounds__(kStreamThreads, 2)
 k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const I8Params P) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ uint64_t full[16], empty[16], done;       /* at most 88 KiB / 7 KiB or 190 KiB / 21 KiB stages */
@@ -449,39 +451,54 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     }
     if (shares > 1) cluster_sync_all(); else __syncthreads();
     if (ok) {
-        /* a warp takes a token, its lanes four channels each; the tokens go round the warps of the cluster */
-        const int warps = kStreamThreads / 32 * shares;
-        for (int c = 4 * lane; c < P.nt; c += 128) {
+        /* four channels of a token a thread, all of them spread over the threads of the cluster; the peers' words of two
+         * such items are requested together (one at a time: 1.5 us more at 128 tokens and five shares) */
+        const int quads = P.nt / 4, items = P.m * quads, step = kStreamThreads * shares;
+        const auto finish = [&](int item, int4 v) {
+            const int t = item / quads, c = 4 * (item - t * quads), live = P.n - n0 - c;
+            const float sa = sa_s[t];
             const float4 sb = *(const float4*)(sb_s + c);
-            const int live = P.n - n0 - c;
-            for (int t = crank * (kStreamThreads / 32) + warp; t < P.m && live > 0; t += warps) {
-                int4 v = *(const int4*)(sums + t * pitch + c);
-                if (shares > 1) {
-                    const uint32_t mine = smem_u32(sums + t * pitch + c);
-                    for (int r = 0; r < shares; ++r) {
-                        if (r == crank) continue;
-                        int4 w;
-                        asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(mapa_u32(mine, (uint32_t)r)) : "memory");
-                        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+            const float y[4] = {scaled((uint32_t)v.x, sa, sb.x), scaled((uint32_t)v.y, sa, sb.y), scaled((uint32_t)v.z, sa, sb.z), scaled((uint32_t)v.w, sa, sb.w)};
+            const int64_t at = (int64_t)t * P.y_pitch + n0 + c;
+            if (P.y_f32) {
+                float* const o = (float*)P.y + at;
+                if (P.y_quads && live >= 4) *(float4*)o = make_float4(y[0], y[1], y[2], y[3]);
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) if (j < live) o[j] = y[j];
+            } else {
+                uint16_t* const o = (uint16_t*)P.y + at;
+                if (P.y_quads && live >= 4) *(uint2*)o = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) if (j < live) o[j] = f32_to_bf16(y[j]);
+            }
+        };
+        const auto word_of = [&](int item) { const int t = item / quads; return sums + t * pitch + 4 * (item - t * quads); };
+        if (shares == 1) {
+            for (int i = threadIdx.x; i < items; i += step) finish(i, *(const int4*)word_of(i));
+        } else {
+            for (int i = crank * kStreamThreads + (int)threadIdx.x; i < items; i += 2 * step) {
+                int4 w[2][kMaxShares];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (i + h * step < items) {
+                        const uint32_t mine = smem_u32(word_of(i + h * step));
+#pragma unroll
+                        for (int r = 0; r < kMaxShares; ++r)
+                            if (r < shares)
+                                asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                                             : "=r"(w[h][r].x), "=r"(w[h][r].y), "=r"(w[h][r].z), "=r"(w[h][r].w) : "r"(mapa_u32(mine, (uint32_t)r)));
                     }
-                }
-                const float sa = sa_s[t];
-                const float y[4] = {scaled((uint32_t)v.x, sa, sb.x), scaled((uint32_t)v.y, sa, sb.y), scaled((uint32_t)v.z, sa, sb.z), scaled((uint32_t)v.w, sa, sb.w)};
-                const int64_t at = (int64_t)t * P.y_pitch + n0 + c;
-                if (P.y_f32) {
-                    float* const o = (float*)P.y + at;
-                    if (P.y_quads && live >= 4) *(float4*)o = make_float4(y[0], y[1], y[2], y[3]);
-                    else
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) if (j < live) o[j] = y[j];
-                } else {
-                    uint16_t* const o = (uint16_t*)P.y + at;
-                    if (P.y_quads && live >= 4) *(uint2*)o = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-                    else
+                for (int h = 0; h < 2; ++h)
+                    if (i + h * step < items) {
+                        int4 v = w[h][0];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) if (j < live) o[j] = f32_to_bf16(y[j]);
-                }
+                        for (int r = 1; r < kMaxShares; ++r)
+                            if (r < shares) { v.x += w[h][r].x; v.y += w[h][r].y; v.z += w[h][r].z; v.w += w[h][r].w; }
+                        finish(i + h * step, v);
+                    }
             }
         }
     }
@@ -580,7 +597,27 @@ int tc_i8_pair(const R3dGemmI8& p, cudaStream_t st) {
     return nh == 2 ? run_pair<2>(P, ta, tb, ty, st) : run_pair<1>(P, ta, tb, ty, st);
 }
 
+/* clusters of `shares` CTAs that the device holds at once at one CTA an SM. Each lies in one GPC, so 27 clusters of five
+ * do not fit 148 SMs (26 do; measured: a second wave, 28 instead of 17 us). Two CTAs an SM hold at least twice as
+ * many; the query itself counts one for kernels that allocate tensor memory. */
+int resident_clusters(int dev, int shares) {
+    static std::atomic<int> known[kTcMaxDevices][kMaxShares + 1];
+    int n = known[dev][shares].load(std::memory_order_relaxed);
+    if (n) return n;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)shares); cfg.blockDim = dim3(kStreamThreads); cfg.dynamicSmemBytes = kStreamSmem;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)shares; at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at; cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, k_i8_stream, &cfg) != cudaSuccess || n < 1) { (void)cudaGetLastError(); n = 1; }
+    known[dev][shares].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
+    static bool set[kTcMaxDevices] = {};
+    if (!allow_smem(k_i8_stream, kStreamSmem, set)) return RAD_E_DEVICE;
     I8Params P = params_of(p);
     P.mb = (p.m + 7) / 8 * 8;
     /* Up to 64 tokens two CTAs an SM with 96 channels each, above one with 192. A K block costs a CTA about 145 ns
@@ -592,8 +629,9 @@ int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     const int tiles0 = (p.n + base - 1) / base;
     P.nt = base;
     P.shares = slots / tiles0;
-    if (P.shares > 8) P.shares = 8;
+    if (P.shares > kMaxShares) P.shares = kMaxShares;
     if (P.shares > P.nk / 8) P.shares = P.nk / 8;
+    while (P.shares > 1 && per_sm * resident_clusters(tc_device(), P.shares) < tiles0) --P.shares;
     if (P.shares < 2) {
         P.shares = 1;
         long best = -1;
@@ -610,8 +648,6 @@ int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     const size_t ring = (size_t)P.stages * stage + 128 * kStageK;
     const size_t sums = (size_t)p.m * (P.nt + 4) * 4;
     const size_t smem = 1024 + (ring > sums ? ring : sums);
-    static bool set[kTcMaxDevices] = {};
-    if (!allow_smem(k_i8_stream, kStreamSmem, set)) return RAD_E_DEVICE;
     if (smem > kStreamSmem) return RAD_E_UNSUPPORTED;
     CUtensorMap ta, tb;
     if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, P.mb) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt)) return RAD_E_UNSUPPORTED;
