@@ -2,7 +2,7 @@
 
     python -m libr3d_b200.build
 
-The shared object lands next to this file so that it travels with the source tree; there
+The shared object (and _bind.so, the Python side of its int8 step) lands next to this file so that it travels with the source tree; there
 is no JIT cache and no installed copy. Objects are rebuilt only when a source or header is
 newer. `-fmad=false`: the kernels spell every fused multiply-add they want, because a
 contracted mul+add is a different rounding than the arithmetic contract states.
@@ -20,6 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "build"
 SO = PKG / "libr3d_b200.so"
+BIND = PKG / "_bind.so"
 
 SOURCES = [
     "rows_table.cpp",
@@ -93,7 +94,30 @@ def build_plugin(verbose: bool = False, ptxas_info: bool = False) -> Path:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    build_bind()
     return SO
+
+
+def build_bind() -> Path:
+    """_bind.so: ops.py's call path in C++ (torch's headers, the plugin beside it)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    src = CSRC / "bind.cpp"
+    if _stale(BIND, [src, SO, *(ROOT / "include").glob("*.h")]):
+        home = Path(torch.__file__).resolve().parent
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               *(f"-isystem{p}" for p in cpp_extension.include_paths("cuda")), f"-isystem{sysconfig.get_paths()['include']}",
+               "-I", str(ROOT / "include"), str(src), "-o", str(BIND),
+               f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda",
+               f"-L{PKG}", f"-l:{SO.name}", "-Wl,-rpath,$ORIGIN"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            sys.stderr.write(r.stdout + r.stderr)
+            raise RuntimeError("g++ failed on bind.cpp")
+    return BIND
 
 
 if __name__ == "__main__":

@@ -7,8 +7,6 @@ current CUDA stream. Nothing is computed here.
 """
 from __future__ import annotations
 
-import ctypes as C
-import threading
 from typing import Any
 
 import torch
@@ -275,56 +273,33 @@ def sample_argmax(logits: torch.Tensor, token: torch.Tensor, params: torch.Tenso
 
 
 # ---------------------------------------------------------------------- the int8 band and its sampler
-_RAD_OF = {torch.float32: abi.RAD_F32, torch.bfloat16: abi.RAD_BF16, torch.int8: abi.RAD_I8, torch.int32: abi.RAD_I32}
 _NAME_OF = {torch.float32: "f32", torch.bfloat16: "bf16"}
-_tls = threading.local()
+_KIND_OF = {torch.float32: 0, torch.bfloat16: 1}
+_I8, _F32, _I32 = 2, 0, 3
+_bind = None
 
 
-class _Declared:
-    """An op declared for one set of shapes, strides, types and parameters: the resolved row and its RadArgs, in
-    which a call only writes its operands' addresses. One per thread, as a call fills it in."""
-
-    def __init__(self, op: str, query: dict, tensors: tuple):
-        P = plugin()
-        self.row = P.resolve(op, query)
-        if self.row is None:
-            raise RuntimeError(f"no row serves {op} {query}")
-        self.pack = ArgPack([_desc(t, abi.RAD_F32 if t is None else _RAD_OF[t.dtype]) for t in tensors], query)
-        self.slots = [self.pack.t[i] for i in range(len(tensors))]
-        self.argp = C.byref(self.pack.args)
-        self.fn = P._launch_t(self.row.launch)
+def _load_bind():
+    """_bind.so stands beside the plugin and uses the same loaded library."""
+    global _bind
+    plugin()
+    try:
+        from . import _bind as loaded
+    except ImportError as e:
+        raise ImportError("libr3d_b200/_bind.so is not built: run `python -m libr3d_b200.build`") from e
+    _bind = loaded
+    return loaded
 
 
-def _run(op: str, params: tuple, tensors: tuple) -> Row:
+def _run(op: str, params: tuple, *tensors) -> None:
     """One call of `op` on the operands' device, on that device's current stream. `params`: (key, value) pairs;
     `tensors`: by schema position, None where an optional one is absent."""
-    key = (op, params, *[None if t is None else (t.dtype, t.shape, t.stride(), t.get_device()) for t in tensors])
-    try:
-        declared = _tls.declared
-    except AttributeError:
-        declared = _tls.declared = {}
-    d = declared.get(key)
-    if d is None:
-        for t in tensors:
-            if t is not None and t.dtype not in _RAD_OF:
-                raise TypeError(f"{op}: no {t.dtype} operands")
-        if len({t.get_device() for t in tensors if t is not None}) > 1 or not tensors[0].is_cuda:
-            raise ValueError(f"{op}: operands on one CUDA device are needed, got {[t.device for t in tensors if t is not None]}")
-        if len(declared) >= 1024:                   # shapes that keep changing: start over
-            declared.clear()
-        d = declared[key] = _Declared(op, dict(params), tensors)
-    for slot, t in zip(d.slots, tensors):
-        if t is not None:
-            slot.data = t.data_ptr()
-    dev = tensors[0].get_device()
-    if dev == torch.cuda.current_device():
-        rc = d.fn(d.argp, torch.cuda.current_stream(dev).cuda_stream)
-    else:
-        with torch.cuda.device(dev):
-            rc = d.fn(d.argp, torch.cuda.current_stream(dev).cuda_stream)
-    if rc != abi.RAD_OK:
-        raise RowRefused(d.row.name, rc)
-    return d.row
+    not_taken = (_bind or _load_bind()).issue(op, params, *tensors)
+    if not_taken is not None:
+        row, rc = not_taken
+        if row is None:
+            raise RuntimeError(f"no row serves {op} {dict(params)}")
+        raise RowRefused(row, rc)
 
 
 def gemm_i8a8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -332,22 +307,20 @@ def gemm_i8a8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     """y[..., N] = (sum_k a[..., k] * b[n, k]) * a_scale[...] * b_scale[n]: int8 codes [..., K] and [N, K], one f32
     scale a token ([...] or [..., 1]) and one f32 or bf16 scale a channel ([N] or [N, 1]). The sum is exact (K at
     most 131071), the result is rounded once, to `out_dtype` (bf16 or f32), or to y's type where y is given."""
-    K, N = a.shape[-1], b.shape[0]
+    N, K = b.shape
     if y is None:
-        y = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=a.device)
-    if a.dim() > 0 and a.numel() == 0 and K and y.numel() == 0:
-        return y                                    # no tokens
-    _run("gemm_nt_q", (("M", y.numel() // max(N, 1)), ("N", N), ("K", K), ("group", K), ("dtype", "i8a8")),
-         (a, a_scale, b, b_scale, y, None, None))
+        if out_dtype not in _KIND_OF:
+            raise TypeError(f"gemm_i8a8: bf16 or f32 results, got {out_dtype}")
+        y = (_bind or _load_bind()).rows(a, N, _KIND_OF[out_dtype])
+    M = a.numel() // K if K else 0
+    if M or not K:                                  # no tokens: nothing to do
+        _run("gemm_nt_q", (("M", M), ("N", N), ("K", K), ("group", K), ("dtype", "i8a8")), a, a_scale, b, b_scale, y)
     return y
 
 
 def _codes_for(x: torch.Tensor, n: int, q: torch.Tensor | None, scale: torch.Tensor | None):
-    if q is None:
-        q = torch.empty((*x.shape[:-1], n), dtype=torch.int8, device=x.device)
-    if scale is None:
-        scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
-    return q, scale
+    new = (_bind or _load_bind()).rows
+    return new(x, n, _I8) if q is None else q, new(x, 1, _F32) if scale is None else scale
 
 
 def _act_name(op: str, x: torch.Tensor) -> str:
@@ -363,7 +336,7 @@ def quant_token_i8(x: torch.Tensor, q: torch.Tensor | None = None,
     n = x.shape[-1]
     q, scale = _codes_for(x, n, q, scale)
     if x.numel() or not n:
-        _run("quant_token_i8", (("M", x.numel() // max(n, 1)), ("n", n), ("dtype", _act_name("quant_token_i8", x))), (x, q, scale))
+        _run("quant_token_i8", (("M", x.numel() // max(n, 1)), ("n", n), ("dtype", _act_name("quant_token_i8", x))), x, q, scale)
     return q, scale
 
 
@@ -375,7 +348,7 @@ def gated_quant_token_i8(gate_up: torch.Tensor, q: torch.Tensor | None = None, s
     q, scale = _codes_for(gate_up, n, q, scale)
     if gate_up.numel() or not n:
         _run("gated_quant_token_i8", (("M", gate_up.numel() // max(2 * n, 1)), ("n", n),
-                                      ("dtype", _act_name("gated_quant_token_i8", gate_up)), ("act", act)), (gate_up, q, scale, out))
+                                      ("dtype", _act_name("gated_quant_token_i8", gate_up)), ("act", act)), gate_up, q, scale, out)
     return q, scale
 
 
@@ -390,7 +363,7 @@ def rmsnorm_quant_token_i8(x: torch.Tensor, w: torch.Tensor, q: torch.Tensor | N
     if x.numel() or not n:
         _run("rmsnorm_quant_token_i8",
              (("M", x.numel() // max(n, 1)), ("n", n), ("eps", float(eps)), ("wadd", float(wadd)),
-              ("dtype", _act_name("rmsnorm_quant_token_i8", x))), (x, residual, w, q, scale, out))
+              ("dtype", _act_name("rmsnorm_quant_token_i8", x))), x, residual, w, q, scale, out)
     return q, scale
 
 
@@ -408,10 +381,10 @@ def sample_nucleus(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.
     `logprob` (f32) receives the log of the token's share of what was kept, `kept` (int32) how many tokens were."""
     V = logits.shape[-1]
     if token is None:
-        token = torch.empty(logits.shape[:-1], dtype=torch.int32, device=logits.device)
+        token = (_bind or _load_bind()).rows(logits, -1, _I32)
     if logits.numel() or not V:
         _run("sample_nucleus", (("M", logits.numel() // max(V, 1)), ("n_vocab", V), ("dtype", _act_name("sample_nucleus", logits))),
-             (logits, u, temperature, top_k, top_p, min_p, token, logprob, kept))
+             logits, u, temperature, top_k, top_p, min_p, token, logprob, kept)
     return token
 
 
