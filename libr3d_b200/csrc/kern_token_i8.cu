@@ -11,8 +11,11 @@
  * NaN or infinite, so it reaches the product's output, and the codes of what cannot be scaled are 0.
  *
  * Bound by memory: x is read once (rmsnorm also reads and writes the residual), one byte a value is written. So a
- * block owns a row and keeps it in registers between the reduction and the codes.
+ * block owns a row and keeps h in registers between the reduction and the codes: k_token_i8_regs, eight values a
+ * thread and chunk, by 16-byte loads where every operand's rows lie on the 16-byte grid (codes: 8), else one value at
+ * a time, neighbouring threads next to each other. Rows of more than 32768 values are read again for each step.
  */
+#include <atomic>
 #include <cmath>
 #include "r3d_kernels.h"
 #include "r3d_numerics.cuh"
@@ -30,7 +33,7 @@ struct TokenI8 {
     int8_t* q; int64_t q_pitch;
     float* scale; int64_t s_pitch;
     void* ob; int ob_f32; int64_t ob_pitch;
-    int n;
+    int n, rows;
     float eps, wadd;
 };
 
@@ -41,22 +44,60 @@ __device__ __forceinline__ float narrow(float v, const uint16_t*) { return bf16_
 __device__ __forceinline__ void st1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void st1(uint16_t* p, float v) { *p = f32_to_bf16(v); }
 
-/* max that keeps a NaN: the larger bit pattern of two non-negative floats is the larger value, NaN above all */
-__device__ __forceinline__ float max_nan(float a, float b) {
-    return __uint_as_float(max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
+__device__ __forceinline__ float max_nan(float a, float b) {          /* keeps a NaN */
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
+/* two values an instruction */
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 two_of(float a, float b) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void parts_of(f2 v, float* f) { asm("mov.b64 {%0, %1}, %2;" : "=f"(f[0]), "=f"(f[1]) : "l"(v)); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 
+/* over the block, the same in every thread; every warp finishes it by itself (one warp doing so for all, the quotients
+ * behind it included, saves a tenth of the instructions and waits longer: 54.5 instead of 51.2 us for 8192 x 5120) */
 template <typename F>
 __device__ __forceinline__ float block_reduce(float v, float* part, F f) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-    const int warps = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = part[0];
-    for (int i = 1; i < warps; ++i) v = f(v, part[i]);
-    __syncthreads();
+    v = lane < warps ? part[lane] : 0.0f;                          /* 0 is neutral for both: a sum, a largest size */
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
+}
+
+/* 1.5 * 2^23: the low byte of fma(h, step, kCode) is the whole number nearest to h * step, ties to even */
+constexpr float kCode = 12582912.0f;
+
+/* a row of zeros, and one so small that 127 / amax is not a number of this type, has step 0: codes 0. So has a row
+ * with a NaN or an infinity in it */
+__device__ __forceinline__ float step_of(float amax) { return amax < 0x1p-100f || !(amax < INFINITY) ? 0.0f : 127.0f / amax; }
+__device__ __forceinline__ float scale_of(float amax) { return amax < 0x1p-100f ? 1.0f : amax / 127.0f; }
+
+/* silu(g) * u or sigmoid(g) * u; the exponential and the quotient by the special-function unit, 2 ulp each */
+template <int KIND>
+__device__ __forceinline__ f2 gate2(f2 g, f2 u) {
+    float e[2];
+    parts_of(mul2(g, two_of(-1.442695041f, -1.442695041f)), e);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[i]));
+    parts_of(add2(two_of(e[0], e[1]), two_of(1.0f, 1.0f)), e);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e[i]));
+    const f2 s = two_of(e[0], e[1]);
+    return mul2(KIND == kSilu ? mul2(g, s) : s, u);
+}
+template <int KIND>
+__device__ __forceinline__ float gate(float g, float u) {
+    float f[2];
+    parts_of(gate2<KIND>(two_of(g, 0.0f), two_of(u, 0.0f)), f);
+    return f[0];
 }
 
 template <int KIND, typename T>
@@ -68,15 +109,239 @@ __device__ __forceinline__ float value_of(const TokenI8& P, int64_t row, int i, 
         const float w = P.w_f32 ? ((const float*)P.w)[i] : bf16_to_f32(((const uint16_t*)P.w)[i]);
         return v * rs * (w + P.wadd);
     }
-    const float g = ld1(x + i), u = ld1(x + P.n + i);
-    const float s = __fdividef(1.0f, 1.0f + __expf(-g));
-    return (KIND == kSilu ? g * s : s) * u;
+    return gate<KIND>(ld1(x + i), ld1(x + P.n + i));
 }
 
-/* any width, any alignment: the row is read again for each of the passes (it stays in the caches) */
+/* Eight neighbouring values as they lie in memory. */
+template <typename T> struct Raw;
+template <> struct Raw<uint16_t> {
+    uint32_t w[4];
+    __device__ __forceinline__ void get(const uint16_t* p) { const uint4 v = *(const uint4*)p; w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+    __device__ __forceinline__ void put(uint16_t* p) const { *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]); }
+    __device__ __forceinline__ f2 pair(int j) const { return two_of(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)); }
+    __device__ __forceinline__ void set(int j, f2 v) {
+        float f[2];
+        parts_of(v, f);
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(f[1]), "f"(f[0]));
+    }
+    /* the sum of two bf16 numbers rounded once: what its f32 sum, narrowed, is (that one is exact up to 2^16 between
+     * them, and beyond that both round to the larger) */
+    __device__ __forceinline__ void add(const Raw& o) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(w[j]) : "r"(w[j]), "r"(o.w[j]));
+    }
+    __device__ __forceinline__ void scalars(const uint16_t* p, int at, int n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = (unsigned)(at + 2 * j) < (unsigned)n ? p[at + 2 * j] : 0, hi = (unsigned)(at + 2 * j + 1) < (unsigned)n ? p[at + 2 * j + 1] : 0;
+            w[j] = lo | hi << 16;
+        }
+    }
+    __device__ __forceinline__ void put_scalars(uint16_t* p, int at, int n) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if ((unsigned)(at + j) < (unsigned)n) p[at + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+    }
+};
+template <> struct Raw<float> {
+    f2 v[4];
+    __device__ __forceinline__ void get(const float* p) {
+        const ulonglong2 a = *(const ulonglong2*)p, b = *(const ulonglong2*)(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+    }
+    __device__ __forceinline__ void put(float* p) const { *(ulonglong2*)p = make_ulonglong2(v[0], v[1]); *(ulonglong2*)(p + 4) = make_ulonglong2(v[2], v[3]); }
+    __device__ __forceinline__ f2 pair(int j) const { return v[j]; }
+    __device__ __forceinline__ void set(int j, f2 x) { v[j] = x; }
+    __device__ __forceinline__ void add(const Raw& o) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = add2(v[j], o.v[j]);
+    }
+    __device__ __forceinline__ void scalars(const float* p, int at, int n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[j] = two_of((unsigned)(at + 2 * j) < (unsigned)n ? p[at + 2 * j] : 0.0f, (unsigned)(at + 2 * j + 1) < (unsigned)n ? p[at + 2 * j + 1] : 0.0f);
+    }
+    __device__ __forceinline__ void put_scalars(float* p, int at, int n) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[2];
+            parts_of(v[j], f);
+            if ((unsigned)(at + 2 * j) < (unsigned)n) p[at + 2 * j] = f[0];
+            if ((unsigned)(at + 2 * j + 1) < (unsigned)n) p[at + 2 * j + 1] = f[1];
+        }
+    }
+};
+/* the chunk at value `at` of a row, which may reach over either end of it: by 16 bytes where `fast` */
+template <typename T>
+__device__ __forceinline__ Raw<T> load_chunk(const T* row, int at, int n, bool fast) {
+    Raw<T> r;
+    if (fast) r.get(row + at); else r.scalars(row, at, n);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* row, int at, int n, bool fast, const f2* h) {
+    Raw<T> r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.set(j, h[j]);
+    if (fast) r.put(row + at); else r.put_scalars(row, at, n);
+}
+__device__ __forceinline__ bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+/* The block walks rows gridDim apart. A row is cut into chunks of eight values on x's 16-byte grid, wherever the row
+ * begins, C chunks a thread; what else lies on that grid (the residual of an odd width as well) is accessed by 16 bytes
+ * too. GRID: every row of every operand begins on its grid and ends a chunk. While a row is reduced, the next one is on
+ * its way into shared memory by cp.async, each thread's chunks to places of its own: no barrier, no registers.
+ * Instructions, not bytes, bound the bf16 forms at first (46 a value): hence two values an instruction wherever there is
+ * one, and the residual's sum in bf16 pairs. */
+template <int KIND, typename T, int C, bool GRID>
+__global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const TokenI8 P) {
+    constexpr bool kTwo = KIND != kQuant;                         /* the residual, or the up half */
+    constexpr int kPer = 8 * (int)sizeof(T);                      /* bytes of a chunk */
+    extern __shared__ __align__(16) uint8_t slots[];
+    __shared__ float part[2][32];
+    const int n = P.n, threads = blockDim.x;
+    const bool two = kTwo && (KIND != kRms || P.res);
+    const int64_t rows = P.rows;
+    int64_t row = blockIdx.x;
+    const T* x = (const T*)P.x + row * P.x_pitch;                 /* the row's operands: y is the residual or the up half */
+    T* y = KIND == kRms ? (T*)P.res + (P.res ? row * P.r_pitch : 0) : const_cast<T*>(x) + n;
+    const int64_t x_step = P.x_pitch * gridDim.x, y_step = KIND == kRms ? P.r_pitch * gridDim.x : x_step;
+    uint8_t* const slot = slots + threadIdx.x * kPer;             /* chunk c of x: c * threads on; of y: C + c */
+    const auto lead = [&]() { return GRID ? 0 : -(int)(((uintptr_t)x & 15) / sizeof(T)); };
+    const auto whole = [&](int at) { return GRID ? at < n : at >= 0 && at + 8 <= n; };
+    const auto copy = [&](int place, const T* from) {
+#pragma unroll
+        for (int b = 0; b < kPer; b += 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                         ::"r"((uint32_t)__cvta_generic_to_shared(slot + place * threads * kPer) + b), "l"((const char*)from + b) : "memory");
+    };
+    const auto fetch = [&](int first) {
+        const bool y_grid = two && (GRID || on16(y + first));
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int at = first + c * threads * 8;
+            if (!whole(at)) continue;
+            copy(c, x + at);
+            if (kTwo && y_grid) copy(C + c, y + at);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int first = lead() + (int)threadIdx.x * 8;
+    fetch(first);
+    for (; row < rows; row += gridDim.x) {
+        f2 h[C][4];
+        f2 ss = 0, bad = 0;
+        float amax = 0.0f;
+        const int here = first;                                   /* this row's; `first` moves on to the next below */
+        const bool y_grid = two && (GRID || on16(y + here));
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int at = here + c * threads * 8;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[c][j] = 0;
+            if (GRID && at >= n) continue;
+            const bool in = whole(at);
+            Raw<T> r, s;
+            if (in) r.get((const T*)(slot + c * threads * kPer)); else r.scalars(x, at, n);
+            if (two) {
+                if (in && y_grid) s.get((const T*)(slot + (C + c) * threads * kPer)); else s.scalars((const T*)y, at, n);
+                if (KIND == kRms) {
+                    r.add(s);
+                    if (in && y_grid) r.put(y + at); else r.put_scalars(y, at, n);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h[c][j] = r.pair(j);
+                if (KIND == kRms) ss = fma2(h[c][j], h[c][j], ss);
+                else if (KIND != kQuant) h[c][j] = gate2<KIND>(h[c][j], s.pair(j));
+            }
+        }
+        /* the slots have been read once their values are in use */
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) asm volatile("" : "+l"(h[c][j]));
+        if (row + gridDim.x < rows) {
+            x += x_step; y += y_step;
+            first = lead() + (int)threadIdx.x * 8;
+            fetch(first);
+        }
+        if (KIND == kRms) {
+            float half[2];
+            parts_of(ss, half);
+            const float sum = block_reduce(half[0] + half[1], part[0], [](float a, float b) { return a + b; });
+            const float rs = 1.0f / sqrtf(sum / (float)n + P.eps);
+            const f2 rs2 = two_of(rs, rs), wadd2 = two_of(P.wadd, P.wadd);
+            const bool w_grid = GRID || (P.w_f32 ? on16((const float*)P.w + here) : on16((const uint16_t*)P.w + here));
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int at = here + c * threads * 8;
+                if (GRID && at >= n) continue;
+                const bool in = w_grid && whole(at);
+                if (P.w_f32) {
+                    const Raw<float> w = load_chunk((const float*)P.w, at, n, in);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[c][j] = mul2(mul2(h[c][j], rs2), add2(w.pair(j), wadd2));
+                } else {
+                    const Raw<uint16_t> w = load_chunk((const uint16_t*)P.w, at, n, in);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[c][j] = mul2(mul2(h[c][j], rs2), add2(w.pair(j), wadd2));
+                }
+            }
+        }
+        /* fmaxf drops a NaN: 0 * h keeps it */
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float f[2];
+                parts_of(h[c][j], f);
+                amax = fmaxf(fmaxf(amax, fabsf(f[0])), fabsf(f[1]));
+                bad = fma2(h[c][j], two_of(0.0f, 0.0f), bad);
+            }
+        {
+            float f[2];
+            parts_of(bad, f);
+            if (f[0] != 0.0f || f[1] != 0.0f) amax = amax < INFINITY ? NAN : amax;
+        }
+        amax = block_reduce(amax, part[1], max_nan);
+        const float step = step_of(amax);
+        if (threadIdx.x == 0) P.scale[row * P.s_pitch] = scale_of(amax);
+        const f2 step2 = two_of(step, step), code2 = two_of(kCode, kCode);
+        int8_t* const q = P.q + row * P.q_pitch;
+        const bool q_grid = GRID || ((uintptr_t)(q + here) & 7) == 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int at = here + c * threads * 8;
+            if (GRID && at >= n) continue;
+            const bool in = whole(at);
+            uint32_t w[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float f[4];
+                parts_of(fma2(h[c][2 * j], step2, code2), f);
+                parts_of(fma2(h[c][2 * j + 1], step2, code2), f + 2);
+                w[j] = __byte_perm(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040),
+                                   __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040), 0x5410);
+                if (step == 0.0f) w[j] = 0u;
+            }
+            if (in && q_grid) *(uint2*)(q + at) = make_uint2(w[0], w[1]);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; ++j) if ((unsigned)(at + j) < (unsigned)n) q[at + j] = (int8_t)(w[j >> 2] >> (8 * (j & 3)));
+            if (P.ob) {
+                if (P.ob_f32) { float* const o = (float*)P.ob + row * P.ob_pitch; store_chunk(o, at, n, in && on16(o + at), h[c]); }
+                else { uint16_t* const o = (uint16_t*)P.ob + row * P.ob_pitch; store_chunk(o, at, n, in && on16(o + at), h[c]); }
+            }
+        }
+    }
+}
+
+/* rows of more than 32768 values, any alignment: read again for each of the steps (they stay in the caches) */
 template <int KIND, typename T>
 __global__ void __launch_bounds__(512) k_token_i8(const TokenI8 P) {
-    __shared__ float part[16];
+    __shared__ float part[2][32];
     const int64_t row = blockIdx.x;
     float rs = 0.0f;
     if (KIND == kRms) {
@@ -88,18 +353,17 @@ __global__ void __launch_bounds__(512) k_token_i8(const TokenI8 P) {
             if (r) { v = narrow(v + ld1(r + i), r); st1(r + i, v); }
             ss = fmaf(v, v, ss);
         }
-        ss = block_reduce(ss, part, [](float a, float b) { return a + b; });
+        ss = block_reduce(ss, part[0], [](float a, float b) { return a + b; });
         rs = 1.0f / sqrtf(ss / (float)P.n + P.eps);
     }
     float amax = 0.0f;
-    for (int i = threadIdx.x; i < P.n; i += blockDim.x) amax = max_nan(amax, value_of<KIND, T>(P, row, i, rs));
-    amax = block_reduce(amax, part, max_nan);
-    const bool zero = amax < 0x1p-100f;
-    const float step = zero ? 0.0f : 127.0f / amax;
-    if (threadIdx.x == 0) P.scale[row * P.s_pitch] = zero ? 1.0f : amax / 127.0f;
+    for (int i = threadIdx.x; i < P.n; i += blockDim.x) amax = max_nan(amax, fabsf(value_of<KIND, T>(P, row, i, rs)));
+    amax = block_reduce(amax, part[1], max_nan);
+    const float step = step_of(amax);
+    if (threadIdx.x == 0) P.scale[row * P.s_pitch] = scale_of(amax);
     for (int i = threadIdx.x; i < P.n; i += blockDim.x) {
         const float h = value_of<KIND, T>(P, row, i, rs);
-        P.q[row * P.q_pitch + i] = (int8_t)max(-127, min(127, __float2int_rn(h * step)));
+        P.q[row * P.q_pitch + i] = step == 0.0f ? (int8_t)0 : (int8_t)(__float_as_uint(fmaf(h, step, kCode)) & 0xffu);
         if (P.ob) {
             if (P.ob_f32) ((float*)P.ob)[row * P.ob_pitch + i] = h;
             else ((uint16_t*)P.ob)[row * P.ob_pitch + i] = f32_to_bf16(h);
@@ -107,13 +371,56 @@ __global__ void __launch_bounds__(512) k_token_i8(const TokenI8 P) {
     }
 }
 
+template <int KIND, typename T, int C, bool GRID>
+int launch_rows(const TokenI8& P, int rows, int threads, cudaStream_t st) {
+    const int one = KIND == kQuant || (KIND == kRms && !P.res), smem = threads * C * 8 * (int)sizeof(T) * (one ? 1 : 2);
+    const auto kernel = k_token_i8_regs<KIND, T, C, GRID>;
+    static std::atomic<int> fits[33][2];                          /* resident blocks of the device, by warps a block and streams */
+    std::atomic<int>& known = fits[threads / 32][one];
+    int grid = known.load(std::memory_order_relaxed);
+    if (!grid) {
+        int per = 0, dev = 0, sms = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem) != cudaSuccess ||
+            cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+            return RAD_E_DEVICE;
+        grid = (per > 0 ? per : 1) * sms;
+        known.store(grid, std::memory_order_relaxed);
+    }
+    kernel<<<(unsigned)(rows < grid ? rows : grid), threads, smem, st>>>(P);
+    return RAD_OK;
+}
+
+bool rows_on(const void* p, int64_t pitch, int esz, int grid) { return !p || (((uintptr_t)p | (uintptr_t)(pitch * esz)) & (uintptr_t)(grid - 1)) == 0; }
+
+template <int KIND, typename T, bool GRID>
+int launch_regs(const TokenI8& P, int rows, cudaStream_t st) {
+    const int most = P.n + (GRID ? 0 : 16 / (int)sizeof(T) - 1);  /* a row may begin anywhere inside its first 16 bytes */
+    /* Chunks a thread. Few rows: as many threads as the row has chunks (4 x 5120 norm: 2.6 us with one chunk a thread,
+     * 3.0 with two, 3.7 with four). Many rows: fewer threads, whose barriers cost less (8192 x 5120 norm: 62 / 51 / 53 us;
+     * 4099 x 5120 codes alone: 17.8 / 13.7 / 12.5 us; 8192 x 13824 gated: two 101, four 96 us; 16384 x 512 codes:
+     * 8.7 / 7.3 / 8.2 us). */
+    int c = most <= 8192 ? 1 : most <= 16384 ? 2 : 4;
+    if (rows > 2 * 148 && c < 4) c = KIND != kRms && most > 4096 ? 4 : most > 256 ? 2 : 1;
+    const int t = ((most + 8 * c - 1) / (8 * c) + 31) / 32 * 32;
+    return c == 1 ? launch_rows<KIND, T, 1, GRID>(P, rows, t, st) : c == 2 ? launch_rows<KIND, T, 2, GRID>(P, rows, t, st)
+                                                                             : launch_rows<KIND, T, 4, GRID>(P, rows, t, st);
+}
+
+template <int KIND, typename T>
+int launch_type(const TokenI8& P, int rows, cudaStream_t st) {
+    count_launch();
+    const int esz = (int)sizeof(T);
+    const bool grid = P.n % 8 == 0 && rows_on(P.x, P.x_pitch, esz, 16) && rows_on(P.res, P.r_pitch, esz, 16) && rows_on(P.w, 0, 1, 16) &&
+                      rows_on(P.q, P.q_pitch, 1, 8);
+    int rc = RAD_OK;
+    if (P.n > 32760) k_token_i8<KIND, T><<<(unsigned)rows, 512, 0, st>>>(P);
+    else rc = grid ? launch_regs<KIND, T, true>(P, rows, st) : launch_regs<KIND, T, false>(P, rows, st);
+    return rc != RAD_OK ? rc : cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
+}
 template <int KIND>
 int launch_kind(const TokenI8& P, int x_f32, int rows, cudaStream_t st) {
-    const int t = P.n >= 512 ? 512 : (P.n + 31) / 32 * 32;
-    count_launch();
-    if (x_f32) k_token_i8<KIND, float><<<(unsigned)rows, t, 0, st>>>(P);
-    else k_token_i8<KIND, uint16_t><<<(unsigned)rows, t, 0, st>>>(P);
-    return cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
+    return x_f32 ? launch_type<KIND, float>(P, rows, st) : launch_type<KIND, uint16_t>(P, rows, st);
 }
 
 } /* namespace */
@@ -124,7 +431,7 @@ int launch_token_i8(const R3dTokenI8& p, cudaStream_t st) {
     P.w = p.w; P.w_f32 = p.w_dtype == RAD_F32;
     P.q = (int8_t*)p.q; P.q_pitch = p.q_pitch; P.scale = p.scale; P.s_pitch = p.s_pitch;
     P.ob = p.out; P.ob_f32 = p.out_dtype == RAD_F32; P.ob_pitch = p.out_pitch;
-    P.n = p.n; P.eps = p.eps; P.wadd = p.wadd;
+    P.n = p.n; P.rows = p.rows; P.eps = p.eps; P.wadd = p.wadd;
     const int f32 = p.x_dtype == RAD_F32;
     switch (p.kind) {
         case R3D_TOKEN_QUANT:   return launch_kind<kQuant>(P, f32, p.rows, st);
