@@ -73,9 +73,27 @@ __device__ __forceinline__ double exponent_of(const Row& R, uint32_t key) {
     if (R.inf) return isinf(x) ? 0.0 : -HUGE_VAL;
     return (x - R.mx) * R.c;
 }
+/* 2^(exponent + S), rounded to a whole number: 2^n times the Taylor series of 2^r, |r| <= 1/2, to the eleventh power
+ * (its remainder is below 2^-47; 2^0 is 1 exactly), rounded by adding 2^52. */
 __device__ __forceinline__ u64 weight_of(const Row& R, uint32_t key) {
-    if (!key) return 0;
-    return (u64)__double2ull_rn(exp2(exponent_of(R, key) + R.S));
+    const double z = exponent_of(R, key) + R.S;
+    if (!key || !(z > -1.5)) return 0;
+    const double whole = z + 6755399441055744.0;                  /* 1.5 * 2^52: the nearest whole number in the low word */
+    const double r = z - (whole - 6755399441055744.0);
+    double p = 4.445538271870811e-10;                             /* ln(2)^i / i!, i = 11 .. 0 */
+    p = fma(p, r, 7.054911620801122e-09);
+    p = fma(p, r, 1.0178086009239699e-07);
+    p = fma(p, r, 1.3215486790144307e-06);
+    p = fma(p, r, 1.5252733804059841e-05);
+    p = fma(p, r, 1.5403530393381608e-04);
+    p = fma(p, r, 1.3333558146428443e-03);
+    p = fma(p, r, 9.618129107628477e-03);
+    p = fma(p, r, 5.5504108664821576e-02);
+    p = fma(p, r, 0.2402265069591007);
+    p = fma(p, r, 0.6931471805599453);
+    p = fma(p, r, 1.0);
+    const double scaled = __hiloint2double(__double2hiint(p) + (__double2loint(whole) << 20), __double2loint(p));
+    return (u64)__double_as_longlong(scaled + 4503599627370496.0) - 0x4330000000000000ull;
 }
 
 __device__ __forceinline__ float logprob_of(const Row& R, uint32_t key, u64 total) {
@@ -83,7 +101,7 @@ __device__ __forceinline__ float logprob_of(const Row& R, uint32_t key, u64 tota
 }
 
 struct Sum { int n; u64 w; };
-struct Sum3 { u64 w[3]; int n[3]; };
+struct Sum3 { u64 w[3]; };
 
 __device__ Sum block_sum(Sum v, Sum* part) {
 #pragma unroll
@@ -185,19 +203,23 @@ __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
 
 /* ------------------------------------------------------------------ a cluster a row
  * The row is read once, as ordered keys into the shared memory of the cluster's CTAs; a thread owns `e` neighbouring ids
- * (an odd number: its reads fall into banks of their own), so id order is the order of threads. What the CTAs find out
- * goes to all of them through distributed shared memory: the largest key; a histogram of the distance to it in
- * kBins steps over the range of distances that have any weight; sums.
- *   - Filters that leave few: the steps of the histogram that hold k tokens, or surely p of the weight, are gathered
- *     in the first CTA, up to kCap tokens, sorted there, cut and summed.
- *   - Filters that leave many: the last kept key is searched, three probes of exact sums a round.
- *   - None: the running weight alone.
- * Latency bounds it (a round through the cluster is about a microsecond), and for rows without top-k the 64-bit
- * exponential of every token. */
-constexpr int kT = 512;
-constexpr int kBins = 4096;
+ * (an odd number of words: its reads fall into banks of their own), so id order is the order of threads. What the CTAs
+ * find out goes to all of them through distributed shared memory.
+ *   - Top-k of a few: every quarter of a warp knows the largest key it read. The k-th largest of these is a bound that
+ *     at least k tokens reach, and hardly more: they are gathered in the first CTA, sorted, cut and summed there.
+ *     Two rounds through the cluster, and no work on the other tokens but reading them.
+ *   - Top-p alone, or a k beyond that: a histogram of the distance to the largest logit, with counts and exact
+ *     weights, tells the step in which the last kept token lies; the tokens of that step are gathered and sorted, and
+ *     the key and the number of ties at which it ends goes back to all.
+ *   - More tokens in one step than can be gathered (a flat row): the key is searched by exact sums, three probes a round.
+ * The answer among the kept ones follows from running weights by id. Latency bounds single rows (a round through the
+ * cluster is about a microsecond); rows without top-k need the 64-bit exponential of every token. */
+constexpr int kT = 1024, kWarps = kT / 32;
+constexpr int kBins = 2048;
 constexpr int kCap = 2048;
 constexpr int kMaxCluster = 16;
+constexpr int kGroups = 4 * kWarps;                               /* of eight threads */
+constexpr int kSel = 1024;                                        /* groups that are ranked, at most */
 constexpr double kRange = 44.0 * 0.6931471805599453;              /* distances with a weight, in temperatures: 2^-44 and up */
 
 struct Part { u64 w[3]; u64 key; int n[3]; int pad; };
@@ -205,13 +227,16 @@ struct Part { u64 w[3]; u64 key; int n[3]; int pad; };
 struct Shared {
     Part parts[2][kMaxCluster];                                   /* what each CTA says, by turns */
     Part mine;
-    u64 warp_w[kT / 32];
-    int warp_n[kT / 32];
-    Sum3 sums[kT / 32];
-    u64 list[kCap];
-    uint32_t hist[kBins], merged[kBins];
-    int gathered, pick[2];
-    float edge[2];
+    u64 warp_w[kWarps];
+    int warp_n[kWarps];
+    Sum3 sums[kWarps];
+    uint32_t my_tops[kGroups], sel[kSel];
+    int gathered, pick;
+    u64 found;
+    union { u64 list[kCap]; u64 hist_w[kBins]; };                 /* gathered tokens; this CTA's histogram */
+    union { uint32_t tops[kMaxCluster][kGroups]; uint32_t hist_n[kBins]; };   /* the groups' largest keys */
+    u64 all_w[kBins];                                             /* the cluster's histogram */
+    uint32_t all_n[kBins];
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -222,9 +247,14 @@ __device__ __forceinline__ uint32_t peer_addr(const void* p, int rank) {
 }
 __device__ __forceinline__ void peer_put(uint32_t at, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
 __device__ __forceinline__ void peer_put(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
-__device__ __forceinline__ uint32_t peer_get(uint32_t at) {
+__device__ __forceinline__ uint32_t peer_get32(uint32_t at) {
     uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ u64 peer_get64(uint32_t at) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at));
     return v;
 }
 __device__ __forceinline__ void meet() {                          /* of the cluster; orders what was put before it */
@@ -232,12 +262,12 @@ __device__ __forceinline__ void meet() {                          /* of the clus
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-/* one row's state, the same in every thread of the cluster */
+/* the cluster, the same in every thread of it */
 struct Cluster {
     Shared* s;
     int size, rank, turn;
 
-    /* every CTA's `mine` to every CTA; parts() is valid until the turn after next */
+    /* every CTA's `mine` to every CTA, and with it what the threads put before; parts are valid until the turn after next */
     __device__ __forceinline__ const Part* exchange() {
         __syncthreads();
         constexpr int kWords = sizeof(Part) / 8;
@@ -251,61 +281,55 @@ struct Cluster {
     /* sums over the cluster */
     __device__ __forceinline__ Sum3 sum(Sum3 v) {
 #pragma unroll
-        for (int j = 0; j < 3; ++j) {
-            v.n[j] = __reduce_add_sync(0xffffffffu, v.n[j]);
+        for (int j = 0; j < 3; ++j)
 #pragma unroll
             for (int o = 16; o; o >>= 1) v.w[j] += __shfl_xor_sync(0xffffffffu, v.w[j], o);
-        }
         if ((threadIdx.x & 31) == 0) s->sums[threadIdx.x >> 5] = v;
         __syncthreads();
-        if (threadIdx.x < 6) {
-            const int j = threadIdx.x % 3;
-            u64 w = 0; int n = 0;
-            for (int i = 0; i < kT / 32; ++i) { w += s->sums[i].w[j]; n += s->sums[i].n[j]; }
-            if (threadIdx.x < 3) s->mine.w[j] = w; else s->mine.n[j] = n;
+        if (threadIdx.x < 32) {
+            v = s->sums[threadIdx.x];
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+#pragma unroll
+                for (int o = 16; o; o >>= 1) v.w[j] += __shfl_xor_sync(0xffffffffu, v.w[j], o);
+            if (threadIdx.x < 3) s->mine.w[threadIdx.x] = v.w[threadIdx.x];
         }
         const Part* p = exchange();
         Sum3 all{};
         for (int r = 0; r < size; ++r)
 #pragma unroll
-            for (int j = 0; j < 3; ++j) { all.n[j] += p[r].n[j]; all.w[j] += p[r].w[j]; }
+            for (int j = 0; j < 3; ++j) all.w[j] += p[r].w[j];
         return all;
     }
 };
 
 /* exclusive over the block's threads, in their order; *total over all of them */
-__device__ __forceinline__ u64 scan_w(Shared* s, u64 v, u64* total) {
+template <typename V>
+__device__ __forceinline__ V scan(V* warps, V v, V* total) {
+    static_assert(kWarps == 32, "one lane a warp");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    u64 x = v;
+    V x = v;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const u64 y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+    for (int o = 1; o < 32; o <<= 1) { const V y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
     __syncthreads();
-    if (lane == 31) s->warp_w[warp] = x;
+    if (lane == 31) warps[warp] = x;
     __syncthreads();
-    u64 before = 0, all = 0;
-    for (int i = 0; i < kT / 32; ++i) { if (i < warp) before += s->warp_w[i]; all += s->warp_w[i]; }
-    *total = all;
-    return before + x - v;
-}
-__device__ __forceinline__ int scan_n(Shared* s, int v, int* total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    V all = warps[lane];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
-    __syncthreads();
-    if (lane == 31) s->warp_n[warp] = x;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < kT / 32; ++i) { if (i < warp) before += s->warp_n[i]; all += s->warp_n[i]; }
-    *total = all;
-    return before + x - v;
+    for (int o = 1; o < 32; o <<= 1) { const V y = __shfl_up_sync(0xffffffffu, all, o); if (lane >= o) all += y; }
+    *total = __shfl_sync(0xffffffffu, all, 31);
+    const V before = __shfl_sync(0xffffffffu, all, max(warp - 1, 0));
+    return (warp ? before : 0) + x - v;
 }
 
-/* n2 (a power of two) words, largest first */
+/* n2 (a power of two, 32 at least) words, largest first: the first warp alone where it can keep two a lane */
 __device__ __forceinline__ void sort_desc(u64* a, int n2) {
+    const bool one_warp = n2 <= 64;
+    __syncthreads();
+    if (one_warp && threadIdx.x >= 32) { __syncthreads(); return; }
     for (int k = 2; k <= n2; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
-            __syncthreads();
+            if (one_warp) __syncwarp(); else __syncthreads();
             for (int i = threadIdx.x; i < n2 / 2; i += kT) {
                 const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
                 const u64 x = a[lo], y = a[hi];
@@ -315,50 +339,69 @@ __device__ __forceinline__ void sort_desc(u64* a, int n2) {
     __syncthreads();
 }
 
+/* a token's key as it is kept: a bf16 key is the upper half of its f32 one */
+template <typename K> __device__ __forceinline__ uint32_t wide(K k);
+template <> __device__ __forceinline__ uint32_t wide<uint32_t>(uint32_t k) { return k; }
+template <> __device__ __forceinline__ uint32_t wide<uint16_t>(uint16_t k) { return k & 0x8000u ? (uint32_t)k << 16 : k ? (uint32_t)k << 16 | 0xffffu : 0u; }
+
+template <typename K>
 __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const int e) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared* const s = (Shared*)raw;
-    uint32_t* const keys = (uint32_t*)(raw + sizeof(Shared));
+    K* const keys = (K*)(raw + sizeof(Shared));
     Cluster cl;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cl.size));
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cl.rank));
     cl.s = s; cl.turn = 0;
     const int64_t m = blockIdx.x / cl.size;
     const int V = P.n_vocab, base = cl.rank * kT * e, tid = threadIdx.x;
-    uint32_t* const own = keys + tid * e;                         /* ids base + tid * e ... */
+    const K* const own = keys + tid * e;                          /* ids own_id ... own_id + e - 1 */
     const int own_id = base + tid * e;
+    /* the peers' shared memory may be written once they have all begun: waited for below */
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
     const float t = P.temperature ? P.temperature[m * P.t_pitch] : 1.0f, p = P.top_p ? P.top_p[m * P.p_pitch] : 1.0f;
     const float low = P.min_p ? P.min_p[m * P.mp_pitch] : 0.0f, u = P.u[m * P.u_pitch];
     int k = P.top_k ? P.top_k[m * P.k_pitch] : 0;
 
-    /* the peers' shared memory may be written once they have all begun: waited for below */
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-
     /* ---- read the row; its largest key, the lowest id that has it, and how many are not masked */
     u64 best_id = 0;
+    uint32_t top = 0;                                             /* the largest key this thread read */
     int live = 0;
+    {
+        int at = -1;
+        const int here = min(e, (V - base - tid + kT - 1) / kT);  /* negative: none */
 #pragma unroll 8
-    for (int j = 0; j < e; ++j) {
-        const int i = j * kT + tid, id = base + i;
-        const uint32_t key = id < V ? key_of(load_x(P, m, id)) : 0u;
-        keys[i] = key;
-        live += key != 0;
-        if (key) best_id = max(best_id, (u64)key << 32 | (0xffffffffu - (uint32_t)id));
+        for (int j = 0; j < here; ++j) {
+            const uint32_t key = key_of(load_x(P, m, base + j * kT + tid));
+            keys[j * kT + tid] = (K)(sizeof(K) == 2 ? key >> 16 : key);
+            live += key != 0;
+            if (key > top) { top = key; at = j; }
+        }
+        for (int j = max(here, 0); j < e; ++j) keys[j * kT + tid] = 0;
+        if (top) best_id = (u64)top << 32 | (0xffffffffu - (uint32_t)(base + at * kT + tid));
     }
-    for (int i = tid; i < kBins; i += kT) s->hist[i] = 0;
+    {
+        uint32_t g = top;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if ((tid & 7) == 0) s->my_tops[tid >> 3] = g;
+    }
     if (tid == 0) s->gathered = 0;
     live = __reduce_add_sync(0xffffffffu, live);
 #pragma unroll
     for (int o = 16; o; o >>= 1) best_id = max(best_id, (u64)__shfl_xor_sync(0xffffffffu, best_id, o));
     if ((tid & 31) == 0) { s->warp_w[tid >> 5] = best_id; s->warp_n[tid >> 5] = live; }
     __syncthreads();
-    if (tid == 0) {
-        u64 b = 0; int n = 0;
-        for (int i = 0; i < kT / 32; ++i) { b = max(b, s->warp_w[i]); n += s->warp_n[i]; }
-        s->mine.key = b; s->mine.n[0] = n;
+    if (tid < 32) {
+        best_id = s->warp_w[tid];
+        live = __reduce_add_sync(0xffffffffu, s->warp_n[tid]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) best_id = max(best_id, (u64)__shfl_xor_sync(0xffffffffu, best_id, o));
+        if (tid == 0) { s->mine.key = best_id; s->mine.n[0] = live; }
     }
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    for (int i = tid; i < kGroups * cl.size; i += kT) peer_put(peer_addr(&s->tops[cl.rank][i % kGroups], i / kGroups), s->my_tops[i % kGroups]);
     {
         const Part* parts = cl.exchange();
         best_id = 0; live = 0;
@@ -378,113 +421,77 @@ __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const in
     const Row R = row_of(best, t, P.shift);
     const double floor_y = floor_of(low);
     const bool by_k = k < live, by_p = p < 1.0f;
+    /* `n` tokens of this thread that `pick` says, to the list of the first CTA, in any order */
+    const auto gather = [&](auto pick) {
+        int n = 0, n_cta;
+        for (int j = 0; j < e; ++j) { const uint32_t key = wide(own[j]); n += key && pick(key); }
+        int at = scan(s->warp_n, n, &n_cta);
+        if (tid == 0) {
+            uint32_t from;
+            asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(from) : "r"(peer_addr(&s->gathered, 0)), "r"(n_cta) : "memory");
+            s->pick = (int)from;
+        }
+        __syncthreads();
+        at += s->pick;
+        for (int j = 0; j < e && n; ++j) {
+            const uint32_t key = wide(own[j]);
+            if (!key || !pick(key)) continue;
+            if (at < kCap) peer_put(peer_addr(&s->list[at], 0), (u64)key << 32 | (0xffffffffu - (uint32_t)(own_id + j)));
+            ++at; --n;
+        }
+    };
 
-    uint32_t cut = 1;                                             /* kept: keys above cut, and the first `ties` equal to it */
-    int ties = V;
-    if (by_k || by_p) {
-        /* ---- histogram of the distance to the largest logit (key order and step order agree) */
-        const float mx = val_of(best), inv = (float)((kBins - 1) / kRange) / t;
-        const auto bin_of = [&](uint32_t key) {
-            if (R.inf) return key == best ? 0 : kBins - 1;
-            const float d = __fsub_rn(mx, val_of(key)) * inv;
-            return d < (float)(kBins - 1) ? (int)d : d >= (float)(kBins - 1) ? kBins - 1 : 0;     /* not a number: 0 * inf, every weight is 1 */
-        };
-        u64 mass = 0;
-        for (int j = 0; j < e; ++j) {
-            const uint32_t key = own[j];
-            if (!key) continue;
-            atomicAdd(&s->hist[bin_of(key)], 1u);
-            if (!by_k) mass += weight_of(R, key);
+    /* ---- top-k of a few */
+    int sel = 128;                                                /* groups to rank: at least four times k */
+    while (sel < 4 * k && sel <= kSel) sel *= 2;
+    if (by_k && sel <= min(kSel, kGroups * cl.size)) {
+        /* the k-th largest of the groups' keys, neighbours taken together down to `sel` groups */
+        const int of = kGroups * cl.size / sel, share = kT / sel;     /* threads a group */
+        const uint32_t* const tops = &s->tops[0][0];
+        if (tid < sel) {
+            uint32_t g = 0;
+            for (int j = 0; j < of; ++j) g = max(g, tops[tid * of + j]);
+            s->sel[tid] = g;
         }
-        /* the total, which top-p alone is a share of, goes along */
-        Sum3 v{};
-        v.w[0] = mass;
-        const u64 total = cl.sum(v).w[0];                         /* also: every CTA's histogram is complete */
-        const int seg = kBins / cl.size;
-        for (int i = tid; i < seg; i += kT) {
-            const int b = cl.rank * seg + i;
-            uint32_t n = 0;
-            for (int r = 0; r < cl.size; ++r) n += peer_get(peer_addr(&s->hist[b], r));
-            for (int r = 0; r < cl.size; ++r) peer_put(peer_addr(&s->merged[b], r), n);
+        __syncthreads();
+        const uint32_t mine = s->sel[tid / share];
+        int larger = 0;
+        for (int j = tid % share * 4; j < sel; j += share * 4) {
+            const uint4 o = *(const uint4*)&s->sel[j];
+            larger += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
         }
+        for (int o = 1; o < share; o <<= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
+        /* fewer than k groups lie above it: the least such key is the k-th largest */
+        uint32_t bound = __reduce_min_sync(0xffffffffu, larger < k ? mine : 0xffffffffu);
+        if ((tid & 31) == 0) s->warp_n[tid >> 5] = (int)bound;
+        __syncthreads();
+        bound = __reduce_min_sync(0xffffffffu, (uint32_t)s->warp_n[tid & 31]);
+        gather([&](uint32_t key) { return key >= bound; });
         meet();
-        /* ---- the steps that hold the first k tokens, or surely p of the weight: a token of step b weighs at least what
-         * the end of its step does (less a little for the rounding of b) */
-        constexpr int kEach = kBins / kT;
-        int n_own = 0; float low_own = 0.0f;
-        uint32_t cnt[kEach];
-        const float per_bin = (float)(kRange / (kBins - 1) * 1.4426950408889634);    /* halvings a step */
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            cnt[j] = s->merged[tid * kEach + j];
-            n_own += (int)cnt[j];
-            low_own += (float)cnt[j] * exp2f(-per_bin * (float)(tid * kEach + j + 1)) * 0.999f;
-        }
-        int all_n; u64 all_w;
-        int n_before = scan_n(s, n_own, &all_n);
-        const u64 low_before = scan_w(s, (u64)(low_own * 0x1p24f), &all_w);     /* rounded down, and again below */
-        const u64 need_low = by_k ? 0 : (u64)((double)want_of(p, total) * exp2((double)(24 - R.S))) + 1;
-        if (tid == 0) { s->pick[0] = kBins; s->pick[1] = 0; }
-        __syncthreads();
-        u64 low_run = low_before;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const int b = tid * kEach + j;
-            const int n_after = n_before + (int)cnt[j];
-            if (by_k) { if (n_before < k && n_after >= k) { s->pick[0] = b; s->pick[1] = n_after; } }
-            else if (cnt[j]) {
-                const u64 after = low_run + (u64)((float)cnt[j] * exp2f(-per_bin * (float)(b + 1)) * 0.999f * 0x1p24f);
-                if (after >= need_low && b < kBins - 1) atomicMin(&s->pick[0], b);
-                low_run = after;
-            }
-            n_before = n_after;
-        }
-        __syncthreads();
-        const int top = s->pick[0];
-        int n_top = by_k ? s->pick[1] : 0;
-        if (!by_k && top < kBins) {                               /* how many the chosen steps hold */
-            int n = 0;
-#pragma unroll
-            for (int j = 0; j < kEach; ++j) if (tid * kEach + j <= top) n += (int)cnt[j];
-            scan_n(s, n, &n_top);
-        }
-        if (top < kBins && n_top <= kCap) {
-            /* ---- few: to the first CTA, in any order */
-            int n = 0, n_cta;
-            for (int j = 0; j < e; ++j) n += own[j] && bin_of(own[j]) <= top;
-            int at = scan_n(s, n, &n_cta);
-            if (tid == 0) {
-                uint32_t from;
-                asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(from) : "r"(peer_addr(&s->gathered, 0)), "r"(n_cta) : "memory");
-                s->pick[0] = (int)from;
-            }
-            __syncthreads();
-            at += s->pick[0];
-            for (int j = 0; j < e && n; ++j)
-                if (own[j] && bin_of(own[j]) <= top)
-                    peer_put(peer_addr(&s->list[at++], 0), (u64)own[j] << 32 | (0xffffffffu - (uint32_t)(own_id + j)));
+        const int n_top = (int)peer_get32(peer_addr(&s->gathered, 0));
+        if (bound && n_top <= kCap) {
+            if (!first_cta) { meet(); return; }                   /* the first CTA's memory outlives the reads of it, too */
             meet();
-            if (!first_cta) return;
             int n2 = 32;
             while (n2 < n_top) n2 <<= 1;
             for (int i = n_top + tid; i < n2; i += kT) s->list[i] = 0;
             sort_desc(s->list, n2);
             const int each = (n2 + kT - 1) / kT, i0 = tid * each;
-            const auto weight_at = [&](int i) { return i < n2 ? weight_of(R, (uint32_t)(s->list[i] >> 32)) : 0ull; };
             u64 w = 0, sum, dummy;
-            for (int i = i0; i < i0 + each; ++i) if (i < k) w += weight_at(i);
-            u64 before = scan_w(s, w, &sum);
-            const u64 want = by_p ? want_of(p, by_k ? sum : total) : ~0ull;
+            for (int i = i0; i < i0 + each && i < k; ++i) w += i < n_top ? weight_of(R, (uint32_t)(s->list[i] >> 32)) : 0ull;
+            u64 before = scan(s->warp_w, w, &sum);
+            const u64 want = by_p ? want_of(p, sum) : ~0ull;
             int kept = 0;
             w = 0;
             for (int i = i0; i < i0 + each && i < k && i < n_top; ++i) {
-                const u64 x = weight_at(i);
-                if (i && (before >= want || exponent_of(R, (uint32_t)(s->list[i] >> 32)) < floor_y)) break;
+                const uint32_t key = (uint32_t)(s->list[i] >> 32);
+                if (i && (before >= want || exponent_of(R, key) < floor_y)) break;
+                const u64 x = weight_of(R, key);
                 before += x; w += x; ++kept;
             }
             int n_kept;
-            scan_n(s, kept, &n_kept);
-            scan_w(s, w, &sum);
+            scan(s->warp_n, kept, &n_kept);
+            scan(s->warp_w, w, &sum);
             /* by id, ascending: the low words are 0xffffffff - id; the key moves below */
             n2 = 32;
             while (n2 < n_kept) n2 <<= 1;
@@ -493,7 +500,7 @@ __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const in
             w = 0;
             const int each2 = (n2 + kT - 1) / kT, j0 = tid * each2;
             for (int i = j0; i < j0 + each2 && i < n_kept; ++i) w += weight_of(R, (uint32_t)s->list[i]);
-            before = scan_w(s, w, &dummy);
+            before = scan(s->warp_w, w, &dummy);
             const u64 point = point_of(u, sum);
             for (int i = j0; i < j0 + each2 && i < n_kept; ++i) {
                 const uint32_t key = (uint32_t)s->list[i];
@@ -504,17 +511,110 @@ __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const in
             }
             return;
         }
-        /* ---- many: the largest key c with enough tokens (weight) from c on. enough(sum over keys in [c, hi)) */
-        const auto search = [&](uint32_t lo, uint32_t hi, u64 need, u64* above, auto value) {
+    }
+
+    uint32_t cut = 1;                                             /* kept: keys above cut, and the first `ties` equal to it */
+    int ties = V;
+    if (by_k || by_p) {
+        /* ---- histogram of the distance to the largest logit (key order and step order agree) */
+        __syncthreads();
+        for (int i = tid; i < kBins; i += kT) { s->hist_n[i] = 0; s->hist_w[i] = 0; }
+        __syncthreads();
+        const float mx = val_of(best), inv = (float)((kBins - 1) / kRange) / t;
+        const auto bin_of = [&](uint32_t key) {
+            if (R.inf) return key == best ? 0 : kBins - 1;
+            const float d = __fsub_rn(mx, val_of(key)) * inv;
+            return d < (float)(kBins - 1) ? (int)d : d >= (float)(kBins - 1) ? kBins - 1 : 0;     /* not a number: 0 * inf, every weight is 1 */
+        };
+#pragma unroll 2
+        for (int j = 0; j < e; ++j) {
+            const uint32_t key = wide(own[j]);
+            if (!key) continue;
+            const int b = bin_of(key);
+            atomicAdd(&s->hist_n[b], 1u);
+            if (by_p) {
+                const u64 x = weight_of(R, key);
+                if (x) atomicAdd(&s->hist_w[b], x);
+            }
+        }
+        __syncthreads();
+        meet();
+        const int seg = kBins / cl.size;
+        for (int i = tid; i < seg; i += kT) {
+            const int b = cl.rank * seg + i;
+            uint32_t ns[kMaxCluster], n = 0;
+            u64 ws[kMaxCluster], w = 0;
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) if (r < cl.size) { ns[r] = peer_get32(peer_addr(&s->hist_n[b], r)); ws[r] = peer_get64(peer_addr(&s->hist_w[b], r)); }
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) if (r < cl.size) { n += ns[r]; w += ws[r]; }
+            for (int r = 0; r < cl.size; ++r) { peer_put(peer_addr(&s->all_n[b], r), n); peer_put(peer_addr(&s->all_w[b], r), w); }
+        }
+        meet();
+        static_assert(kBins == 2 * kT, "two steps a thread");
+        const uint32_t n0 = s->all_n[2 * tid], n1 = s->all_n[2 * tid + 1];
+        const u64 w0 = s->all_w[2 * tid], w1 = s->all_w[2 * tid + 1];
+        int live2; u64 total;
+        const int n_before = scan(s->warp_n, (int)(n0 + n1), &live2);
+        const u64 w_before = scan(s->warp_w, w0 + w1, &total);
+        /* the step whose running count (weight) first reaches `need`, and what lies before it */
+        const auto step_at = [&](u64 before, u64 a, u64 b, u64 need, u64* above) {
+            __syncthreads();
+            if (before < need && before + a + b >= need) {
+                const bool second = before + a < need;
+                s->pick = 2 * tid + second;
+                s->found = second ? before + a : before;
+            }
+            __syncthreads();
+            *above = s->found;
+            return s->pick;
+        };
+        /* the largest key c of a step such that above + the value of the step's keys from c on reaches `need`; *above
+         * moves on to what lies over c. The step's tokens are gathered and sorted, or the key is searched */
+        const auto key_at = [&](int step, uint32_t least, u64 need, u64* above, auto value) {
+            meet();
+            if (first_cta && tid == 0) s->gathered = 0;
+            meet();
+            gather([&](uint32_t key) { return key >= least && bin_of(key) == step; });
+            meet();
+            const int n = (int)peer_get32(peer_addr(&s->gathered, 0));
+            if (n <= kCap) {
+                if (first_cta) {
+                    int n2 = 32;
+                    while (n2 < n) n2 <<= 1;
+                    for (int i = n + tid; i < n2; i += kT) s->list[i] = 0;
+                    sort_desc(s->list, n2);
+                    const int each = (n2 + kT - 1) / kT, i0 = tid * each;
+                    u64 v = 0, all;
+                    for (int i = i0; i < i0 + each && i < n; ++i) v += value((uint32_t)(s->list[i] >> 32));
+                    u64 run = *above + scan(s->warp_w, v, &all);
+                    for (int i = i0; i < i0 + each && i < n; ++i) {
+                        const uint32_t key = (uint32_t)(s->list[i] >> 32);
+                        const u64 x = value(key);
+                        if (run < need && run + x >= need) {
+                            int over = i;                          /* ties of it may stand before it */
+                            u64 then = run;
+                            while (over > 0 && (uint32_t)(s->list[over - 1] >> 32) == key) { --over; then -= x; }
+                            s->mine.key = key; s->mine.w[0] = then;
+                        }
+                        run += x;
+                    }
+                }
+                const Part* parts = cl.exchange();
+                *above = parts[0].w[0];
+                return (uint32_t)parts[0].key;
+            }
+            uint32_t lo = least, hi = best + 1;
+            u64 over = 0;                                         /* of the step's keys from hi on */
             while (hi - lo > 1) {
-                const uint32_t step = max(1u, (hi - lo) / 4);
+                const uint32_t d = max(1u, (hi - lo) / 4);
                 uint32_t c[3];
 #pragma unroll
-                for (int j = 0; j < 3; ++j) c[j] = min(lo + (j + 1) * step, hi);
+                for (int j = 0; j < 3; ++j) c[j] = min(lo + (j + 1) * d, hi);
                 Sum3 v3{};
                 for (int j = 0; j < e; ++j) {
-                    const uint32_t key = own[j];
-                    if (key < c[0] || key >= hi) continue;
+                    const uint32_t key = wide(own[j]);
+                    if (key < c[0] || key >= hi || bin_of(key) != step) continue;
                     const u64 x = value(key);
                     v3.w[0] += x;
                     if (key >= c[1]) v3.w[1] += x;
@@ -522,31 +622,35 @@ __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const in
                 }
                 v3 = cl.sum(v3);
                 int j = -1;
-                for (int i = 0; i < 3; ++i) if (c[i] < hi && *above + v3.w[i] >= need) j = i;
-                const uint32_t nhi = j < 2 ? c[j + 1] : hi;
-                if (j < 2 && nhi < hi) *above += v3.w[j + 1];
+                for (int i = 0; i < 3; ++i) if (c[i] < hi && *above + over + v3.w[i] >= need) j = i;
+                if (j < 2 && c[j + 1] < hi) { over += v3.w[j + 1]; hi = c[j + 1]; }
                 if (j >= 0) lo = c[j];
-                hi = nhi;
             }
+            *above += over;
             return lo;
         };
-        u64 above = 0;
+        u64 above;
         if (by_k) {
-            cut = search(1u, best + 1, (u64)k, &above, [](uint32_t) { return 1ull; });
+            const int step = step_at((u64)n_before, n0, n1, (u64)k, &above);
+            cut = key_at(step, 1u, (u64)k, &above, [](uint32_t) { return 1ull; });
             ties = (int)((u64)k - above);
         }
         if (by_p) {
-            Sum3 v3{};
-            for (int j = 0; j < e; ++j) if (own[j] > cut) v3.w[0] += weight_of(R, own[j]);
-            const u64 over = by_k ? cl.sum(v3).w[0] : total;
-            const u64 one = weight_of(R, cut), want = want_of(p, by_k ? over + (u64)ties * one : total);
-            above = 0;
+            u64 over = total;
+            if (by_k) {                                           /* the weight over the cut: whole steps, and the cut's own */
+                Sum3 v3{};
+                for (int j = 0; j < e; ++j) { const uint32_t key = wide(own[j]); if (key > cut) v3.w[0] += weight_of(R, key); }
+                over = cl.sum(v3).w[0];
+            }
+            const u64 want = want_of(p, by_k ? over + (u64)ties * weight_of(R, cut) : total);
+            above = over;
             if (!by_k || over >= want) {
-                cut = search(by_k ? cut : 1u, best + 1, want, &above, [&](uint32_t key) { return weight_of(R, key); });
+                const int step = step_at(w_before, w0, w1, want, &above);
+                cut = key_at(step, by_k ? cut : 1u, want, &above, [&](uint32_t key) { return weight_of(R, key); });
                 ties = V;
-            } else above = over;
-            const u64 one_cut = weight_of(R, cut);
-            if (one_cut && want > above) ties = (int)min((u64)ties, (want - above + one_cut - 1) / one_cut);
+            }
+            const u64 one = weight_of(R, cut);
+            if (one && want > above) ties = (int)min((u64)ties, (want - above + one - 1) / one);
         }
     }
 
@@ -554,40 +658,65 @@ __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const in
     int tie_rank = 0;
     if (ties < V) {
         int n = 0, n_cta;
-        for (int j = 0; j < e; ++j) n += own[j] == cut;
-        tie_rank = scan_n(s, n, &n_cta);
+        for (int j = 0; j < e; ++j) n += wide(own[j]) == cut;
+        tie_rank = scan(s->warp_n, n, &n_cta);
         if (tid == 0) s->mine.n[0] = n_cta;
         const Part* parts = cl.exchange();
         for (int r = 0; r < cl.rank; ++r) tie_rank += parts[r].n[0];
     }
-    const auto each_kept = [&](auto f) {
-        int rank = tie_rank;
-        for (int j = 0; j < e; ++j) {
-            const uint32_t key = own[j];
-            if (key < cut || !key || (key == cut && rank++ >= ties) || exponent_of(R, key) < floor_y) continue;
-            if (!f(j, key)) return;
-        }
-    };
+    int rank = tie_rank;
+    const bool by_low = low > 0.0f;
+    const auto kept = [&](uint32_t key) { return key >= cut && (key > cut || rank++ < ties) && (!by_low || exponent_of(R, key) >= floor_y); };
     u64 w = 0, w_cta;
     int n = 0, n_cta;
-    each_kept([&](int, uint32_t key) { w += weight_of(R, key); ++n; return true; });
-    u64 before = scan_w(s, w, &w_cta);
-    scan_n(s, n, &n_cta);
+#pragma unroll 2
+    for (int j = 0; j < e; ++j) {
+        const uint32_t key = wide(own[j]);
+        if (!kept(key)) continue;
+        w += weight_of(R, key);
+        ++n;
+    }
+    u64 before = scan(s->warp_w, w, &w_cta);
+    scan(s->warp_n, n, &n_cta);
     if (tid == 0) { s->mine.w[0] = w_cta; s->mine.n[0] = n_cta; }
     const Part* parts = cl.exchange();
-    u64 sum = 0; int kept = 0;
+    u64 sum = 0;
+    int n_kept = 0;
     for (int r = 0; r < cl.size; ++r) {
         if (r < cl.rank) before += parts[r].w[0];
-        sum += parts[r].w[0]; kept += parts[r].n[0];
+        sum += parts[r].w[0]; n_kept += parts[r].n[0];
     }
     const u64 point = point_of(u, sum);
-    if (before <= point && point < before + w)
-        each_kept([&](int j, uint32_t key) {
+    if (before <= point && point < before + w) {
+        rank = tie_rank;
+        for (int j = 0; j < e; ++j) {
+            const uint32_t key = wide(own[j]);
+            if (!kept(key)) continue;
             before += weight_of(R, key);
-            if (before <= point) return true;
-            answer(P, m, own_id + j, kept, logprob_of(R, key, sum));
-            return false;
-        });
+            if (before <= point) continue;
+            answer(P, m, own_id + j, n_kept, logprob_of(R, key, sum));
+            break;
+        }
+    }
+}
+
+template <typename K>
+int launch_row(const R3dNucleus& P, int size, int e, size_t smem, cudaStream_t st) {
+    static std::atomic<bool> set[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return RAD_E_DEVICE;
+    if (!set[dev].load(std::memory_order_relaxed)) {
+        if (cudaFuncSetAttribute(k_nucleus_row<K>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
+            cudaFuncSetAttribute(k_nucleus_row<K>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return RAD_E_DEVICE;
+        set[dev].store(true, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)P.rows * (unsigned)size); cfg.blockDim = dim3(kT); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)size; at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_nucleus_row<K>, P, e) == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
 }
 
 } /* namespace */
@@ -598,29 +727,21 @@ int launch_nucleus(const R3dNucleus& p, cudaStream_t st) {
     while ((1ll << bits) < (long long)p.n_vocab) ++bits;
     P.shift = 62 - bits < 50 ? 62 - bits : 50;
     count_launch();
-    int size = getenv("DEV_CL") ? atoi(getenv("DEV_CL")) : 8;
-    int e = (p.n_vocab + kT * size - 1) / (kT * size);
-    e |= 1;
-    const size_t smem = sizeof(Shared) + (size_t)kT * e * 4;
+    const int ksz = p.x_dtype == RAD_F32 ? 4 : 2;
+    int size = 1, e = 0;
+    size_t smem = 0;
+    for (;; size *= 2) {
+        e = ((p.n_vocab + kT * size - 1) / (kT * size)) | 1;
+        smem = sizeof(Shared) + (size_t)kT * e * ksz;
+        if (size == kMaxCluster) break;
+        if (smem <= 220 * 1024 && ((long long)p.rows * size >= 148 || kT * e <= 4096)) break;
+    }
+    if (getenv("DEV_CL")) { size = atoi(getenv("DEV_CL")); e = ((p.n_vocab + kT * size - 1) / (kT * size)) | 1; smem = sizeof(Shared) + (size_t)kT * e * ksz; }
     if (smem > 220 * 1024) {
         k_nucleus_long<<<(unsigned)p.rows, 1024, 0, st>>>(P);
         return cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
     }
-    static std::atomic<bool> set[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return RAD_E_DEVICE;
-    if (!set[dev].load(std::memory_order_relaxed)) {
-        if (cudaFuncSetAttribute(k_nucleus_row, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024) != cudaSuccess ||
-            cudaFuncSetAttribute(k_nucleus_row, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return RAD_E_DEVICE;
-        set[dev].store(true, std::memory_order_relaxed);
-    }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)p.rows * (unsigned)size); cfg.blockDim = dim3(kT); cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)size; at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_nucleus_row, P, e) == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
+    return ksz == 4 ? launch_row<uint32_t>(P, size, e, smem, st) : launch_row<uint16_t>(P, size, e, smem, st);
 }
 
 } /* namespace r3d */
