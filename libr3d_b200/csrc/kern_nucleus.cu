@@ -15,6 +15,7 @@
  */
 #include <atomic>
 #include <cmath>
+#include <cstddef>
 #include <cstdlib>
 #include "r3d_kernels.h"
 #include "r3d_numerics.cuh"
@@ -95,6 +96,45 @@ __device__ __forceinline__ u64 weight_of(const Row& R, uint32_t key) {
     const double scaled = __hiloint2double(__double2hiint(p) + (__double2loint(whole) << 20), __double2loint(p));
     return (u64)__double_as_longlong(scaled + 4503599627370496.0) - 0x4330000000000000ull;
 }
+
+/* The same with a table of 2^(i / 128) and the series to the fourth power (its remainder for r <= 2^-8 is below 2^-49):
+ * twelve operations of the 64-bit pipe, which does sixteen lanes a clock, instead of nineteen. A table of whole numbers and
+ * 64-bit products of them, seventy instructions, was no faster. */
+struct Powers { double of[128]; };
+constexpr Powers make_powers() {
+    Powers t{};
+    for (int i = 0; i < 128; ++i) {
+        const double x = 0.6931471805599453 * i / 128.0;
+        double sum = 1.0, term = 1.0;
+        for (int j = 1; j < 30; ++j) { term *= x / j; sum += term; }
+        t.of[i] = sum;
+    }
+    return t;
+}
+__device__ const Powers kPowers = make_powers();
+
+struct Weigh {
+    double mx, c;                                                 /* the largest logit; 128 log2(e) / T */
+    float top, limit;                                             /* the largest again; the distance from which nothing weighs */
+    int S;
+    bool inf;
+    __device__ __forceinline__ u64 of(const double* powers, uint32_t key) const {
+        const float x = val_of(key);
+        if (inf) return key && x == top ? 1ull << S : 0ull;
+        if (!key || !(__fsub_rn(top, x) <= limit)) return 0;
+        const double z = ((double)x - mx) * c, whole = z + 6755399441055744.0;       /* 1.5 * 2^52: the nearest whole number in the low word */
+        const double r = z - (whole - 6755399441055744.0);
+        const int j = __double2loint(whole);
+        constexpr double l = 0.6931471805599453 / 128.0;          /* the series of 2^(r / 128) */
+        double p = l * l * l * l / 24.0;
+        p = fma(p, r, l * l * l / 6.0);
+        p = fma(p, r, l * l / 2.0);
+        p = fma(p, r, l);
+        p = fma(p, r, 1.0) * powers[j & 127];
+        const double scaled = __hiloint2double(__double2hiint(p) + (((j >> 7) + S) << 20), __double2loint(p));
+        return (u64)__double_as_longlong(scaled + 4503599627370496.0) - 0x4330000000000000ull;
+    }
+};
 
 __device__ __forceinline__ float logprob_of(const Row& R, uint32_t key, u64 total) {
     return (float)(0.6931471805599453 * (exponent_of(R, key) + R.S) - log((double)total));
@@ -205,38 +245,42 @@ __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
  * The row is read once, as ordered keys into the shared memory of the cluster's CTAs; a thread owns `e` neighbouring ids
  * (an odd number of words: its reads fall into banks of their own), so id order is the order of threads. What the CTAs
  * find out goes to all of them through distributed shared memory.
- *   - Top-k of a few: every quarter of a warp knows the largest key it read. The k-th largest of these is a bound that
- *     at least k tokens reach, and hardly more: they are gathered in the first CTA, sorted, cut and summed there.
- *     Two rounds through the cluster, and no work on the other tokens but reading them.
- *   - Top-p alone, or a k beyond that: a histogram of the distance to the largest logit, with counts and exact
- *     weights, tells the step in which the last kept token lies; the tokens of that step are gathered and sorted, and
- *     the key and the number of ties at which it ends goes back to all.
- *   - More tokens in one step than can be gathered (a flat row): the key is searched by exact sums, three probes a round.
- * The answer among the kept ones follows from running weights by id. Latency bounds single rows (a round through the
- * cluster is about a microsecond); rows without top-k need the 64-bit exponential of every token. */
-constexpr int kT = 1024, kWarps = kT / 32;
-constexpr int kBins = 2048;
-constexpr int kCap = 2048;
+ *   - Top-k of a few: every eight threads know the largest key they read. The k-th largest of these is a bound that at
+ *     least k tokens reach, and hardly more: they are gathered in the first CTA, which ranks them, cuts and sums. Two
+ *     rounds through the cluster, and no work on the other tokens but reading them.
+ *   - Top-p alone, or a k beyond that: a histogram of the distance to the largest logit gives the exact step of the k-th
+ *     token, and for top-p a window of steps in which its end lies by the steps' middle weights; one pass of exact sums
+ *     proves the window (or moves it). The tokens of the window are gathered and ranked, and the key and the number of
+ *     ties at which the kept ones end goes back to all.
+ *   - More tokens in a window than can be gathered (a flat row): the key is searched by exact sums, three probes a round.
+ * The answer among the kept ones follows from running weights by id.
+ * Latency bounds single rows: a round through the cluster is about a microsecond, and so is the first run through a few
+ * hundred instructions, which is why what is used more than once is a call here. Rows without top-k need the
+ * exponential of every token. (An atomic add of 64 bits in shared memory takes ten times one of 32: a histogram of exact
+ * weights cost 12 of 37 us.) */
+constexpr int kT = 512, kWarps = kT / 32, kGroups = 4 * kWarps;   /* groups of eight threads */
+constexpr int kBins = 1024, kBinsEach = kBins / kT;
+constexpr int kCap = 1024;                                        /* gathered tokens, at most */
 constexpr int kMaxCluster = 16;
-constexpr int kGroups = 4 * kWarps;                               /* of eight threads */
-constexpr int kSel = 1024;                                        /* groups that are ranked, at most */
-constexpr double kRange = 44.0 * 0.6931471805599453;              /* distances with a weight, in temperatures: 2^-44 and up */
+constexpr double kRange = 26.0;                                   /* halvings of weight over the steps; the last takes the rest */
 
-struct Part { u64 w[3]; u64 key; int n[3]; int pad; };
+struct Part { u64 w[3]; u64 key; };
 
 struct Shared {
     Part parts[2][kMaxCluster];                                   /* what each CTA says, by turns */
     Part mine;
+    double c, floor_y, drop;                                      /* log2(e) / T; min-p as an exponent, and in logits */
+    float limit;
+    Powers powers;
     u64 warp_w[kWarps];
     int warp_n[kWarps];
     Sum3 sums[kWarps];
-    uint32_t my_tops[kGroups], sel[kSel];
-    int gathered, pick;
-    u64 found;
-    union { u64 list[kCap]; u64 hist_w[kBins]; };                 /* gathered tokens; this CTA's histogram */
-    union { uint32_t tops[kMaxCluster][kGroups]; uint32_t hist_n[kBins]; };   /* the groups' largest keys */
-    u64 all_w[kBins];                                             /* the cluster's histogram */
-    uint32_t all_n[kBins];
+    uint32_t my_tops[kGroups];
+    alignas(16) uint32_t sel[kT];                                 /* read by 16 bytes */
+    int gathered, pick, from;
+    u64 list[kCap], weight[kCap];                                 /* gathered tokens, key << 32 | ~id; their values */
+    union { uint32_t tops[kMaxCluster][kGroups]; uint32_t hist[kBins]; };   /* the groups' largest keys; this CTA's histogram */
+    uint32_t upto[kBins];                                         /* the cluster's, summed up to each step */
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -247,14 +291,9 @@ __device__ __forceinline__ uint32_t peer_addr(const void* p, int rank) {
 }
 __device__ __forceinline__ void peer_put(uint32_t at, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
 __device__ __forceinline__ void peer_put(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
-__device__ __forceinline__ uint32_t peer_get32(uint32_t at) {
+__device__ __forceinline__ uint32_t peer_get(uint32_t at) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at));
-    return v;
-}
-__device__ __forceinline__ u64 peer_get64(uint32_t at) {
-    u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at));
     return v;
 }
 __device__ __forceinline__ void meet() {                          /* of the cluster; orders what was put before it */
@@ -262,6 +301,14 @@ __device__ __forceinline__ void meet() {                          /* of the clus
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+#pragma unroll 1
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+static_assert(offsetof(Shared, sel) % 16 == 0, "read by 16 bytes");
+static_assert(offsetof(Shared, parts) % 8 == 0 && offsetof(Shared, mine) % 8 == 0 && sizeof(Part) % 8 == 0, "sent by 8 bytes");
 /* the cluster, the same in every thread of it */
 struct Cluster {
     Shared* s;
@@ -269,74 +316,83 @@ struct Cluster {
 
     /* every CTA's `mine` to every CTA, and with it what the threads put before; parts are valid until the turn after next */
     __device__ __forceinline__ const Part* exchange() {
+        const Part* p = s->parts[turn];
+        send(s, size, rank, turn);
+        turn ^= 1;
+        return p;
+    }
+    __device__ static __noinline__ void send(Shared* s, int size, int rank, int turn) {
         __syncthreads();
         constexpr int kWords = sizeof(Part) / 8;
         for (int i = threadIdx.x; i < size * kWords; i += kT)
             peer_put(peer_addr((u64*)&s->parts[turn][rank] + i % kWords, i / kWords), ((const u64*)&s->mine)[i % kWords]);
         meet();
-        const Part* p = s->parts[turn];
-        turn ^= 1;
-        return p;
     }
     /* sums over the cluster */
     __device__ __forceinline__ Sum3 sum(Sum3 v) {
-#pragma unroll
-        for (int j = 0; j < 3; ++j)
-#pragma unroll
-            for (int o = 16; o; o >>= 1) v.w[j] += __shfl_xor_sync(0xffffffffu, v.w[j], o);
-        if ((threadIdx.x & 31) == 0) s->sums[threadIdx.x >> 5] = v;
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            v = s->sums[threadIdx.x];
-#pragma unroll
-            for (int j = 0; j < 3; ++j)
-#pragma unroll
-                for (int o = 16; o; o >>= 1) v.w[j] += __shfl_xor_sync(0xffffffffu, v.w[j], o);
-            if (threadIdx.x < 3) s->mine.w[threadIdx.x] = v.w[threadIdx.x];
-        }
+        block_sums(s, v.w[0], v.w[1], v.w[2]);
         const Part* p = exchange();
         Sum3 all{};
-        for (int r = 0; r < size; ++r)
-#pragma unroll
-            for (int j = 0; j < 3; ++j) all.w[j] += p[r].w[j];
+#pragma unroll 1
+        for (int r = 0; r < size; ++r) { all.w[0] += p[r].w[0]; all.w[1] += p[r].w[1]; all.w[2] += p[r].w[2]; }
         return all;
+    }
+    __device__ static __noinline__ void block_sums(Shared* s, u64 a, u64 b, u64 c) {
+        a = warp_sum(a); b = warp_sum(b); c = warp_sum(c);
+        if ((threadIdx.x & 31) == 0) s->sums[threadIdx.x >> 5] = Sum3{{a, b, c}};
+        __syncthreads();
+        if (threadIdx.x < 3) {
+            u64 v = 0;
+            for (int i = 0; i < kT / 32; ++i) v += s->sums[i].w[threadIdx.x];
+            s->mine.w[threadIdx.x] = v;
+        }
     }
 };
 
 /* exclusive over the block's threads, in their order; *total over all of them */
 template <typename V>
-__device__ __forceinline__ V scan(V* warps, V v, V* total) {
-    static_assert(kWarps == 32, "one lane a warp");
+__device__ __noinline__ V scan(V* warps, V v, V* total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     V x = v;
-#pragma unroll
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) { const V y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
     __syncthreads();
     if (lane == 31) warps[warp] = x;
     __syncthreads();
-    V all = warps[lane];
-#pragma unroll
+    V all = lane < kWarps ? warps[lane] : (V)0;
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) { const V y = __shfl_up_sync(0xffffffffu, all, o); if (lane >= o) all += y; }
     *total = __shfl_sync(0xffffffffu, all, 31);
     const V before = __shfl_sync(0xffffffffu, all, max(warp - 1, 0));
-    return (warp ? before : 0) + x - v;
+    return (warp ? before : (V)0) + x - v;
 }
 
-/* n2 (a power of two, 32 at least) words, largest first: the first warp alone where it can keep two a lane */
-__device__ __forceinline__ void sort_desc(u64* a, int n2) {
-    const bool one_warp = n2 <= 64;
-    __syncthreads();
-    if (one_warp && threadIdx.x >= 32) { __syncthreads(); return; }
-    for (int k = 2; k <= n2; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            if (one_warp) __syncwarp(); else __syncthreads();
-            for (int i = threadIdx.x; i < n2 / 2; i += kT) {
-                const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-                const u64 x = a[lo], y = a[hi];
-                if ((x < y) == ((lo & k) == 0)) { a[lo] = y; a[hi] = x; }
-            }
-        }
-    __syncthreads();
+/* For the i-th of n gathered tokens (i = the thread's place among groups of kT / n2 threads): how many stand before it
+ * in the order, the sum of their values, and of those with a larger key. */
+struct Before { int n; u64 all, larger; };
+__device__ __noinline__ Before before_of(const u64* list, const u64* weight, int n, int i, int share) {
+    const u64 a = i < n ? list[i] : ~0ull;
+    Before r{0, 0, 0};
+#pragma unroll 4
+    for (int j = threadIdx.x % share; j < n; j += share) {
+        const u64 o = list[j], v = o > a ? weight[j] : 0;
+        r.n += o > a;
+        r.all += v;
+        r.larger += (uint32_t)(o >> 32) > (uint32_t)(a >> 32) ? v : 0;
+    }
+#pragma unroll 1
+    for (int o = 1; o < share; o <<= 1) {
+        r.n += __shfl_xor_sync(0xffffffffu, r.n, o);
+        r.all += __shfl_xor_sync(0xffffffffu, r.all, o);
+        r.larger += __shfl_xor_sync(0xffffffffu, r.larger, o);
+    }
+    return r;
+}
+/* threads for each of n tokens, a power of two up to a warp */
+__device__ __forceinline__ int share_of(int n) {
+    int share = 32;
+    while (share > 1 && n * share > kT) share >>= 1;
+    return share;
 }
 
 /* a token's key as it is kept: a bf16 key is the upper half of its f32 one */
@@ -345,7 +401,7 @@ template <> __device__ __forceinline__ uint32_t wide<uint32_t>(uint32_t k) { ret
 template <> __device__ __forceinline__ uint32_t wide<uint16_t>(uint16_t k) { return k & 0x8000u ? (uint32_t)k << 16 : k ? (uint32_t)k << 16 | 0xffffu : 0u; }
 
 template <typename K>
-__global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const int e) {
+__global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const int e) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared* const s = (Shared*)raw;
     K* const keys = (K*)(raw + sizeof(Shared));
@@ -366,46 +422,55 @@ __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const in
 
     /* ---- read the row; its largest key, the lowest id that has it, and how many are not masked */
     u64 best_id = 0;
-    uint32_t top = 0;                                             /* the largest key this thread read */
     int live = 0;
     {
+        uint32_t top = 0;                                         /* the largest key this thread read */
         int at = -1;
         const int here = min(e, (V - base - tid + kT - 1) / kT);  /* negative: none */
-#pragma unroll 8
-        for (int j = 0; j < here; ++j) {
-            const uint32_t key = key_of(load_x(P, m, base + j * kT + tid));
-            keys[j * kT + tid] = (K)(sizeof(K) == 2 ? key >> 16 : key);
-            live += key != 0;
-            if (key > top) { top = key; at = j; }
+        /* sixteen loads on their way at a time */
+#pragma unroll 1
+        for (int j0 = 0; j0 < e; j0 += 16) {
+            float x[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = j0 + j < here ? load_x(P, m, base + (j0 + j) * kT + tid) : -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                if (j0 + j >= e) break;
+                const uint32_t key = key_of(x[j]);
+                keys[(j0 + j) * kT + tid] = (K)(sizeof(K) == 2 ? key >> 16 : key);
+                live += key != 0;
+                if (key > top) { top = key; at = j0 + j; }
+            }
         }
-        for (int j = max(here, 0); j < e; ++j) keys[j * kT + tid] = 0;
         if (top) best_id = (u64)top << 32 | (0xffffffffu - (uint32_t)(base + at * kT + tid));
-    }
-    {
-        uint32_t g = top;
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if ((tid & 7) == 0) s->my_tops[tid >> 3] = g;
+        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if ((tid & 7) == 0) s->my_tops[tid >> 3] = top;
     }
-    if (tid == 0) s->gathered = 0;
+    if (tid < 128) s->powers.of[tid] = kPowers.of[tid];
     live = __reduce_add_sync(0xffffffffu, live);
-#pragma unroll
+#pragma unroll 1
     for (int o = 16; o; o >>= 1) best_id = max(best_id, (u64)__shfl_xor_sync(0xffffffffu, best_id, o));
     if ((tid & 31) == 0) { s->warp_w[tid >> 5] = best_id; s->warp_n[tid >> 5] = live; }
     __syncthreads();
     if (tid < 32) {
-        best_id = s->warp_w[tid];
-        live = __reduce_add_sync(0xffffffffu, s->warp_n[tid]);
-#pragma unroll
+        best_id = tid < kWarps ? s->warp_w[tid] : 0;
+        live = __reduce_add_sync(0xffffffffu, tid < kWarps ? s->warp_n[tid] : 0);
+#pragma unroll 1
         for (int o = 16; o; o >>= 1) best_id = max(best_id, (u64)__shfl_xor_sync(0xffffffffu, best_id, o));
-        if (tid == 0) { s->mine.key = best_id; s->mine.n[0] = live; }
+        if (tid == 0) { s->mine.key = best_id; s->mine.w[0] = (u64)live; s->gathered = 0; }
+    } else if (tid < 64) {                                        /* one warp: a quotient and a logarithm in 64 bits */
+        const double c = t > 0.0f ? 1.4426950408889634 / (double)t : 0.0, y = floor_of(low);
+        if (tid == 32) { s->c = c; s->floor_y = y; s->drop = y / c; s->limit = (float)((P.shift + 1.25) / c); }
     }
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+#pragma unroll 1
     for (int i = tid; i < kGroups * cl.size; i += kT) peer_put(peer_addr(&s->tops[cl.rank][i % kGroups], i / kGroups), s->my_tops[i % kGroups]);
     {
         const Part* parts = cl.exchange();
         best_id = 0; live = 0;
-        for (int r = 0; r < cl.size; ++r) { best_id = max(best_id, parts[r].key); live += parts[r].n[0]; }
+#pragma unroll 1
+        for (int r = 0; r < cl.size; ++r) { best_id = max(best_id, parts[r].key); live += (int)parts[r].w[0]; }
     }
     const uint32_t best = (uint32_t)(best_id >> 32);
     const bool first_cta = cl.rank == 0;
@@ -418,97 +483,98 @@ __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const in
         if (first_cta && tid == 0) answer(P, m, (int)(0xffffffffu - (uint32_t)best_id), 1, 0.0f);
         return;
     }
-    const Row R = row_of(best, t, P.shift);
-    const double floor_y = floor_of(low);
+    Row R;
+    R.c = s->c; R.mx = (double)val_of(best); R.inf = isinf(val_of(best)); R.S = P.shift;
     const bool by_k = k < live, by_p = p < 1.0f;
-    /* `n` tokens of this thread that `pick` says, to the list of the first CTA, in any order */
-    const auto gather = [&](auto pick) {
+    const Weigh weigh{R.mx, R.c * 128.0, val_of(best), s->limit, R.S, R.inf};
+    const auto weight = [&](uint32_t key) { return weigh.of(s->powers.of, key); };
+    /* the least key that min-p keeps: from the 32 next to where the bound falls (all keys, if it falls lower) */
+    uint32_t least_key = 1;
+    if (low > 0.0f) {
+        const double floor_y = s->floor_y;
+        const uint32_t guess = R.inf || !(R.c > 0.0) ? best : key_of((float)fmax(R.mx + s->drop, -3.4e38));
+        const uint32_t mine = max(min(guess, best), 32u) - 16 + (tid & 31);
+        const bool in = mine <= best && exponent_of(R, mine) >= floor_y;
+        least_key = __reduce_min_sync(0xffffffffu, in ? mine : 0xffffffffu);
+        if (least_key == max(min(guess, best), 32u) - 16) least_key = 1;          /* even the lowest looked at is kept: T without end */
+        if (R.inf) least_key = best;
+    }
+    /* the tokens that `pick` says, to the lists of the first `to` CTAs, in any order */
+    const auto gather = [&](int to, auto pick) {
         int n = 0, n_cta;
+#pragma unroll 1
         for (int j = 0; j < e; ++j) { const uint32_t key = wide(own[j]); n += key && pick(key); }
         int at = scan(s->warp_n, n, &n_cta);
         if (tid == 0) {
             uint32_t from;
             asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(from) : "r"(peer_addr(&s->gathered, 0)), "r"(n_cta) : "memory");
-            s->pick = (int)from;
+            s->from = (int)from;
         }
         __syncthreads();
-        at += s->pick;
+        at += s->from;
+#pragma unroll 1
         for (int j = 0; j < e && n; ++j) {
             const uint32_t key = wide(own[j]);
             if (!key || !pick(key)) continue;
-            if (at < kCap) peer_put(peer_addr(&s->list[at], 0), (u64)key << 32 | (0xffffffffu - (uint32_t)(own_id + j)));
+            if (at < kCap)
+                for (int r = 0; r < to; ++r) peer_put(peer_addr(&s->list[at], r), (u64)key << 32 | (0xffffffffu - (uint32_t)(own_id + j)));
             ++at; --n;
         }
     };
 
     /* ---- top-k of a few */
     int sel = 128;                                                /* groups to rank: at least four times k */
-    while (sel < 4 * k && sel <= kSel) sel *= 2;
-    if (by_k && sel <= min(kSel, kGroups * cl.size)) {
+    while (sel < 4 * k && sel <= kT) sel *= 2;
+    if (by_k && sel <= min(kT, kGroups * cl.size)) {
         /* the k-th largest of the groups' keys, neighbours taken together down to `sel` groups */
-        const int of = kGroups * cl.size / sel, share = kT / sel;     /* threads a group */
+        const int of = kGroups * cl.size / sel, share = min(kT / sel, 32);     /* threads a group */
         const uint32_t* const tops = &s->tops[0][0];
         if (tid < sel) {
             uint32_t g = 0;
+#pragma unroll 1
             for (int j = 0; j < of; ++j) g = max(g, tops[tid * of + j]);
             s->sel[tid] = g;
         }
         __syncthreads();
-        const uint32_t mine = s->sel[tid / share];
+        const uint32_t mine = tid / share < sel ? s->sel[tid / share] : 0u;
         int larger = 0;
+#pragma unroll 1
         for (int j = tid % share * 4; j < sel; j += share * 4) {
             const uint4 o = *(const uint4*)&s->sel[j];
             larger += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
         }
+#pragma unroll 1
         for (int o = 1; o < share; o <<= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
         /* fewer than k groups lie above it: the least such key is the k-th largest */
-        uint32_t bound = __reduce_min_sync(0xffffffffu, larger < k ? mine : 0xffffffffu);
+        uint32_t bound = __reduce_min_sync(0xffffffffu, larger < k && tid / share < sel ? mine : 0xffffffffu);
         if ((tid & 31) == 0) s->warp_n[tid >> 5] = (int)bound;
         __syncthreads();
-        bound = __reduce_min_sync(0xffffffffu, (uint32_t)s->warp_n[tid & 31]);
-        gather([&](uint32_t key) { return key >= bound; });
+        bound = __reduce_min_sync(0xffffffffu, (tid & 31) < kWarps ? (uint32_t)s->warp_n[tid & 31] : 0xffffffffu);
+        gather(1, [&](uint32_t key) { return key >= bound; });
         meet();
-        const int n_top = (int)peer_get32(peer_addr(&s->gathered, 0));
-        if (bound && n_top <= kCap) {
-            if (!first_cta) { meet(); return; }                   /* the first CTA's memory outlives the reads of it, too */
-            meet();
-            int n2 = 32;
-            while (n2 < n_top) n2 <<= 1;
-            for (int i = n_top + tid; i < n2; i += kT) s->list[i] = 0;
-            sort_desc(s->list, n2);
-            const int each = (n2 + kT - 1) / kT, i0 = tid * each;
-            u64 w = 0, sum, dummy;
-            for (int i = i0; i < i0 + each && i < k; ++i) w += i < n_top ? weight_of(R, (uint32_t)(s->list[i] >> 32)) : 0ull;
-            u64 before = scan(s->warp_w, w, &sum);
+        const int n = (int)peer_get(peer_addr(&s->gathered, 0));
+        meet();                                                   /* all have read it */
+        if (bound && n <= kT) {                                   /* a thread for each */
+            if (!first_cta) return;
+            for (int i = tid; i < n; i += kT) s->weight[i] = weight((uint32_t)(s->list[i] >> 32));
+            __syncthreads();
+            const int sh = share_of(n), i = tid / sh;
+            const bool mine_too = i < n && tid % sh == 0;         /* one thread speaks for a token */
+            const Before b = before_of(s->list, s->weight, n, i, sh);
+            const u64 me = i < n ? s->list[i] : 0, w = i < n ? s->weight[i] : 0;
+            const uint32_t key = (uint32_t)(me >> 32);
+            u64 sum;
+            scan(s->warp_w, mine_too && b.n < k ? w : 0ull, &sum);
             const u64 want = by_p ? want_of(p, sum) : ~0ull;
-            int kept = 0;
-            w = 0;
-            for (int i = i0; i < i0 + each && i < k && i < n_top; ++i) {
-                const uint32_t key = (uint32_t)(s->list[i] >> 32);
-                if (i && (before >= want || exponent_of(R, key) < floor_y)) break;
-                const u64 x = weight_of(R, key);
-                before += x; w += x; ++kept;
-            }
-            int n_kept;
-            scan(s->warp_n, kept, &n_kept);
-            scan(s->warp_w, w, &sum);
-            /* by id, ascending: the low words are 0xffffffff - id; the key moves below */
-            n2 = 32;
-            while (n2 < n_kept) n2 <<= 1;
-            for (int i = tid; i < n2; i += kT) { const u64 v2 = s->list[i]; s->list[i] = i < n_kept ? v2 << 32 | v2 >> 32 : 0ull; }
-            sort_desc(s->list, n2);
-            w = 0;
-            const int each2 = (n2 + kT - 1) / kT, j0 = tid * each2;
-            for (int i = j0; i < j0 + each2 && i < n_kept; ++i) w += weight_of(R, (uint32_t)s->list[i]);
-            before = scan(s->warp_w, w, &dummy);
-            const u64 point = point_of(u, sum);
-            for (int i = j0; i < j0 + each2 && i < n_kept; ++i) {
-                const uint32_t key = (uint32_t)s->list[i];
-                const u64 x = weight_of(R, key);
-                if (before <= point && point < before + x)
-                    answer(P, m, (int)(0xffffffffu - (uint32_t)(s->list[i] >> 32)), n_kept, logprob_of(R, key, sum));
-                before += x;
-            }
+            const bool keep = mine_too && b.n < k && (b.n == 0 || (b.all < want && key >= least_key));
+            scan(s->warp_w, keep ? w : 0ull, &sum);
+            const int n_kept = __syncthreads_count(keep);
+            /* by id, ascending: the low words are 0xffffffff - id, and what is not kept weighs nothing */
+            if (mine_too) { s->list[i] = me << 32 | key; s->weight[i] = keep ? w : 0; }
+            __syncthreads();
+            const u64 before = before_of(s->list, s->weight, n, i, sh).all, point = point_of(u, sum);
+            if (keep && before <= point && point < before + w)
+                answer(P, m, (int)(0xffffffffu - (uint32_t)me), n_kept, logprob_of(R, key, sum));
             return;
         }
     }
@@ -517,140 +583,178 @@ __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const in
     int ties = V;
     if (by_k || by_p) {
         /* ---- histogram of the distance to the largest logit (key order and step order agree) */
-        __syncthreads();
-        for (int i = tid; i < kBins; i += kT) { s->hist_n[i] = 0; s->hist_w[i] = 0; }
-        __syncthreads();
-        const float mx = val_of(best), inv = (float)((kBins - 1) / kRange) / t;
+        const float mx = val_of(best), inv = (float)((kBins - 1) / kRange * 1.4426950408889634) / t;
         const auto bin_of = [&](uint32_t key) {
             if (R.inf) return key == best ? 0 : kBins - 1;
             const float d = __fsub_rn(mx, val_of(key)) * inv;
             return d < (float)(kBins - 1) ? (int)d : d >= (float)(kBins - 1) ? kBins - 1 : 0;     /* not a number: 0 * inf, every weight is 1 */
         };
-#pragma unroll 2
+        __syncthreads();
+        for (int i = tid; i < kBins; i += kT) s->hist[i] = 0;
+        __syncthreads();
+#pragma unroll 1
         for (int j = 0; j < e; ++j) {
             const uint32_t key = wide(own[j]);
-            if (!key) continue;
-            const int b = bin_of(key);
-            atomicAdd(&s->hist_n[b], 1u);
-            if (by_p) {
-                const u64 x = weight_of(R, key);
-                if (x) atomicAdd(&s->hist_w[b], x);
-            }
+            if (key) atomicAdd(&s->hist[bin_of(key)], 1u);
+        }
+        meet();
+        /* each CTA sums its share of the steps, `size` threads a step, and tells all */
+        const int seg = kBins / cl.size;
+#pragma unroll
+        for (int i = tid; i < kBins; i += kT) {
+            const int b = cl.rank * seg + i / cl.size, r = i % cl.size;
+            uint32_t n = peer_get(peer_addr(&s->hist[b], r));
+#pragma unroll 1
+            for (int o = 1; o < cl.size; o <<= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+            peer_put(peer_addr(&s->upto[b], r), n);
+        }
+        meet();
+        uint32_t cnt[kBinsEach], n_own = 0;
+        float est[kBinsEach], est_own = 0.0f;
+        const float per_bin = (float)(kRange / (kBins - 1));       /* halvings a step */
+#pragma unroll
+        for (int j = 0; j < kBinsEach; ++j) {
+            cnt[j] = s->upto[kBinsEach * tid + j];
+            est[j] = (float)cnt[j] * exp2f(-per_bin * ((float)(kBinsEach * tid + j) + 0.5f));
+            n_own += cnt[j]; est_own += est[j];
+        }
+        int dummy;
+        int upto = scan(s->warp_n, (int)n_own, &dummy);
+#pragma unroll
+        for (int j = 0; j < kBinsEach; ++j) {
+            const int before = upto;
+            upto += (int)cnt[j];
+            if (by_k && before < k && upto >= k) s->pick = kBinsEach * tid + j;       /* the step of the k-th token */
+            s->upto[kBinsEach * tid + j] = (uint32_t)upto;
         }
         __syncthreads();
-        meet();
-        const int seg = kBins / cl.size;
-        for (int i = tid; i < seg; i += kT) {
-            const int b = cl.rank * seg + i;
-            uint32_t ns[kMaxCluster], n = 0;
-            u64 ws[kMaxCluster], w = 0;
-#pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) if (r < cl.size) { ns[r] = peer_get32(peer_addr(&s->hist_n[b], r)); ws[r] = peer_get64(peer_addr(&s->hist_w[b], r)); }
-#pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) if (r < cl.size) { n += ns[r]; w += ws[r]; }
-            for (int r = 0; r < cl.size; ++r) { peer_put(peer_addr(&s->all_n[b], r), n); peer_put(peer_addr(&s->all_w[b], r), w); }
-        }
-        meet();
-        static_assert(kBins == 2 * kT, "two steps a thread");
-        const uint32_t n0 = s->all_n[2 * tid], n1 = s->all_n[2 * tid + 1];
-        const u64 w0 = s->all_w[2 * tid], w1 = s->all_w[2 * tid + 1];
-        int live2; u64 total;
-        const int n_before = scan(s->warp_n, (int)(n0 + n1), &live2);
-        const u64 w_before = scan(s->warp_w, w0 + w1, &total);
-        /* the step whose running count (weight) first reaches `need`, and what lies before it */
-        const auto step_at = [&](u64 before, u64 a, u64 b, u64 need, u64* above) {
-            __syncthreads();
-            if (before < need && before + a + b >= need) {
-                const bool second = before + a < need;
-                s->pick = 2 * tid + second;
-                s->found = second ? before + a : before;
-            }
-            __syncthreads();
-            *above = s->found;
-            return s->pick;
-        };
-        /* the largest key c of a step such that above + the value of the step's keys from c on reaches `need`; *above
-         * moves on to what lies over c. The step's tokens are gathered and sorted, or the key is searched */
-        const auto key_at = [&](int step, uint32_t least, u64 need, u64* above, auto value) {
-            meet();
-            if (first_cta && tid == 0) s->gathered = 0;
-            meet();
-            gather([&](uint32_t key) { return key >= least && bin_of(key) == step; });
-            meet();
-            const int n = (int)peer_get32(peer_addr(&s->gathered, 0));
-            if (n <= kCap) {
-                if (first_cta) {
-                    int n2 = 32;
-                    while (n2 < n) n2 <<= 1;
-                    for (int i = n + tid; i < n2; i += kT) s->list[i] = 0;
-                    sort_desc(s->list, n2);
-                    const int each = (n2 + kT - 1) / kT, i0 = tid * each;
-                    u64 v = 0, all;
-                    for (int i = i0; i < i0 + each && i < n; ++i) v += value((uint32_t)(s->list[i] >> 32));
-                    u64 run = *above + scan(s->warp_w, v, &all);
-                    for (int i = i0; i < i0 + each && i < n; ++i) {
-                        const uint32_t key = (uint32_t)(s->list[i] >> 32);
-                        const u64 x = value(key);
-                        if (run < need && run + x >= need) {
-                            int over = i;                          /* ties of it may stand before it */
-                            u64 then = run;
-                            while (over > 0 && (uint32_t)(s->list[over - 1] >> 32) == key) { --over; then -= x; }
-                            s->mine.key = key; s->mine.w[0] = then;
-                        }
-                        run += x;
+        const int k_step = s->pick;
+        const auto count_to = [&](int b) { return b > 0 ? (int)s->upto[b - 1] : 0; };      /* tokens in steps below b */
+
+        /* the largest key c in the steps [from, to) such that above + the value of their keys >= c reaches `need`;
+         * *above moves on to what lies over c. The tokens are gathered and ranked, or the key is searched */
+        const auto key_at = [&](int from, int to, uint32_t least, u64 need, u64* above, bool ones) {
+            const auto inside = [&](uint32_t key) { if (key < least) return false; const int b = bin_of(key); return b >= from && b < to; };
+            const auto value = [&](uint32_t key) { return ones ? 1ull : weight(key); };
+            if (count_to(to) - count_to(from) <= kCap) {
+                if (first_cta && tid == 0) s->gathered = 0;
+                meet();
+                gather(cl.size, inside);
+                if (tid == 0) s->mine.key = 0;
+                meet();
+                /* each CTA ranks its share of them */
+                const int n = (int)peer_get(peer_addr(&s->gathered, 0));
+                for (int i = tid; i < n; i += kT) s->weight[i] = value((uint32_t)(s->list[i] >> 32));
+                __syncthreads();
+                const int here = (n + cl.size - 1) / cl.size, sh = share_of(here);
+#pragma unroll 1
+                for (int j = tid / sh; j - tid / sh < here; j += kT / sh) {
+                    const int i = j < here ? cl.rank * here + j : n;
+                    const Before b = before_of(s->list, s->weight, n, i, sh);
+                    if (i < n && tid % sh == 0 && *above + b.all < need && *above + b.all + s->weight[i] >= need) {
+                        s->mine.key = s->list[i] >> 32;
+                        s->mine.w[0] = *above + b.larger;
                     }
                 }
                 const Part* parts = cl.exchange();
-                *above = parts[0].w[0];
-                return (uint32_t)parts[0].key;
+                uint32_t found = 0;
+#pragma unroll 1
+                for (int r = 0; r < cl.size; ++r) if (parts[r].key) { found = (uint32_t)parts[r].key; *above = parts[r].w[0]; }
+                return found;
             }
-            uint32_t lo = least, hi = best + 1;
-            u64 over = 0;                                         /* of the step's keys from hi on */
+            /* the keys as they are kept, between those a step to either side of the window */
+            constexpr int kShift = sizeof(K) == 2 ? 16 : 0;
+            const float v_lo = mx - (float)(to + 1) / inv, v_hi = mx - (float)(from - 1) / inv;
+            uint32_t lo = least, hi = best;
+            if (to < kBins && v_lo > -3.0e38f) lo = max(lo, key_of(v_lo));
+            if (from > 1 && v_hi < 3.0e38f && v_hi < mx) hi = min(hi, key_of(v_hi));
+            lo >>= kShift; hi = (hi >> kShift) + 1;
+            u64 over = 0;                                         /* of the keys from hi on */
+#pragma unroll 1
             while (hi - lo > 1) {
                 const uint32_t d = max(1u, (hi - lo) / 4);
-                uint32_t c[3];
-#pragma unroll
-                for (int j = 0; j < 3; ++j) c[j] = min(lo + (j + 1) * d, hi);
-                Sum3 v3{};
+                const uint32_t c0 = min(lo + d, hi), c1 = min(lo + 2 * d, hi), c2 = min(lo + 3 * d, hi);
+                Sum3 v{};
+#pragma unroll 1
                 for (int j = 0; j < e; ++j) {
-                    const uint32_t key = wide(own[j]);
-                    if (key < c[0] || key >= hi || bin_of(key) != step) continue;
-                    const u64 x = value(key);
-                    v3.w[0] += x;
-                    if (key >= c[1]) v3.w[1] += x;
-                    if (key >= c[2]) v3.w[2] += x;
+                    const uint32_t whole = wide(own[j]), key = whole >> kShift;
+                    if (key < c0 || key >= hi || !inside(whole)) continue;
+                    const u64 x = value(whole);
+                    v.w[0] += x;
+                    if (key >= c1) v.w[1] += x;
+                    if (key >= c2) v.w[2] += x;
                 }
-                v3 = cl.sum(v3);
-                int j = -1;
-                for (int i = 0; i < 3; ++i) if (c[i] < hi && *above + over + v3.w[i] >= need) j = i;
-                if (j < 2 && c[j + 1] < hi) { over += v3.w[j + 1]; hi = c[j + 1]; }
-                if (j >= 0) lo = c[j];
+                v = cl.sum(v);
+                const u64 have = *above + over;
+                if (c2 < hi && have + v.w[2] >= need) lo = c2;
+                else if (c1 < hi && have + v.w[1] >= need) { lo = c1; if (c2 < hi) { over += v.w[2]; hi = c2; } }
+                else if (have + v.w[0] >= need) { lo = c0; if (c1 < hi) { over += v.w[1]; hi = c1; } }
+                else { over += v.w[0]; hi = c0; }
             }
             *above += over;
-            return lo;
+            return wide((K)lo);
         };
         u64 above;
         if (by_k) {
-            const int step = step_at((u64)n_before, n0, n1, (u64)k, &above);
-            cut = key_at(step, 1u, (u64)k, &above, [](uint32_t) { return 1ull; });
+            above = (u64)count_to(k_step);
+            cut = key_at(k_step, k_step + 1, 1u, (u64)k, &above, true);
             ties = (int)((u64)k - above);
         }
         if (by_p) {
-            u64 over = total;
-            if (by_k) {                                           /* the weight over the cut: whole steps, and the cut's own */
-                Sum3 v3{};
-                for (int j = 0; j < e; ++j) { const uint32_t key = wide(own[j]); if (key > cut) v3.w[0] += weight_of(R, key); }
-                over = cl.sum(v3).w[0];
+            /* the window: where p of the middle weights ends, and up to two steps to either side if they hold few */
+            float all;
+            float run = scan((float*)s->warp_n, est_own, &all);
+            if (by_k) {                                           /* of the first k tokens */
+                float part = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kBinsEach; ++j) if (kBinsEach * tid + j <= k_step) part += est[j];
+                scan((float*)s->warp_n, part, &all);
             }
-            const u64 want = want_of(p, by_k ? over + (u64)ties * weight_of(R, cut) : total);
-            above = over;
-            if (!by_k || over >= want) {
-                const int step = step_at(w_before, w0, w1, want, &above);
-                cut = key_at(step, by_k ? cut : 1u, want, &above, [&](uint32_t key) { return weight_of(R, key); });
-                ties = V;
+            if (tid == 0) s->pick = by_k ? k_step : kBins - 1;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < kBinsEach; ++j) {
+                if (run < p * all && run + est[j] >= p * all) atomicMin(&s->pick, kBinsEach * tid + j);
+                run += est[j];
             }
-            const u64 one = weight_of(R, cut);
-            if (one && want > above) ties = (int)min((u64)ties, (want - above + one - 1) / one);
+            __syncthreads();
+            const int mid = min(s->pick, kBins - 1);
+            int from = mid, to = mid + 1, width = 1;
+            for (int d = 1; d <= 2; ++d)
+                if (mid >= d && mid + d < kBins && count_to(mid + d + 1) - count_to(mid - d) <= 256) { from = mid - d; to = mid + d + 1; width = to - from; }
+            const u64 tied = by_k ? (u64)ties * weight(cut) : 0;
+#pragma unroll 1
+            for (;;) {
+                Sum3 v{};                                         /* over the cut; of those, in steps below from, below to */
+#pragma unroll 2
+                for (int j = 0; j < e; ++j) {
+                    const uint32_t key = wide(own[j]);
+                    if (by_k ? key <= cut : !key) continue;
+                    const u64 x = weight(key);
+                    const int b = bin_of(key);
+                    v.w[0] += x;
+                    if (b < from) v.w[1] += x;
+                    if (b < to) v.w[2] += x;
+                }
+                v = cl.sum(v);
+                const u64 want = want_of(p, v.w[0] + tied);
+                above = v.w[0];
+                if (by_k && want > v.w[0]) {                      /* it ends among the cut's ties */
+                    const u64 one = weight(cut);
+                    if (one) ties = (int)min((u64)ties, (want - above + one - 1) / one);
+                    break;
+                }
+                if (want > v.w[1] && want <= v.w[2]) {
+                    above = v.w[1];
+                    cut = key_at(from, to, by_k ? cut + 1 : 1u, want, &above, false);
+                    const u64 one = weight(cut);
+                    ties = one ? (int)min((u64)V, (want - above + one - 1) / one) : V;
+                    break;
+                }
+                width *= 8;
+                if (want <= v.w[1]) { to = from; from = max(from - width, 0); }
+                else { from = to; to = min(to + width, kBins); }
+            }
         }
     }
 
@@ -658,41 +762,48 @@ __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const in
     int tie_rank = 0;
     if (ties < V) {
         int n = 0, n_cta;
+#pragma unroll 1
         for (int j = 0; j < e; ++j) n += wide(own[j]) == cut;
         tie_rank = scan(s->warp_n, n, &n_cta);
-        if (tid == 0) s->mine.n[0] = n_cta;
+        if (tid == 0) s->mine.w[0] = (u64)n_cta;
         const Part* parts = cl.exchange();
-        for (int r = 0; r < cl.rank; ++r) tie_rank += parts[r].n[0];
+#pragma unroll 1
+        for (int r = 0; r < cl.rank; ++r) tie_rank += (int)parts[r].w[0];
     }
     int rank = tie_rank;
-    const bool by_low = low > 0.0f;
-    const auto kept = [&](uint32_t key) { return key >= cut && (key > cut || rank++ < ties) && (!by_low || exponent_of(R, key) >= floor_y); };
+    const auto kept = [&](uint32_t key) { return key >= cut && (key > cut || rank++ < ties) && key >= least_key; };
     u64 w = 0, w_cta;
-    int n = 0, n_cta;
+    int n = 0;
 #pragma unroll 2
     for (int j = 0; j < e; ++j) {
         const uint32_t key = wide(own[j]);
         if (!kept(key)) continue;
-        w += weight_of(R, key);
+        w += weight(key);
         ++n;
     }
-    u64 before = scan(s->warp_w, w, &w_cta);
-    scan(s->warp_n, n, &n_cta);
-    if (tid == 0) { s->mine.w[0] = w_cta; s->mine.n[0] = n_cta; }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((tid & 31) == 0) s->warp_n[tid >> 5] = n;
+    u64 before = scan(s->warp_w, w, &w_cta);                      /* its barriers order the counts, too */
+    if (tid < 32) {
+        n = __reduce_add_sync(0xffffffffu, tid < kWarps ? s->warp_n[tid] : 0);
+        if (tid == 0) { s->mine.w[0] = w_cta; s->mine.w[1] = (u64)n; }
+    }
     const Part* parts = cl.exchange();
     u64 sum = 0;
     int n_kept = 0;
+#pragma unroll 1
     for (int r = 0; r < cl.size; ++r) {
         if (r < cl.rank) before += parts[r].w[0];
-        sum += parts[r].w[0]; n_kept += parts[r].n[0];
+        sum += parts[r].w[0]; n_kept += (int)parts[r].w[1];
     }
     const u64 point = point_of(u, sum);
     if (before <= point && point < before + w) {
         rank = tie_rank;
+#pragma unroll 1
         for (int j = 0; j < e; ++j) {
             const uint32_t key = wide(own[j]);
             if (!kept(key)) continue;
-            before += weight_of(R, key);
+            before += weight(key);
             if (before <= point) continue;
             answer(P, m, own_id + j, n_kept, logprob_of(R, key, sum));
             break;
@@ -700,23 +811,30 @@ __global__ void __launch_bounds__(kT) k_nucleus_row(const R3dNucleus P, const in
     }
 }
 
+constexpr size_t kRowSmem = 220 * 1024;
+int each_of(int vocab, int size) { return ((vocab + kT * size - 1) / (kT * size)) | 1; }
+size_t row_smem(int vocab, int size, int ksz) { return sizeof(Shared) + (size_t)kT * each_of(vocab, size) * ksz; }
+
 template <typename K>
-int launch_row(const R3dNucleus& P, int size, int e, size_t smem, cudaStream_t st) {
+int launch_row(const R3dNucleus& P, int size, cudaStream_t st) {
+    const auto kernel = k_nucleus_row<K>;
     static std::atomic<bool> set[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return RAD_E_DEVICE;
     if (!set[dev].load(std::memory_order_relaxed)) {
-        if (cudaFuncSetAttribute(k_nucleus_row<K>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
-            cudaFuncSetAttribute(k_nucleus_row<K>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return RAD_E_DEVICE;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRowSmem) != cudaSuccess ||
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return RAD_E_DEVICE;
         set[dev].store(true, std::memory_order_relaxed);
     }
+    const int e = each_of(P.n_vocab, size);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)P.rows * (unsigned)size); cfg.blockDim = dim3(kT); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.gridDim = dim3((unsigned)P.rows * (unsigned)size); cfg.blockDim = dim3(kT); cfg.stream = st;
+    cfg.dynamicSmemBytes = row_smem(P.n_vocab, size, (int)sizeof(K));
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = (unsigned)size; at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_nucleus_row<K>, P, e) == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
+    return cudaLaunchKernelEx(&cfg, kernel, P, e) == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
 }
 
 } /* namespace */
@@ -728,20 +846,17 @@ int launch_nucleus(const R3dNucleus& p, cudaStream_t st) {
     P.shift = 62 - bits < 50 ? 62 - bits : 50;
     count_launch();
     const int ksz = p.x_dtype == RAD_F32 ? 4 : 2;
-    int size = 1, e = 0;
-    size_t smem = 0;
-    for (;; size *= 2) {
-        e = ((p.n_vocab + kT * size - 1) / (kT * size)) | 1;
-        smem = sizeof(Shared) + (size_t)kT * e * ksz;
-        if (size == kMaxCluster) break;
-        if (smem <= 220 * 1024 && ((long long)p.rows * size >= 148 || kT * e <= 4096)) break;
-    }
-    if (getenv("DEV_CL")) { size = atoi(getenv("DEV_CL")); e = ((p.n_vocab + kT * size - 1) / (kT * size)) | 1; smem = sizeof(Shared) + (size_t)kT * e * ksz; }
-    if (smem > 220 * 1024) {
+    /* CTAs a row: no more than 39 tokens a thread, and more where rows are few, down to nine (151936 tokens: one row
+     * takes 27 / 20 / 16 us on 4 / 8 / 16 CTAs; 64 rows 59 / 56 / 83, 256 rows with filters of their own 521 / 519 on
+     * 4 / 8; 30 rows of 20000 52 / 16 / 18 us on 2 / 4 / 8) */
+    int size = 1;
+    while (size < kMaxCluster && (row_smem(p.n_vocab, size, ksz) > kRowSmem || each_of(p.n_vocab, size) > 39 ||
+                                  ((long long)p.rows * size < 100 && each_of(p.n_vocab, size) > 9))) size *= 2;
+    if (row_smem(p.n_vocab, size, ksz) > kRowSmem) {
         k_nucleus_long<<<(unsigned)p.rows, 1024, 0, st>>>(P);
         return cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
     }
-    return ksz == 4 ? launch_row<uint32_t>(P, size, e, smem, st) : launch_row<uint16_t>(P, size, e, smem, st);
+    return ksz == 4 ? launch_row<uint32_t>(P, size, st) : launch_row<uint16_t>(P, size, st);
 }
 
 } /* namespace r3d */
