@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
  * The row is read once, as ordered keys into the shared memory of the cluster's CTAs; a thread owns `e` neighbouring ids
  * (an odd number of words: its reads fall into banks of their own), so id order is the order of threads. What the CTAs
  * find out goes to all of them through distributed shared memory.
- *   - Top-k of a few: every eight threads know the largest key they read. The k-th largest of these is a bound that at
+ *   - Top-k of a few: every one to eight threads know the largest key they read. The k-th largest of these is a bound that at
  *     least k tokens reach, and hardly more: they are gathered in the first CTA, which ranks them, cuts and sums. Two
  *     rounds through the cluster, and no work on the other tokens but reading them.
  *   - Top-p alone, or a k beyond that: a histogram of the distance to the largest logit gives the exact step of the k-th
@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
  * hundred instructions, which is why what is used more than once is a call here. Rows without top-k need the
  * exponential of every token. (An atomic add of 64 bits in shared memory takes ten times one of 32: a histogram of exact
  * weights cost 12 of 37 us.) */
-constexpr int kT = 512, kWarps = kT / 32, kGroups = 4 * kWarps;   /* groups of eight threads */
+constexpr int kT = 512, kWarps = kT / 32;
+constexpr int kGroups = 1024;                                     /* of threads, in the cluster, at most */
 constexpr int kBins = 1024, kBinsEach = kBins / kT;
 constexpr int kCap = 1024;                                        /* gathered tokens, at most */
 constexpr int kMaxCluster = 16;
@@ -275,11 +276,11 @@ struct Shared {
     u64 warp_w[kWarps];
     int warp_n[kWarps];
     Sum3 sums[kWarps];
-    uint32_t my_tops[kGroups];
+    uint32_t my_tops[kT];
     alignas(16) uint32_t sel[kT];                                 /* read by 16 bytes */
     int gathered, pick, from;
     u64 list[kCap], weight[kCap];                                 /* gathered tokens, key << 32 | ~id; their values */
-    union { uint32_t tops[kMaxCluster][kGroups]; uint32_t hist[kBins]; };   /* the groups' largest keys; this CTA's histogram */
+    union { uint32_t tops[kGroups]; uint32_t hist[kBins]; };   /* the groups' largest keys; this CTA's histogram */
     uint32_t upto[kBins];                                         /* the cluster's, summed up to each step */
 };
 
@@ -420,6 +421,8 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     const float low = P.min_p ? P.min_p[m * P.mp_pitch] : 0.0f, u = P.u[m * P.u_pitch];
     int k = P.top_k ? P.top_k[m * P.k_pitch] : 0;
 
+    const int mine_groups = min(kT, kGroups / cl.size);           /* 1, 1, 2, 4 or 8 threads each */
+
     /* ---- read the row; its largest key, the lowest id that has it, and how many are not masked */
     u64 best_id = 0;
     int live = 0;
@@ -443,9 +446,9 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
             }
         }
         if (top) best_id = (u64)top << 32 | (0xffffffffu - (uint32_t)(base + at * kT + tid));
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if ((tid & 7) == 0) s->my_tops[tid >> 3] = top;
+#pragma unroll 1
+        for (int o = 1; o < kT / mine_groups; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (tid % (kT / mine_groups) == 0) s->my_tops[tid / (kT / mine_groups)] = top;
     }
     if (tid < 128) s->powers.of[tid] = kPowers.of[tid];
     live = __reduce_add_sync(0xffffffffu, live);
@@ -465,7 +468,8 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     }
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 #pragma unroll 1
-    for (int i = tid; i < kGroups * cl.size; i += kT) peer_put(peer_addr(&s->tops[cl.rank][i % kGroups], i / kGroups), s->my_tops[i % kGroups]);
+    for (int i = tid; i < mine_groups * cl.size; i += kT)
+        peer_put(peer_addr(&s->tops[cl.rank * mine_groups + i % mine_groups], i / mine_groups), s->my_tops[i % mine_groups]);
     {
         const Part* parts = cl.exchange();
         best_id = 0; live = 0;
@@ -523,16 +527,15 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     };
 
     /* ---- top-k of a few */
-    int sel = 128;                                                /* groups to rank: at least four times k */
-    while (sel < 4 * k && sel <= kT) sel *= 2;
-    if (by_k && sel <= min(kT, kGroups * cl.size)) {
+    int sel = 128;                                                /* groups to rank: at least twice k, which lets through 1.4 k tokens */
+    while (sel < 2 * k && sel <= kT) sel *= 2;
+    if (by_k && sel <= kT) {
         /* the k-th largest of the groups' keys, neighbours taken together down to `sel` groups */
-        const int of = kGroups * cl.size / sel, share = min(kT / sel, 32);     /* threads a group */
-        const uint32_t* const tops = &s->tops[0][0];
+        const int of = mine_groups * cl.size / sel, share = min(kT / sel, 32);     /* threads a group */
         if (tid < sel) {
             uint32_t g = 0;
 #pragma unroll 1
-            for (int j = 0; j < of; ++j) g = max(g, tops[tid * of + j]);
+            for (int j = 0; j < of; ++j) g = max(g, s->tops[tid * of + j]);
             s->sel[tid] = g;
         }
         __syncthreads();
@@ -636,7 +639,9 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         const auto key_at = [&](int from, int to, uint32_t least, u64 need, u64* above, bool ones) {
             const auto inside = [&](uint32_t key) { if (key < least) return false; const int b = bin_of(key); return b >= from && b < to; };
             const auto value = [&](uint32_t key) { return ones ? 1ull : weight(key); };
-            if (count_to(to) - count_to(from) <= kCap) {
+            /* ranking takes as many steps as the square of their number over the CTAs: a thousand on 4, 512 on one */
+            const int many = count_to(to) - count_to(from);
+            if (many <= kCap && many * many <= cl.size << 18) {
                 if (first_cta && tid == 0) s->gathered = 0;
                 meet();
                 gather(cl.size, inside);
