@@ -375,14 +375,16 @@ template <int KIND, typename T, int C, bool GRID>
 int launch_rows(const TokenI8& P, int rows, int threads, cudaStream_t st) {
     const int one = KIND == kQuant || (KIND == kRms && !P.res), smem = threads * C * 8 * (int)sizeof(T) * (one ? 1 : 2);
     const auto kernel = k_token_i8_regs<KIND, T, C, GRID>;
-    static std::atomic<int> fits[33][2];                          /* resident blocks of the device, by warps a block and streams */
-    std::atomic<int>& known = fits[threads / 32][one];
+    static std::atomic<int> fits[64][33][2];                      /* resident blocks, by device, warps a block and streams */
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return RAD_E_DEVICE;
+    std::atomic<int>& known = fits[dev][threads / 32][one];
     int grid = known.load(std::memory_order_relaxed);
     if (!grid) {
-        int per = 0, dev = 0, sms = 0;
+        int per = 0, sms = 0;
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess ||
             cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem) != cudaSuccess ||
-            cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+            cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
             return RAD_E_DEVICE;
         grid = (per > 0 ? per : 1) * sms;
         known.store(grid, std::memory_order_relaxed);

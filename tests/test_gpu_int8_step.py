@@ -6,6 +6,7 @@ conversion and two multiplications (3 * 2^-24 relative), with bf16 output one mo
 `rounds` f32 roundings, so |h * step| moves by at most 127 * (rounds + 3) * 2^-24 and a code differs by one only where
 the 64-bit quotient lies that near a half. Tokens and counts are whole numbers and have to be equal: the rows' running
 sums lie further from every border than the fixed point's error."""
+import ctypes as C
 import math
 
 import numpy as np
@@ -16,6 +17,13 @@ from libr3d_b200 import abi, ops
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def no_wait_expired():
+    yield
+    torch.cuda.synchronize()
+    assert ops.plugin().lib.r3d_b200_stream_status() == 0
 
 
 def _rng(seed):
@@ -73,6 +81,23 @@ def test_gemm_views(M, N, K, pa, pb, py, off):
     ops.gemm_i8a8(a, sa, b, sb, whole[:, :N])
     _check_gemm(a, sa, b, sb, whole[:, :N])
     assert bool((whole[:, N:] == 7.0).all())
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 100, 128), (40, 5120, 1024), (100, 640, 5008), (300, 1000, 272), (600, 4700, 512)])
+def test_gemm_arms_give_the_same_bits(M, N, K):
+    g = _rng(M + N)
+    a, b = _i8(g, M, K), _i8(g, N, K)
+    sa, sb = torch.rand(M, generator=g, device="cuda"), torch.rand(N, generator=g, device="cuda")
+    got = []
+    for arm in (abi.R3D_ARM_EXACT, abi.R3D_ARM_TILE):
+        y = torch.empty(M, N, dtype=BF16, device="cuda")
+        q = abi.R3dGemmI8()
+        q.a, q.a_scale, q.b, q.b_scale, q.y = (t.data_ptr() for t in (a, sa, b, sb, y))
+        q.m, q.n, q.k, q.bs_dtype, q.y_dtype, q.arm = M, N, K, abi.RAD_F32, abi.RAD_BF16, arm
+        q.a_pitch, q.b_pitch, q.y_pitch, q.as_pitch, q.bs_pitch = K, K, N, 1, 1
+        assert ops.plugin().lib.r3d_b200_gemm_i8a8(C.byref(q), torch.cuda.current_stream().cuda_stream) == abi.RAD_OK
+        got.append(y)
+    assert torch.equal(*got)
 
 
 def test_gemm_arms_give_the_same_bits_and_batches_fold():
@@ -261,6 +286,58 @@ def test_sample_one_filter(V, dt, only):
     t, k = t + 0.1, k.clamp_min(1)
     u = torch.rand(M, generator=g, device="cuda")
     _check_sample(x, u, t if only == "t" else None, k if only == "k" else None, p if only == "p" else None, low if only == "low" else None)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("V,ks", [(3000, (257, 300, 1000, 2000, 2999)), (70000, (257, 999, 4000, 30000, 69000))])
+def test_sample_large_k_alone_and_with_top_p(V, ks, dt):
+    g = _rng(V + 1)
+    M = len(ks)
+    x = (torch.randn(M, V, generator=g, device="cuda") * 1.5).to(dt)
+    u, k = torch.rand(M, generator=g, device="cuda"), torch.tensor(ks, dtype=torch.int32, device="cuda")
+    for t in (0.05, 1.0, 20.0):
+        t = torch.full((M,), t, device="cuda")
+        _check_sample(x, u, t, k)
+        _check_sample(x, u, t, k, torch.tensor([0.3, 0.99, 0.9, 0.5, 0.999], device="cuda"))
+
+
+@pytest.mark.parametrize("V", [1200, 60000])
+def test_sample_rows_whose_logits_lie_next_to_each_other(V):
+    """more tokens in a step of the histogram than are gathered: the key is searched"""
+    g = _rng(V)
+    x = torch.stack([torch.rand(V, generator=g, device="cuda") * s + o for s, o in ((1e-3, 0.0), (1e-3, 5.0), (0.01, -3.0), (1e-30, 0.0))])
+    x[3, 7] = -1e-3
+    u = torch.rand(4, generator=g, device="cuda")
+    p = torch.tensor([0.5, 0.9, 0.25, 0.7], device="cuda")
+    k = torch.tensor([V // 2, V - 1, V // 3, V // 2], dtype=torch.int32, device="cuda")
+    _check_sample(x, u, None, None, p)
+    _check_sample(x, u, None, k, None)
+    _check_sample(x, u, None, k, p)
+    two = torch.where(torch.rand(4, V, generator=g, device="cuda") < 0.4, 2.0, 2.015625).to(BF16)
+    _check_sample(two, u, None, None, p)
+    _check_sample(two, u, None, k, p)
+
+
+def test_sample_temperatures_far_apart():
+    g = _rng(77)
+    M, V = 8, 20000
+    x = torch.randn(M, V, generator=g, device="cuda") * 3
+    t = torch.tensor([1e-4, 1e-2, 0.1, 0.3, 3.0, 30.0, 1e4, math.inf], device="cuda")
+    u, p = torch.rand(M, generator=g, device="cuda"), torch.full((M,), 0.97, device="cuda")
+    k = torch.full((M,), 60, dtype=torch.int32, device="cuda")
+    _check_sample(x, u, t)
+    _check_sample(x, u, t, None, p)
+    _check_sample(x, u, t, k, p, torch.full((M,), 0.02, device="cuda"))
+
+
+@pytest.mark.parametrize("V,dt", [(500001, F32), (700001, F32), (900001, F32), (1300001, BF16)])
+def test_sample_long_vocabularies(V, dt):
+    """from what sixteen CTAs keep to what they cannot"""
+    g = _rng(V)
+    x = (torch.randn(3, V, generator=g, device="cuda") * 2).to(dt)
+    u = torch.rand(3, generator=g, device="cuda")
+    k = torch.tensor([0, 50, 7000], dtype=torch.int32, device="cuda")
+    _check_sample(x, u, None, k, torch.tensor([0.8, 0.9, 1.0], device="cuda"))
 
 
 def test_sample_flat_and_tied_rows():
