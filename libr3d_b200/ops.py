@@ -1,5 +1,6 @@
 """The ops of the quantised-matmul path as a caller issues them: `gemm_nt_q` and
-`logits_gemm`, with device tensors (torch is used for device memory and streams only).
+`logits_gemm`, the int8 step around `gemm_i8a8`, and the sampler behind the logits, with device tensors (torch is used
+for device memory and streams only).
 
 Each call does what the radiance engine does for the op: resolve the band to a row by the
 rows' constraints and priorities, then call that row's `launch` with a RadArgs on the
@@ -41,6 +42,27 @@ def _desc(t: torch.Tensor | None, dtype: int, shape=None, stride=None) -> abi.Ra
                        stride if stride is not None else t.stride())
 
 
+def _group_of(dtype: str, K: int) -> int:
+    return {"fp8a8": 128, "i8a8": K}.get(dtype, 32)
+
+
+def _gemm_descs(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, y: torch.Tensor,
+                dtype: str, K: int) -> list[abi.RadTensor]:
+    """gemm_nt_q's operands by schema position, a_sum and b_ref absent."""
+    adt, ydt = abi.RAD_F8E4M3, abi.RAD_BF16
+    sdt = abi.RAD_F32 if b_scale.dtype == torch.float32 else abi.RAD_BF16
+    if dtype == "fp8a8":
+        bdesc = _desc(b, abi.RAD_F8E4M3)
+    elif dtype == "i8a8":
+        adt, bdesc = abi.RAD_I8, _desc(b, abi.RAD_I8)
+        ydt = abi.RAD_F32 if y.dtype == torch.float32 else abi.RAD_BF16
+    else:
+        bdesc = _desc(b, abi.RAD_FP4E2M1, shape=[b.shape[0], K], stride=[K, 1])
+        sdt = abi.RAD_E8M0
+    return [_desc(a, adt), _desc(a_scale, abi.RAD_F32), bdesc, _desc(b_scale, sdt), _desc(y, ydt),
+            _desc(None, abi.RAD_F32), _desc(None, abi.RAD_BF16)]
+
+
 def gemm_nt_q(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
               y: torch.Tensor, *, dtype: str, N: int, K: int, group: int | None = None,
               M_param: int | None = None, row: str | None = None) -> Row:
@@ -49,13 +71,15 @@ def gemm_nt_q(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     a: uint8 e4m3 codes [M,K]; a_scale: float32 [M, K/128]
     dtype "fp8a8":   b uint8 e4m3 codes [N,K]; b_scale bf16 (or f32) [N/128 | N, K/128]
     dtype "mxfp4a8": b uint8 packed e2m1 [N,K/2] (low nibble = even k); b_scale uint8 E8M0 [N,K/32]
+    dtype "i8a8":    a int8 codes, a_scale float32 [M] or [M,1]; b int8 codes [N,K]; b_scale f32 or bf16 [N] or [N,1];
+                     y bf16 or f32 (gemm_i8a8 is the same with y made for the caller)
     `row` forces a row by name; otherwise the band is resolved like the engine would.
     Returns the row that served the call; raises RowRefused on a nonzero status.
     """
     P = plugin()
     M = y.numel() // N
     if group is None:
-        group = 128 if dtype == "fp8a8" else 32
+        group = _group_of(dtype, K)
     query: dict[str, Any] = dict(M=M_param if M_param is not None else M, N=N, K=K,
                                  group=group, dtype=dtype)
     if row is None:
@@ -64,16 +88,7 @@ def gemm_nt_q(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
             raise RuntimeError(f"no row serves gemm_nt_q {query}")
     else:
         r = next(x for x in P.rows() if x.name == row)
-    if dtype == "fp8a8":
-        bdesc = _desc(b, abi.RAD_F8E4M3)
-        sdt = abi.RAD_F32 if b_scale.dtype == torch.float32 else abi.RAD_BF16
-    else:
-        bdesc = _desc(b, abi.RAD_FP4E2M1, shape=[b.shape[0], K], stride=[K, 1])
-        sdt = abi.RAD_E8M0
-    tensors = [_desc(a, abi.RAD_F8E4M3), _desc(a_scale, abi.RAD_F32), bdesc,
-               _desc(b_scale, sdt), _desc(y, abi.RAD_BF16), _desc(None, abi.RAD_F32),
-               _desc(None, abi.RAD_BF16)]
-    pack = ArgPack(tensors, query)
+    pack = ArgPack(_gemm_descs(a, a_scale, b, b_scale, y, dtype, K), query)
     rc = P.launch_row(r, pack, _stream())
     if rc != abi.RAD_OK:
         raise RowRefused(r.name, rc)
@@ -399,22 +414,14 @@ class BoundGemm:
                  row: str | None = None):
         P = plugin()
         M = y.numel() // N
-        group = 128 if dtype == "fp8a8" else 32
+        group = _group_of(dtype, K)
         query: dict[str, Any] = dict(M=M, N=N, K=K, group=group, dtype=dtype)
         self.row = (P.resolve("gemm_nt_q", query) if row is None
                     else next(x for x in P.rows() if x.name == row))
         if self.row is None:
             raise RuntimeError(f"no row serves gemm_nt_q {query}")
-        if dtype == "fp8a8":
-            bdesc = _desc(b, abi.RAD_F8E4M3)
-            sdt = abi.RAD_F32 if b_scale.dtype == torch.float32 else abi.RAD_BF16
-        else:
-            bdesc = _desc(b, abi.RAD_FP4E2M1, shape=[b.shape[0], K], stride=[K, 1])
-            sdt = abi.RAD_E8M0
         self._keep = (a, a_scale, b, b_scale, y)
-        self.pack = ArgPack([_desc(a, abi.RAD_F8E4M3), _desc(a_scale, abi.RAD_F32), bdesc,
-                             _desc(b_scale, sdt), _desc(y, abi.RAD_BF16),
-                             _desc(None, abi.RAD_F32), _desc(None, abi.RAD_BF16)], query)
+        self.pack = ArgPack(_gemm_descs(a, a_scale, b, b_scale, y, dtype, K), query)
         self._fn = P._launch_t(self.row.launch)
         import ctypes as _C
         self._argp = _C.byref(self.pack.args)

@@ -100,6 +100,21 @@ def test_gemm_arms_give_the_same_bits(M, N, K):
     assert torch.equal(*got)
 
 
+def test_gemm_by_the_ops_general_entry_and_declared_once():
+    g = _rng(6)
+    M, N, K = 9, 200, 384
+    a, b = _i8(g, M, K), _i8(g, N, K)
+    sa, sb = torch.rand(M, 1, generator=g, device="cuda"), torch.rand(N, 1, generator=g, device="cuda")
+    for out in (BF16, F32):
+        want = ops.gemm_i8a8(a, sa, b, sb, out_dtype=out)
+        y = torch.empty_like(want)
+        assert ops.gemm_nt_q(a, sa, b, sb, y, dtype="i8a8", N=N, K=K).name == "gemm_nt_q_i8a8"
+        assert torch.equal(y, want)
+        y.zero_()
+        ops.BoundGemm(a, sa, b, sb, y, dtype="i8a8", N=N, K=K).issue()
+        assert torch.equal(y, want)
+
+
 def test_gemm_arms_give_the_same_bits_and_batches_fold():
     g = _rng(3)
     a, b = _i8(g, 2, 21, 640), _i8(g, 384, 640)
