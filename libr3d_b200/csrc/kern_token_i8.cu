@@ -227,6 +227,9 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
     };
     int first = lead() + (int)threadIdx.x * 8;
     fetch(first);
+    /* a norm's two reductions lie a barrier apart each; the other kinds have one barrier a row, so that a warp may be a row
+     * ahead of another that still reads: their rows take the two places by turns */
+    int turn = 1;
     for (; row < rows; row += gridDim.x) {
         f2 h[C][4];
         f2 ss = 0, bad = 0;
@@ -305,7 +308,8 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
             parts_of(bad, f);
             if (f[0] != 0.0f || f[1] != 0.0f) amax = amax < INFINITY ? NAN : amax;
         }
-        amax = block_reduce(amax, part[1], max_nan);
+        amax = block_reduce(amax, part[turn], max_nan);
+        if (KIND != kRms) turn ^= 1;
         const float step = step_of(amax);
         if (threadIdx.x == 0) P.scale[row * P.s_pitch] = scale_of(amax);
         const f2 step2 = two_of(step, step), code2 = two_of(kCode, kCode);

@@ -211,6 +211,24 @@ def test_rmsnorm_quant_token(n, dt, res):
     assert s[1].item() == 1.0 and not q[1].any()
 
 
+@pytest.mark.parametrize("n", [512, 2056, 5120])
+def test_many_rows_of_scales_far_apart(n):
+    """a block walks many rows, one behind the other: each keeps its own largest value"""
+    g = _rng(n + 3)
+    M = 30000
+    amp = 2.0 ** torch.randint(-40, 40, (M, 1), generator=g, device="cuda")
+    x = (torch.randn(M, n, generator=g, device="cuda") * amp).to(BF16)
+    q, s = ops.quant_token_i8(x)
+    want = x.double().abs().amax(-1, keepdim=True) / 127           # one rounding to f32: half a step, 2^-24
+    assert bool(((s.double() - want).abs() <= 2.0 ** -24 * want).all())
+    assert bool((q.abs().amax(-1) == 127).all())
+    q, s = ops.gated_quant_token_i8(x)
+    assert bool((q.abs().amax(-1) == 127).all())
+    for i in range(0, M, 5000):
+        one_q, one_s = ops.gated_quant_token_i8(x[i:i + 3])
+        assert torch.equal(one_q, q[i:i + 3]) and torch.equal(one_s, s[i:i + 3])
+
+
 def test_producers_on_views_leave_the_rest():
     g = _rng(11)
     x = torch.randn(6, 3 * 200 + 5, generator=g, device="cuda").to(BF16)
