@@ -13,7 +13,8 @@
  * Bound by memory: x is read once (rmsnorm also reads and writes the residual), one byte a value is written. So a
  * block owns a row and keeps h in registers between the reduction and the codes: k_token_i8_regs, eight values a
  * thread and chunk, by 16-byte loads where every operand's rows lie on the 16-byte grid (codes: 8), else one value at
- * a time, neighbouring threads next to each other. Rows of more than 32768 values are read again for each step.
+ * a time, neighbouring threads next to each other. Rows of more than 32760 values, or of f32 values and two streams beyond
+ * 27648, which the shared memory does not hold, are read again for each step.
  */
 #include <atomic>
 #include <cmath>
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
     }
 }
 
-/* rows of more than 32768 values, any alignment: read again for each of the steps (they stay in the caches) */
+/* rows too long for that, any alignment: read again for each of the steps (they stay in the caches) */
 template <int KIND, typename T>
 __global__ void __launch_bounds__(512) k_token_i8(const TokenI8 P) {
     __shared__ float part[2][32];
@@ -375,6 +376,14 @@ __global__ void __launch_bounds__(512) k_token_i8(const TokenI8 P) {
     }
 }
 
+constexpr int kSlotBytes = 224 * 1024;
+/* a row's values as they are fetched; the threads' places are at most a warp's of 32 values each more (8 KiB of f32 pairs) */
+template <int KIND, typename T>
+bool fits_slots(const TokenI8& P) {
+    const int streams = KIND == kQuant || (KIND == kRms && !P.res) ? 1 : 2;
+    return P.n <= 32760 && (int64_t)P.n * streams * (int)sizeof(T) <= kSlotBytes - 8 * 1024;
+}
+
 template <int KIND, typename T, int C, bool GRID>
 int launch_rows(const TokenI8& P, int rows, int threads, cudaStream_t st) {
     const int one = KIND == kQuant || (KIND == kRms && !P.res), smem = threads * C * 8 * (int)sizeof(T) * (one ? 1 : 2);
@@ -386,7 +395,7 @@ int launch_rows(const TokenI8& P, int rows, int threads, cudaStream_t st) {
     int grid = known.load(std::memory_order_relaxed);
     if (!grid) {
         int per = 0, sms = 0;
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess ||
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlotBytes) != cudaSuccess ||
             cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem) != cudaSuccess ||
             cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
             return RAD_E_DEVICE;
@@ -420,7 +429,7 @@ int launch_type(const TokenI8& P, int rows, cudaStream_t st) {
     const bool grid = P.n % 8 == 0 && rows_on(P.x, P.x_pitch, esz, 16) && rows_on(P.res, P.r_pitch, esz, 16) && rows_on(P.w, 0, 1, 16) &&
                       rows_on(P.q, P.q_pitch, 1, 8);
     int rc = RAD_OK;
-    if (P.n > 32760) k_token_i8<KIND, T><<<(unsigned)rows, 512, 0, st>>>(P);
+    if (!fits_slots<KIND, T>(P)) k_token_i8<KIND, T><<<(unsigned)rows, 512, 0, st>>>(P);
     else rc = grid ? launch_regs<KIND, T, true>(P, rows, st) : launch_regs<KIND, T, false>(P, rows, st);
     return rc != RAD_OK ? rc : cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
 }

@@ -229,6 +229,14 @@ def test_many_rows_of_scales_far_apart(n):
         assert torch.equal(one_q, q[i:i + 3]) and torch.equal(one_s, s[i:i + 3])
 
 
+@pytest.mark.parametrize("n", [24000, 25613, 27641, 27648, 27649, 28000, 32753, 32760, 32761])
+def test_wide_rows_of_two_f32_streams(n):
+    """next to what the shared memory of a block holds"""
+    test_gated_quant_token(n, F32, "silu")
+    test_rmsnorm_quant_token(n, F32, True)
+    test_gated_quant_token(n, BF16, "silu")
+
+
 def test_producers_on_views_leave_the_rest():
     g = _rng(11)
     x = torch.randn(6, 3 * 200 + 5, generator=g, device="cuda").to(BF16)
