@@ -87,7 +87,7 @@ def gemm_nt_q(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
         if r is None:
             raise RuntimeError(f"no row serves gemm_nt_q {query}")
     else:
-        r = next(x for x in P.rows() if x.name == row)
+        r = next(x for x in P.rows() + P.ext_rows() if x.name == row)
     pack = ArgPack(_gemm_descs(a, a_scale, b, b_scale, y, dtype, K), query)
     rc = P.launch_row(r, pack, _stream())
     if rc != abi.RAD_OK:
@@ -417,7 +417,7 @@ class BoundGemm:
         group = _group_of(dtype, K)
         query: dict[str, Any] = dict(M=M, N=N, K=K, group=group, dtype=dtype)
         self.row = (P.resolve("gemm_nt_q", query) if row is None
-                    else next(x for x in P.rows() if x.name == row))
+                    else next(x for x in P.rows() + P.ext_rows() if x.name == row))
         if self.row is None:
             raise RuntimeError(f"no row serves gemm_nt_q {query}")
         self._keep = (a, a_scale, b, b_scale, y)

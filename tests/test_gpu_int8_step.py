@@ -113,6 +113,9 @@ def test_gemm_by_the_ops_general_entry_and_declared_once():
         y.zero_()
         ops.BoundGemm(a, sa, b, sb, y, dtype="i8a8", N=N, K=K).issue()
         assert torch.equal(y, want)
+        y.zero_()
+        ops.gemm_nt_q(a, sa, b, sb, y, dtype="i8a8", N=N, K=K, row="gemm_nt_q_i8a8")
+        assert torch.equal(y, want)
 
 
 def test_gemm_arms_give_the_same_bits_and_batches_fold():
@@ -499,3 +502,64 @@ def test_a_step_of_them_captured_and_replayed():
         graph.replay()
         again = step(x * (1 + seed), res.clone())
         assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.parametrize("M", [3, 90, 300])
+def test_two_streams_at_once_and_again(M):
+    """the same calls on two streams at a time, many times over: every answer is the first one's"""
+    g = _rng(21 + M)
+    H, N = 1280, 1536
+    x = torch.randn(M, H, generator=g, device="cuda").to(BF16)
+    w = torch.ones(H, device="cuda")
+    b, sb = ops.quant_token_i8(torch.randn(N, H, generator=g, device="cuda"))
+    c, sc = ops.quant_token_i8(torch.randn(6000, N // 2, generator=g, device="cuda"))
+    u = torch.rand(M, generator=g, device="cuda")
+    p = torch.full((M,), 0.8, device="cuda")
+
+    def step():
+        q, s = ops.rmsnorm_quant_token_i8(x, w, eps=1e-6)
+        q, s = ops.gated_quant_token_i8(ops.gemm_i8a8(q, s, b, sb))
+        logits = ops.gemm_i8a8(q, s, c, sc)
+        return q, s, logits, ops.sample_nucleus(logits, u, top_p=p)
+
+    want = step()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(step())
+    torch.cuda.synchronize()
+    for one in got:
+        assert all(torch.equal(a, b) for a, b in zip(want, one))
+
+
+def test_norm_written_over_its_input():
+    g = _rng(30)
+    x = torch.randn(700, 1000, generator=g, device="cuda").to(BF16)
+    w = torch.rand(1000, generator=g, device="cuda")
+    out = torch.empty_like(x)
+    q, s = ops.rmsnorm_quant_token_i8(x, w, eps=1e-5, out=out)
+    again = ops.rmsnorm_quant_token_i8(x, w, eps=1e-5, out=x)
+    assert torch.equal(x, out) and torch.equal(q, again[0]) and torch.equal(s, again[1])
+
+
+def test_rows_and_tokens_beyond_32_bit_offsets():
+    """logits, codes and results of more than 2^31 elements: the last rows are those of a call of their own"""
+    M, V = 70000, 32001
+    x = torch.empty(M, V, dtype=BF16, device="cuda")
+    g = _rng(31)
+    x[-3:] = (torch.randn(3, V, generator=g, device="cuda") * 4).to(BF16)
+    x[:-3] = x[-1:]
+    u = torch.rand(M, generator=g, device="cuda")
+    token = ops.sample_nucleus(x, u, top_k=torch.full((1,), 30, dtype=torch.int32, device="cuda").expand(M))
+    assert torch.equal(token[-3:], ops.sample_nucleus(x[-3:].clone(), u[-3:], top_k=torch.full((3,), 30, dtype=torch.int32, device="cuda")))
+    q, s = ops.quant_token_i8(x)
+    one_q, one_s = ops.quant_token_i8(x[-3:].clone())
+    assert torch.equal(q[-3:], one_q) and torch.equal(s[-3:], one_s)
+    del x
+    b, sb = _i8(g, 24, V), torch.rand(24, generator=g, device="cuda")
+    assert torch.equal(ops.gemm_i8a8(q, s, b, sb)[-3:], ops.gemm_i8a8(one_q, one_s, b, sb))
+    b, sb = _i8(_rng(32), 32768, 32), torch.rand(32768, generator=_rng(33), device="cuda")
+    y = ops.gemm_i8a8(q[:, :32].contiguous(), s, b, sb)
+    assert y.numel() > 2 ** 31
+    assert torch.equal(y[-3:], ops.gemm_i8a8(one_q[:, :32].contiguous(), one_s, b, sb))

@@ -1,5 +1,6 @@
 """Host side of the int8 band and the sampler, no GPU needed: their rows, levers and refusals (every call here is
 refused before any device work)."""
+import ctypes as C
 import os
 import subprocess
 import sys
@@ -109,6 +110,34 @@ SAMPLE = dict(logits=T(Z, F, [3, 9]), u=T(Z, F, [3]), temperature=ABSENT, top_k=
 ])
 def test_sample_refusals(plug, over, rc):
     assert _call(plug, "r3d_rad_sample_nucleus", SAMPLE, dict(M=3, n_vocab=9, dtype="f32"), over) == rc
+
+
+def _struct(which, **over):
+    fields = {
+        "gemm": dict(a=Z, a_scale=Z, b=Z, b_scale=Z, y=Z, m=2, n=8, k=16, bs_dtype=F, y_dtype=B, arm=abi.R3D_ARM_AUTO, a_pitch=16, b_pitch=16, y_pitch=8,
+                     as_pitch=1, bs_pitch=1),
+        "norm": dict(x=Z, residual=None, w=Z, q=Z, scale=Z, out=None, kind=abi.R3D_TOKEN_RMSNORM, x_dtype=B, w_dtype=F, out_dtype=B, rows=2, n=8, eps=1e-6,
+                     x_pitch=8, r_pitch=8, q_pitch=8, s_pitch=1, out_pitch=8),
+        "sample": dict(logits=Z, u=Z, token=Z, logprob=None, kept=None, rows=2, n_vocab=8, x_dtype=F, x_pitch=8, u_pitch=1, token_pitch=1, lp_pitch=1, kept_pitch=1),
+    }[which] | over
+    s = {"gemm": abi.R3dGemmI8, "norm": abi.R3dTokenI8, "sample": abi.R3dNucleus}[which]()
+    for k, v in fields.items():
+        setattr(s, k, v)
+    return s
+
+
+@pytest.mark.parametrize("kind,over,rc", [
+    ("gemm", dict(b=None), INVAL), ("gemm", dict(a_scale=None), INVAL), ("gemm", dict(m=0), SHAPE), ("gemm", dict(k=131072), SHAPE), ("gemm", dict(n=1 << 28), SHAPE),
+    ("gemm", dict(a_pitch=-16), STRIDE), ("gemm", dict(y_pitch=7), STRIDE), ("gemm", dict(bs_dtype=abi.RAD_F16), DTYPE), ("gemm", dict(y_dtype=I8), DTYPE),
+    ("norm", dict(w=None), INVAL), ("norm", dict(kind=4), INVAL), ("norm", dict(kind=-1), INVAL), ("norm", dict(kind=abi.R3D_TOKEN_QUANT), INVAL),
+    ("norm", dict(x_dtype=abi.RAD_F16), DTYPE), ("norm", dict(w_dtype=I8), DTYPE), ("norm", dict(out=Z, out_dtype=I8), DTYPE), ("norm", dict(rows=0), SHAPE),
+    ("norm", dict(q_pitch=7), STRIDE), ("norm", dict(residual=Z, r_pitch=0), STRIDE), ("norm", dict(s_pitch=0), STRIDE), ("norm", dict(x_pitch=-8), STRIDE),
+    ("sample", dict(token=None), INVAL), ("sample", dict(x_dtype=abi.RAD_F16), DTYPE), ("sample", dict(n_vocab=0), SHAPE), ("sample", dict(rows=-1), SHAPE),
+    ("sample", dict(token_pitch=0), STRIDE), ("sample", dict(u_pitch=-1), STRIDE), ("sample", dict(kept=Z, kept_pitch=0), STRIDE),
+])
+def test_launch_layer_refusals(plug, kind, over, rc):
+    call = {"gemm": plug.lib.r3d_b200_gemm_i8a8, "norm": plug.lib.r3d_b200_token_i8, "sample": plug.lib.r3d_b200_sample_nucleus}[kind]
+    assert call(C.byref(_struct(kind, **over)), None) == rc
 
 
 def test_ops_refuse_what_they_cannot_take():
