@@ -362,11 +362,12 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
 constexpr int kStreamThreads = 32 * 6;
 constexpr int kMaxShares = 8;                      /* a portable cluster */
 constexpr size_t kStreamSmem = 220 * 1024;
+constexpr int kMaxStages = 16;                     /* 88 KiB of 7 KiB or 190 KiB of 15 KiB: 12 */
 
 __global__ void __launch_bounds__(kStreamThreads, 2)
 k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const I8Params P) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint64_t full[16], empty[16], done;       /* at most 88 KiB / 7 KiB or 190 KiB / 21 KiB stages */
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
     __shared__ uint32_t tmem_slot;
     __shared__ float sa_s[128];
     __shared__ __align__(16) float sb_s[256];
@@ -620,28 +621,50 @@ int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     if (!allow_smem(k_i8_stream, kStreamSmem, set)) return RAD_E_DEVICE;
     I8Params P = params_of(p);
     P.mb = (p.m + 7) / 8 * 8;
-    /* Up to 64 tokens two CTAs an SM with 96 channels each, above one with 192. A K block costs a CTA about 145 ns
-     * however few channels it has (measured from 16 to 64), so where those tiles leave slots idle, the CTAs of a
-     * cluster share K instead of taking fewer channels each: 5120 channels, K = 13824, 16 tokens take 15.0 us with 54
-     * tiles x 4 shares, 22.4 us with 160 tiles of 32. A share is at least eight K blocks (4096 x 4096: 4 shares 6.6 us,
-     * 8 shares 6.9 us). Where they do not, the tile is the multiple of 16 with which the last wave is fullest. */
-    const int per_sm = P.mb <= 64 ? 2 : 1, base = per_sm == 2 ? 96 : 192, slots = tc_sm_count() * per_sm;
-    const int tiles0 = (p.n + base - 1) / base;
-    P.nt = base;
-    P.shares = slots / tiles0;
-    if (P.shares > kMaxShares) P.shares = kMaxShares;
-    if (P.shares > P.nk / 8) P.shares = P.nk / 8;
-    while (P.shares > 1 && per_sm * resident_clusters(tc_device(), P.shares) < tiles0) --P.shares;
-    if (P.shares < 2) {
-        P.shares = 1;
+    const int sms = tc_sm_count();
+    const int per_sm = P.mb <= 64 || p.n >= 160 * sms ? 2 : 1, slots = sms * per_sm;
+    P.shares = 1;
+    if (per_sm == 1) {
+        /* 65 tokens and more, fewer than 160 channels an SM: a CTA has an SM, and the channels of a tile and the K shares are
+         * those with the lowest cost of a K block (its two operands' way into shared memory), of a tile's results, and of
+         * adding the shares' sums, in nanoseconds, fitted to 540 measured forms of thirteen sizes (12288 channels, K = 4096,
+         * 128 tokens: 128 tiles of 96 14.8 us, 192 channels in two shares 19.0 us; 5120, 13824: 4 shares of 160 channels
+         * 18.6 us, 2 of 80 18.8, 4 of 192 19.9). Beyond 160 channels an SM two CTAs, one's results under the other's loads
+         * (27648, 5120, 128 tokens: 29.2 us, one CTA of 192 channels 31.4; 20480, 4096: 20.0 us and, with one, 19.7). */
         long best = -1;
-        for (int nt = base / 2; nt <= base * 4 / 3; nt += 16) {
-            const long tiles = (p.n + nt - 1) / nt, cost = (tiles + slots - 1) / slots * (nt + 16 + P.mb / 4);
-            if (best < 0 || cost <= best) { best = cost; P.nt = nt; }
+        for (int nt = 48; nt <= 256; nt += 16)
+            for (int sh = 1; sh <= kMaxShares && (sh == 1 || 5 * sh <= P.nk); ++sh) {
+                const long tiles = (p.n + nt - 1) / nt;
+                if (sh > 1 && (tiles * sh > slots || tiles > resident_clusters(tc_device(), sh))) break;
+                const long cost = (tiles * sh + slots - 1) / slots * ((P.nk + sh - 1) / sh * (61 + 5L * (P.mb + nt) / 8) + (long)P.mb * nt / 5) +
+                                  (sh > 1 ? (long)P.mb * nt / 20 : 0);
+                if (best < 0 || cost < best) { best = cost; P.nt = nt; P.shares = sh; }
+            }
+    } else {
+        /* Two CTAs an SM with 96 channels each. A K block costs a CTA about 145 ns however few channels it has (measured
+         * from 16 to 64), so where those tiles leave slots idle, the CTAs of a cluster share K instead of taking fewer
+         * channels each: 5120 channels, K = 13824, 16 tokens take 15.0 us with 54 tiles x 4 shares, 22.4 us with 160 tiles
+         * of 32 (other forms of 64 to 128 channels and 3 to 6 shares: 14.8 to 15.3). A share is at least eight K blocks
+         * (4096 x 4096: 4 shares 6.6 us, 8 shares 6.9 us). Where they do not, the tile is the multiple of 16 with which the
+         * last wave is fullest. */
+        const int tiles0 = (p.n + 95) / 96;
+        P.nt = 96;
+        P.shares = slots / tiles0;
+        if (P.shares > kMaxShares) P.shares = kMaxShares;
+        if (P.shares > P.nk / 8) P.shares = P.nk / 8;
+        while (P.shares > 1 && per_sm * resident_clusters(tc_device(), P.shares) < tiles0) --P.shares;
+        if (P.shares < 2) {
+            P.shares = 1;
+            long best = -1;
+            for (int nt = 48; nt <= 128; nt += 16) {
+                const long tiles = (p.n + nt - 1) / nt, cost = (tiles + slots - 1) / slots * (nt + 16 + P.mb / 4);
+                if (best < 0 || cost <= best) { best = cost; P.nt = nt; }
+            }
         }
     }
     const int tiles = (p.n + P.nt - 1) / P.nt, stage = (P.mb + P.nt) * kStageK;
     P.stages = (per_sm == 2 ? 88 * 1024 : 190 * 1024) / stage;
+    if (P.stages > kMaxStages) P.stages = kMaxStages;
     const int esz = P.y_f32 ? 4 : 2;
     P.y_quads = (((uintptr_t)p.y | (uintptr_t)(p.y_pitch * esz)) & (uintptr_t)(4 * esz - 1)) == 0;
     /* the MMA reads 128 token rows from wherever the token tile starts: the last stage's reach 16 KiB on */

@@ -58,6 +58,12 @@ def test_gemm_against_whole_numbers(M, N, K, out):
     _check_gemm(a, sa, b, sb, ops.gemm_i8a8(a, sa, b, sb, out_dtype=out))
 
 
+@pytest.mark.parametrize("M,N,K", [(65, 700, 5120), (72, 24001, 400), (96, 5119, 4112), (100, 2560, 8192), (113, 30000, 256), (127, 9000, 1296), (128, 96, 20000)])
+def test_gemm_tiles_and_shares_up_to_128_tokens(M, N, K):
+    test_gemm_against_whole_numbers(M, N, K, BF16)
+    test_gemm_against_whole_numbers(M, N, K, F32)
+
+
 def test_gemm_extremes_stay_inside_32_bits():
     K = 131071
     a = torch.full((3, K), -128, dtype=torch.int8, device="cuda")
