@@ -16,7 +16,6 @@
 #include <atomic>
 #include <cmath>
 #include <cstddef>
-#include <cstdlib>
 #include "r3d_kernels.h"
 #include "r3d_numerics.cuh"
 
@@ -308,7 +307,7 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
     return v;
 }
 
-static_assert(offsetof(Shared, sel) % 16 == 0, "read by 16 bytes");
+static_assert(offsetof(Shared, sel) % 16 == 0 && sizeof(Shared) % 16 == 0, "read by 16 bytes");
 static_assert(offsetof(Shared, parts) % 8 == 0 && offsetof(Shared, mine) % 8 == 0 && sizeof(Part) % 8 == 0, "sent by 8 bytes");
 /* the cluster, the same in every thread of it */
 struct Cluster {
@@ -401,17 +400,28 @@ template <typename K> __device__ __forceinline__ uint32_t wide(K k);
 template <> __device__ __forceinline__ uint32_t wide<uint32_t>(uint32_t k) { return k; }
 template <> __device__ __forceinline__ uint32_t wide<uint16_t>(uint16_t k) { return k & 0x8000u ? (uint32_t)k << 16 : k ? (uint32_t)k << 16 | 0xffffu : 0u; }
 
+/* key_of by the integer pipe alone: +0 folds -0; the keys of what is not masked lie next to each other */
+__device__ __forceinline__ uint32_t key_fast(uint32_t bits) {
+    const int v = __float_as_int(__uint_as_float(bits) + 0.0f);
+    const uint32_t k = (uint32_t)v ^ ((uint32_t)(v >> 31) | 0x80000000u);
+    return k - 0x00800000u <= 0xff000000u ? k : 0u;               /* from the least number to +inf */
+}
+
 template <typename K>
 __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const int e) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared* const s = (Shared*)raw;
-    K* const keys = (K*)(raw + sizeof(Shared));
+    constexpr int kEach = 16 / (int)sizeof(K);                    /* values of 16 bytes, as logits and as keys */
     Cluster cl;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cl.size));
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cl.rank));
     cl.s = s; cl.turn = 0;
     const int64_t m = blockIdx.x / cl.size;
     const int V = P.n_vocab, base = cl.rank * kT * e, tid = threadIdx.x;
+    /* the keys lie to the 16-byte grid as the logits do */
+    const K* const x = (const K*)P.logits + m * P.x_pitch + base;
+    const int lead = (int)((uintptr_t)x & 15) / (int)sizeof(K);
+    K* const keys = (K*)(raw + sizeof(Shared)) + lead;
     const K* const own = keys + tid * e;                          /* ids own_id ... own_id + e - 1 */
     const int own_id = base + tid * e;
     /* the peers' shared memory may be written once they have all begun: waited for below */
@@ -429,23 +439,51 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     {
         uint32_t top = 0;                                         /* the largest key this thread read */
         int at = -1;
-        const int here = min(e, (V - base - tid + kT - 1) / kT);  /* negative: none */
-        /* sixteen loads on their way at a time */
+        const int here = min(kT * e, V - base);                   /* ids of this CTA; negative: none */
+        const auto take = [&](uint32_t bits, int i) {
+            const uint32_t key = key_fast(bits);
+            live += key != 0;
+            if (key > top) { top = key; at = i; }
+            return key;
+        };
+        const auto take_one = [&](int i) {
+            const uint32_t bits = i < here ? (uint32_t)x[i] << (sizeof(K) == 2 ? 16 : 0) : 0xff800000u;
+            keys[i] = (K)(take(bits, i) >> (sizeof(K) == 2 ? 16 : 0));
+        };
+        if (e < 16) {                                             /* few: every thread reads some, for the groups below */
+#pragma unroll 4
+            for (int j = 0; j < e; ++j) take_one(j * kT + tid);
+        } else {
+            constexpr int kFlight = 4;                            /* loads of 16 bytes on their way at a time */
 #pragma unroll 1
-        for (int j0 = 0; j0 < e; j0 += 16) {
-            float x[16];
+            for (int i0 = tid * kEach - lead; i0 < kT * e; i0 += kFlight * kT * kEach) {
+                uint4 w[kFlight];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = j0 + j < here ? load_x(P, m, base + (j0 + j) * kT + tid) : -INFINITY;
+                for (int j = 0; j < kFlight; ++j) {
+                    const int i = i0 + j * kT * kEach;
+                    if (i >= 0 && i + kEach <= here) w[j] = *(const uint4*)(x + i);
+                }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                if (j0 + j >= e) break;
-                const uint32_t key = key_of(x[j]);
-                keys[(j0 + j) * kT + tid] = (K)(sizeof(K) == 2 ? key >> 16 : key);
-                live += key != 0;
-                if (key > top) { top = key; at = j0 + j; }
+                for (int j = 0; j < kFlight; ++j) {
+                    const int i = i0 + j * kT * kEach;
+                    if (i >= 0 && i + kEach <= here) {
+                        uint32_t* const u = (uint32_t*)&w[j];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            if (sizeof(K) == 2) {
+                                const uint32_t a = take(u[c] << 16, i + 2 * c), b = take(u[c] & 0xffff0000u, i + 2 * c + 1);
+                                u[c] = __byte_perm(a, b, 0x7632);
+                            } else u[c] = take(u[c], i + c);
+                        }
+                        *(uint4*)(keys + i) = w[j];
+                    } else {
+#pragma unroll 1
+                        for (int c = 0; c < kEach; ++c) if (i + c >= 0 && i + c < kT * e) take_one(i + c);
+                    }
+                }
             }
         }
-        if (top) best_id = (u64)top << 32 | (0xffffffffu - (uint32_t)(base + at * kT + tid));
+        if (top) best_id = (u64)top << 32 | (0xffffffffu - (uint32_t)(base + at));
 #pragma unroll 1
         for (int o = 1; o < kT / mine_groups; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (tid % (kT / mine_groups) == 0) s->my_tops[tid / (kT / mine_groups)] = top;
@@ -818,7 +856,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
 
 constexpr size_t kRowSmem = 220 * 1024;
 int each_of(int vocab, int size) { return ((vocab + kT * size - 1) / (kT * size)) | 1; }
-size_t row_smem(int vocab, int size, int ksz) { return sizeof(Shared) + (size_t)kT * each_of(vocab, size) * ksz; }
+size_t row_smem(int vocab, int size, int ksz) { return sizeof(Shared) + 16 + (size_t)kT * each_of(vocab, size) * ksz; }
 
 template <typename K>
 int launch_row(const R3dNucleus& P, int size, cudaStream_t st) {
