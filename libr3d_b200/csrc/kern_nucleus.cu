@@ -6,10 +6,10 @@
  * weight reaches p times the weight that top-k left, min-p those with w_i >= min_p; the first token always stays.
  * The answer is the first kept token, by ascending id, whose running weight exceeds u times the kept weight.
  *
- * Weights are whole numbers of 2^-S (S the largest for which a row's sum fits 62 bits; 44 at 151936 tokens), made
- * from 64-bit floating point. Their sums are exact in any order, so the answer depends neither on the order of
- * threads nor on how a row is split, and it agrees with a 64-bit computation except where a running sum is
- * within about sqrt(V) 2^-S of a border.
+ * Weights are whole numbers of 2^-S (S the largest for which a row's sum fits 62 bits; 44 at 151936 tokens). Their
+ * sums are exact in any order, so the answer depends neither on the order of threads nor on how a row is split. A weight
+ * is off by at most 2.3 2^-39 of itself and half a unit (mostly by a fifth of that), so the answer is a 64-bit
+ * computation's except where that one's running sum lies within about 2^-39 of the kept weight of a border.
  *
  * -inf and NaN logits are masked: never kept. A row with nothing left reports token -1, kept 0, logprob -inf.
  */
@@ -73,37 +73,18 @@ __device__ __forceinline__ double exponent_of(const Row& R, uint32_t key) {
     if (R.inf) return isinf(x) ? 0.0 : -HUGE_VAL;
     return (x - R.mx) * R.c;
 }
-/* 2^(exponent + S), rounded to a whole number: 2^n times the Taylor series of 2^r, |r| <= 1/2, to the eleventh power
- * (its remainder is below 2^-47; 2^0 is 1 exactly), rounded by adding 2^52. */
-__device__ __forceinline__ u64 weight_of(const Row& R, uint32_t key) {
-    const double z = exponent_of(R, key) + R.S;
-    if (!key || !(z > -1.5)) return 0;
-    const double whole = z + 6755399441055744.0;                  /* 1.5 * 2^52: the nearest whole number in the low word */
-    const double r = z - (whole - 6755399441055744.0);
-    double p = 4.445538271870811e-10;                             /* ln(2)^i / i!, i = 11 .. 0 */
-    p = fma(p, r, 7.054911620801122e-09);
-    p = fma(p, r, 1.0178086009239699e-07);
-    p = fma(p, r, 1.3215486790144307e-06);
-    p = fma(p, r, 1.5252733804059841e-05);
-    p = fma(p, r, 1.5403530393381608e-04);
-    p = fma(p, r, 1.3333558146428443e-03);
-    p = fma(p, r, 9.618129107628477e-03);
-    p = fma(p, r, 5.5504108664821576e-02);
-    p = fma(p, r, 0.2402265069591007);
-    p = fma(p, r, 0.6931471805599453);
-    p = fma(p, r, 1.0);
-    const double scaled = __hiloint2double(__double2hiint(p) + (__double2loint(whole) << 20), __double2loint(p));
-    return (u64)__double_as_longlong(scaled + 4503599627370496.0) - 0x4330000000000000ull;
-}
-
-/* The same with a table of 2^(i / 128) and the series to the fourth power (its remainder for r <= 2^-8 is below 2^-49):
- * twelve operations of the 64-bit pipe, which does sixteen lanes a clock, instead of nineteen. A table of whole numbers and
- * 64-bit products of them, seventy instructions, was no faster. */
-struct Powers { double of[128]; };
+/* 2^y as a whole number of 2^-S, y = (x - mx) log2(e) / T. One 64-bit multiply-add makes 128 y in fixed point: the high
+ * word its whole part, the low word the fraction r. 2^y is then 2^(whole / 128), by table and exponent, times
+ * 1 + r (C1 + r (C2 + r C3)), the polynomial that meets (2^(r / 128) - 1) / r at the three Chebyshev points of [0, 1], in
+ * 32-bit products of units of 2^-39; one more 64-bit multiply-add rounds by adding 2^52. A row's largest logit weighs 2^S
+ * exactly. No case is tested for: NaN (what is masked) and what lies far below give a high word out of range, which is
+ * held at a weight of a quarter. 22 cycles of a scheduler for a warp's 32; with twelve operations in 64 bits, or with
+ * whole numbers alone (64-bit shifts, half as fast as products), 60. */
+struct Powers { double of[128]; };                                /* 2^(-i / 128) */
 constexpr Powers make_powers() {
     Powers t{};
     for (int i = 0; i < 128; ++i) {
-        const double x = 0.6931471805599453 * i / 128.0;
+        const double x = -0.6931471805599453 * i / 128.0;
         double sum = 1.0, term = 1.0;
         for (int j = 1; j < 30; ++j) { term *= x / j; sum += term; }
         t.of[i] = sum;
@@ -114,24 +95,19 @@ __device__ const Powers kPowers = make_powers();
 
 struct Weigh {
     double mx, c;                                                 /* the largest logit; 128 log2(e) / T */
-    float top, limit;                                             /* the largest again; the distance from which nothing weighs */
+    float top;                                                    /* the largest again */
     int S;
     bool inf;
-    __device__ __forceinline__ u64 of(const double* powers, uint32_t key) const {
-        const float x = val_of(key);
-        if (inf) return key && x == top ? 1ull << S : 0ull;
-        if (!key || !(__fsub_rn(top, x) <= limit)) return 0;
-        const double z = ((double)x - mx) * c, whole = z + 6755399441055744.0;       /* 1.5 * 2^52: the nearest whole number in the low word */
-        const double r = z - (whole - 6755399441055744.0);
-        const int j = __double2loint(whole);
-        constexpr double l = 0.6931471805599453 / 128.0;          /* the series of 2^(r / 128) */
-        double p = l * l * l * l / 24.0;
-        p = fma(p, r, l * l * l / 6.0);
-        p = fma(p, r, l * l / 2.0);
-        p = fma(p, r, l);
-        p = fma(p, r, 1.0) * powers[j & 127];
-        const double scaled = __hiloint2double(__double2hiint(p) + (((j >> 7) + S) << 20), __double2loint(p));
-        return (u64)__double_as_longlong(scaled + 4503599627370496.0) - 0x4330000000000000ull;
+    __device__ __forceinline__ u64 of(const double* powers, float x) const {
+        if (inf) return x == top ? 1ull << S : 0ull;
+        const double z = fma((double)x - mx, c, 1572864.0);       /* 1.5 * 2^20: the fraction is the low word */
+        const uint32_t down = min(0x41380000u - (uint32_t)__double2hiint(z), (uint32_t)(S + 2) << 7);
+        const uint32_t r = (uint32_t)__double2loint(z);
+        const uint32_t q = __umulhi(r, 2977044473u + __umulhi(r, 8060653u + __umulhi(r, 14580u)));
+        const double a = powers[down & 127];
+        const double power = __hiloint2double(__double2hiint(a) + (S << 20) - (int)((down & ~127u) << 13), __double2loint(a));
+        const double more = __longlong_as_double((long long)((u64)q * 8192u + 0x3ff0000000000000ull));
+        return (u64)__double_as_longlong(fma(more, power, 4503599627370496.0)) - 0x4330000000000000ull;
     }
 };
 
@@ -181,6 +157,8 @@ __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
     const float t = P.temperature ? P.temperature[m * P.t_pitch] : 1.0f;
     const bool greedy = !(t > 0.0f);
     const Row R = row_of(best, t, P.shift);
+    const Weigh weigh{R.mx, R.c * 128.0, val_of(best), R.S, R.inf};
+    const auto weight_of = [&](uint32_t key) { return weigh.of(kPowers.of, val_of(key)); };
 
     const int live = sum_if([&](Sum& s, uint32_t k, int) { s.n += k != 0; }).n;
     int k = P.top_k ? P.top_k[m * P.k_pitch] : 0;
@@ -204,15 +182,15 @@ __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
     }
     const float p = P.top_p ? P.top_p[m * P.p_pitch] : 1.0f;
     if (!greedy && p < 1.0f) {
-        const u64 over = sum_if([&](Sum& s, uint32_t key, int) { if (key > cut) s.w += weight_of(R, key); }).w;
-        const u64 total = over + (cut > 1 ? (u64)ties * weight_of(R, cut) : sum_if([&](Sum& s, uint32_t key, int) { if (key == cut) s.w += weight_of(R, key); }).w);
+        const u64 over = sum_if([&](Sum& s, uint32_t key, int) { if (key > cut) s.w += weight_of(key); }).w;
+        const u64 total = over + (cut > 1 ? (u64)ties * weight_of(cut) : sum_if([&](Sum& s, uint32_t key, int) { if (key == cut) s.w += weight_of(key); }).w);
         const u64 want = want_of(p, total);
         if (over >= want) {
-            cut = search([&](uint32_t c) { return sum_if([&](Sum& s, uint32_t key, int) { if (key >= c) s.w += weight_of(R, key); }).w >= want; });
+            cut = search([&](uint32_t c) { return sum_if([&](Sum& s, uint32_t key, int) { if (key >= c) s.w += weight_of(key); }).w >= want; });
             ties = V;
         }
-        const u64 above = sum_if([&](Sum& s, uint32_t key, int) { if (key > cut) s.w += weight_of(R, key); }).w;
-        const u64 one = weight_of(R, cut);
+        const u64 above = sum_if([&](Sum& s, uint32_t key, int) { if (key > cut) s.w += weight_of(key); }).w;
+        const u64 one = weight_of(cut);
         if (one && want > above) ties = (int)min((u64)ties, (want - above + one - 1) / one);
     }
     /* the cut's last kept id */
@@ -229,13 +207,13 @@ __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
     const auto keep = [&](uint32_t key, int i) {
         return key && (key > cut || (key == cut && i <= last)) && (greedy || exponent_of(R, key) >= floor_y);
     };
-    const Sum all = sum_if([&](Sum& s, uint32_t key, int i) { if (keep(key, i)) { ++s.n; s.w += weight_of(R, key); } });
+    const Sum all = sum_if([&](Sum& s, uint32_t key, int i) { if (keep(key, i)) { ++s.n; s.w += weight_of(key); } });
     const float u = P.u[m * P.u_pitch];
     const u64 at = point_of(u, all.w);
     int lo = 0, hi = V - 1;
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (sum_if([&](Sum& s, uint32_t key, int i) { if (i <= mid && keep(key, i)) s.w += weight_of(R, key); }).w > at) hi = mid; else lo = mid + 1;
+        if (sum_if([&](Sum& s, uint32_t key, int i) { if (i <= mid && keep(key, i)) s.w += weight_of(key); }).w > at) hi = mid; else lo = mid + 1;
     }
     if (threadIdx.x == 0) answer(P, m, lo, all.n, logprob_of(R, key_at(lo), all.w));
 }
@@ -270,7 +248,6 @@ struct Shared {
     Part parts[2][kMaxCluster];                                   /* what each CTA says, by turns */
     Part mine;
     double c, floor_y, drop;                                      /* log2(e) / T; min-p as an exponent, and in logits */
-    float limit;
     Powers powers;
     u64 warp_w[kWarps];
     int warp_n[kWarps];
@@ -278,6 +255,7 @@ struct Shared {
     uint32_t my_tops[kT];
     alignas(16) uint32_t sel[kT];                                 /* read by 16 bytes */
     int gathered, pick, from;
+    uint32_t edge[2];
     u64 list[kCap], weight[kCap];                                 /* gathered tokens, key << 32 | ~id; their values */
     union { uint32_t tops[kGroups]; uint32_t hist[kBins]; };   /* the groups' largest keys; this CTA's histogram */
     uint32_t upto[kBins];                                         /* the cluster's, summed up to each step */
@@ -411,19 +389,18 @@ template <typename K>
 __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const int e) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared* const s = (Shared*)raw;
-    constexpr int kEach = 16 / (int)sizeof(K);                    /* values of 16 bytes, as logits and as keys */
+    constexpr int kEach = 16 / (int)sizeof(K), kPer = 4 / (int)sizeof(K);     /* values of 16 bytes and of four, as logits and as keys */
     Cluster cl;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cl.size));
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cl.rank));
     cl.s = s; cl.turn = 0;
     const int64_t m = blockIdx.x / cl.size;
-    const int V = P.n_vocab, base = cl.rank * kT * e, tid = threadIdx.x;
-    /* the keys lie to the 16-byte grid as the logits do */
+    const int V = P.n_vocab, span = kT * e * kPer - kEach, base = cl.rank * span, tid = threadIdx.x;      /* this CTA's ids */
+    /* the keys lie to the 16-byte grid as the logits do, which takes up to 16 bytes more than the ids' own */
     const K* const x = (const K*)P.logits + m * P.x_pitch + base;
     const int lead = (int)((uintptr_t)x & 15) / (int)sizeof(K);
     K* const keys = (K*)(raw + sizeof(Shared)) + lead;
-    const K* const own = keys + tid * e;                          /* ids own_id ... own_id + e - 1 */
-    const int own_id = base + tid * e;
+    const uint32_t* const words = (const uint32_t*)(raw + sizeof(Shared));
     /* the peers' shared memory may be written once they have all begun: waited for below */
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
@@ -439,7 +416,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     {
         uint32_t top = 0;                                         /* the largest key this thread read */
         int at = -1;
-        const int here = min(kT * e, V - base);                   /* ids of this CTA; negative: none */
+        const int here = min(span, V - base);                   /* ids of this CTA; negative: none */
         const auto take = [&](uint32_t bits, int i) {
             const uint32_t key = key_fast(bits);
             live += key != 0;
@@ -450,13 +427,13 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
             const uint32_t bits = i < here ? (uint32_t)x[i] << (sizeof(K) == 2 ? 16 : 0) : 0xff800000u;
             keys[i] = (K)(take(bits, i) >> (sizeof(K) == 2 ? 16 : 0));
         };
-        if (e < 16) {                                             /* few: every thread reads some, for the groups below */
+        if (e * kPer < 16) {                                      /* few: every thread reads some, for the groups below */
 #pragma unroll 4
-            for (int j = 0; j < e; ++j) take_one(j * kT + tid);
+            for (int i = tid; i < span; i += kT) take_one(i);
         } else {
             constexpr int kFlight = 4;                            /* loads of 16 bytes on their way at a time */
 #pragma unroll 1
-            for (int i0 = tid * kEach - lead; i0 < kT * e; i0 += kFlight * kT * kEach) {
+            for (int i0 = tid * kEach - lead; i0 < span; i0 += kFlight * kT * kEach) {
                 uint4 w[kFlight];
 #pragma unroll
                 for (int j = 0; j < kFlight; ++j) {
@@ -478,7 +455,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
                         *(uint4*)(keys + i) = w[j];
                     } else {
 #pragma unroll 1
-                        for (int c = 0; c < kEach; ++c) if (i + c >= 0 && i + c < kT * e) take_one(i + c);
+                        for (int c = 0; c < kEach; ++c) if (i + c >= 0 && i + c < span) take_one(i + c);
                     }
                 }
             }
@@ -488,6 +465,8 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         for (int o = 1; o < kT / mine_groups; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (tid % (kT / mine_groups) == 0) s->my_tops[tid / (kT / mine_groups)] = top;
     }
+    if (tid < lead) keys[tid - lead] = 0;
+    if (tid < kEach - lead) keys[span + tid] = 0;
     if (tid < 128) s->powers.of[tid] = kPowers.of[tid];
     live = __reduce_add_sync(0xffffffffu, live);
 #pragma unroll 1
@@ -502,7 +481,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         if (tid == 0) { s->mine.key = best_id; s->mine.w[0] = (u64)live; s->gathered = 0; }
     } else if (tid < 64) {                                        /* one warp: a quotient and a logarithm in 64 bits */
         const double c = t > 0.0f ? 1.4426950408889634 / (double)t : 0.0, y = floor_of(low);
-        if (tid == 32) { s->c = c; s->floor_y = y; s->drop = y / c; s->limit = (float)((P.shift + 1.25) / c); }
+        if (tid == 32) { s->c = c; s->floor_y = y; s->drop = y / c; }
     }
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 #pragma unroll 1
@@ -528,8 +507,35 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     Row R;
     R.c = s->c; R.mx = (double)val_of(best); R.inf = isinf(val_of(best)); R.S = P.shift;
     const bool by_k = k < live, by_p = p < 1.0f;
-    const Weigh weigh{R.mx, R.c * 128.0, val_of(best), s->limit, R.S, R.inf};
-    const auto weight = [&](uint32_t key) { return weigh.of(s->powers.of, key); };
+    const Weigh weigh{R.mx, R.c * 128.0, val_of(best), R.S, R.inf};
+    const auto weight = [&](uint32_t key) { return weigh.of(s->powers.of, val_of(key)); };
+    /* f(key as it is kept, its value, its id in this CTA) of a word of keys; what is masked, or lies around the row, has key 0
+     * and is not a number */
+    const auto word = [&](int i, auto f) {
+        const uint32_t w = words[i];
+        if (sizeof(K) == 2) {
+            uint32_t sign;                                        /* of both halves; the keys' map the other way round */
+            asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(sign) : "r"(w));
+            const uint32_t v = w ^ (~sign | 0x80008000u);
+            f((K)w, __uint_as_float(v << 16), 2 * i - lead);
+            f((K)(w >> 16), __uint_as_float(v & 0xffff0000u), 2 * i + 1 - lead);
+        } else f((K)w, val_of(w), i - lead);
+    };
+    /* of all, in any order; and of this thread's, by id: threads own neighbouring words, an odd number each (banks of their own) */
+    const auto each = [&](auto f) {
+#pragma unroll 2
+        for (int i = tid; i < kT * e; i += kT) word(i, f);
+    };
+    const auto own = [&](auto f) {
+#pragma unroll 2
+        for (int i = tid * e; i < tid * e + e; ++i) word(i, f);
+    };
+    /* the least kept form that is `key` or more: (a bf16 key stands for one of 2^16) */
+    const auto least_form = [&](uint32_t key) -> uint32_t {
+        if (sizeof(K) == 4) return key;
+        const uint32_t h = key >> 16;
+        return wide((K)h) >= key ? h : h + 1;
+    };
     /* the least key that min-p keeps: from the 32 next to where the bound falls (all keys, if it falls lower) */
     uint32_t least_key = 1;
     if (low > 0.0f) {
@@ -541,27 +547,26 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         if (least_key == max(min(guess, best), 32u) - 16) least_key = 1;          /* even the lowest looked at is kept: T without end */
         if (R.inf) least_key = best;
     }
-    /* the tokens that `pick` says, to the lists of the first `to` CTAs, in any order */
-    const auto gather = [&](int to, auto pick) {
+    /* the tokens whose keys are `from` or more and below `to`, to the lists of the first `copies` CTAs, in any order */
+    const auto gather = [&](int copies, uint32_t from, uint32_t to) {
+        const uint32_t low_form = max(least_form(from), 1u), range = least_form(to) - low_form;
         int n = 0, n_cta;
-#pragma unroll 1
-        for (int j = 0; j < e; ++j) { const uint32_t key = wide(own[j]); n += key && pick(key); }
+        each([&](K key, float, int) { n += key - low_form < range; });
         int at = scan(s->warp_n, n, &n_cta);
         if (tid == 0) {
-            uint32_t from;
-            asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(from) : "r"(peer_addr(&s->gathered, 0)), "r"(n_cta) : "memory");
-            s->from = (int)from;
+            uint32_t first;
+            asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(first) : "r"(peer_addr(&s->gathered, 0)), "r"(n_cta) : "memory");
+            s->from = (int)first;
         }
         __syncthreads();
         at += s->from;
-#pragma unroll 1
-        for (int j = 0; j < e && n; ++j) {
-            const uint32_t key = wide(own[j]);
-            if (!key || !pick(key)) continue;
-            if (at < kCap)
-                for (int r = 0; r < to; ++r) peer_put(peer_addr(&s->list[at], r), (u64)key << 32 | (0xffffffffu - (uint32_t)(own_id + j)));
-            ++at; --n;
-        }
+        if (n)
+            each([&](K key, float, int i) {
+                if (key - low_form >= range) return;
+                if (at < kCap)
+                    for (int r = 0; r < copies; ++r) peer_put(peer_addr(&s->list[at], r), (u64)wide(key) << 32 | (0xffffffffu - (uint32_t)(base + i)));
+                ++at;
+            });
     };
 
     /* ---- top-k of a few */
@@ -591,7 +596,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         if ((tid & 31) == 0) s->warp_n[tid >> 5] = (int)bound;
         __syncthreads();
         bound = __reduce_min_sync(0xffffffffu, (tid & 31) < kWarps ? (uint32_t)s->warp_n[tid & 31] : 0xffffffffu);
-        gather(1, [&](uint32_t key) { return key >= bound; });
+        gather(1, bound, best + 1);
         meet();
         const int n = (int)peer_get(peer_addr(&s->gathered, 0));
         meet();                                                   /* all have read it */
@@ -625,19 +630,15 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     if (by_k || by_p) {
         /* ---- histogram of the distance to the largest logit (key order and step order agree) */
         const float mx = val_of(best), inv = (float)((kBins - 1) / kRange * 1.4426950408889634) / t;
-        const auto bin_of = [&](uint32_t key) {
-            if (R.inf) return key == best ? 0 : kBins - 1;
-            const float d = __fsub_rn(mx, val_of(key)) * inv;
+        const auto bin_of = [&](float x) {
+            if (R.inf) return x == mx ? 0 : kBins - 1;
+            const float d = __fsub_rn(mx, x) * inv;
             return d < (float)(kBins - 1) ? (int)d : d >= (float)(kBins - 1) ? kBins - 1 : 0;     /* not a number: 0 * inf, every weight is 1 */
         };
         __syncthreads();
         for (int i = tid; i < kBins; i += kT) s->hist[i] = 0;
         __syncthreads();
-#pragma unroll 1
-        for (int j = 0; j < e; ++j) {
-            const uint32_t key = wide(own[j]);
-            if (key) atomicAdd(&s->hist[bin_of(key)], 1u);
-        }
+        each([&](K key, float x, int) { if (key) atomicAdd(&s->hist[bin_of(x)], 1u); });
         meet();
         /* each CTA sums its share of the steps, `size` threads a step, and tells all */
         const int seg = kBins / cl.size;
@@ -672,22 +673,41 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         const int k_step = s->pick;
         const auto count_to = [&](int b) { return b > 0 ? (int)s->upto[b - 1] : 0; };      /* tokens in steps below b */
 
-        /* the largest key c in the steps [from, to) such that above + the value of their keys >= c reaches `need`;
-         * *above moves on to what lies over c. The tokens are gathered and ranked, or the key is searched */
-        const auto key_at = [&](int from, int to, uint32_t least, u64 need, u64* above, bool ones) {
-            const auto inside = [&](uint32_t key) { if (key < least) return false; const int b = bin_of(key); return b >= from && b < to; };
-            const auto value = [&](uint32_t key) { return ones ? 1ull : weight(key); };
+        /* the least key in a step below b, by the warps' first and second, for two steps at once: a warp looks at 32 keys */
+        const auto edges = [&](int b0, int b1) {
+            __syncthreads();
+            if (tid < 64) {
+                const int b = tid < 32 ? b0 : b1;
+                uint32_t lo = 0x00800000u, hi = best + 1;         /* from the least number on; the largest logit is in step 0 */
+                if (b <= 0) lo = hi;
+                else if (b >= kBins) { lo = 1; hi = 1; }
+#pragma unroll 1
+                while (lo < hi) {
+                    const uint32_t step = (hi - lo + 31) / 32, at = lo + (tid & 31) * step;
+                    const uint32_t yes = __ballot_sync(0xffffffffu, at >= hi || bin_of(val_of(at)) < b);
+                    if (!yes) { lo += 31 * step + 1; continue; }
+                    const int first = __ffs(yes) - 1;             /* the lane before says no, this one yes */
+                    hi = min(hi, lo + first * step);
+                    if (first) lo += (first - 1) * step + 1;
+                }
+                if ((tid & 31) == 0) s->edge[tid >> 5] = lo;
+            }
+            __syncthreads();
+        };
+        /* the largest key c of the keys [low_key, high_key) such that above + the value of those >= c reaches `need`;
+         * *above moves on to what lies over c. The `many` tokens are gathered and ranked, or the key is searched */
+        const auto key_at = [&](uint32_t low_key, uint32_t high_key, int many, u64 need, u64* above, bool ones) {
+            const auto value = [&](float x) { return ones ? 1ull : weigh.of(s->powers.of, x); };
             /* ranking takes as many steps as the square of their number over the CTAs: a thousand on 4, 512 on one */
-            const int many = count_to(to) - count_to(from);
             if (many <= kCap && many * many <= cl.size << 18) {
                 if (first_cta && tid == 0) s->gathered = 0;
                 meet();
-                gather(cl.size, inside);
+                gather(cl.size, low_key, high_key);
                 if (tid == 0) s->mine.key = 0;
                 meet();
                 /* each CTA ranks its share of them */
                 const int n = (int)peer_get(peer_addr(&s->gathered, 0));
-                for (int i = tid; i < n; i += kT) s->weight[i] = value((uint32_t)(s->list[i] >> 32));
+                for (int i = tid; i < n; i += kT) s->weight[i] = value(val_of((uint32_t)(s->list[i] >> 32)));
                 __syncthreads();
                 const int here = (n + cl.size - 1) / cl.size, sh = share_of(here);
 #pragma unroll 1
@@ -705,28 +725,20 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
                 for (int r = 0; r < cl.size; ++r) if (parts[r].key) { found = (uint32_t)parts[r].key; *above = parts[r].w[0]; }
                 return found;
             }
-            /* the keys as they are kept, between those a step to either side of the window */
-            constexpr int kShift = sizeof(K) == 2 ? 16 : 0;
-            const float v_lo = mx - (float)(to + 1) / inv, v_hi = mx - (float)(from - 1) / inv;
-            uint32_t lo = least, hi = best;
-            if (to < kBins && v_lo > -3.0e38f) lo = max(lo, key_of(v_lo));
-            if (from > 1 && v_hi < 3.0e38f && v_hi < mx) hi = min(hi, key_of(v_hi));
-            lo >>= kShift; hi = (hi >> kShift) + 1;
+            uint32_t lo = max(least_form(low_key), 1u), hi = least_form(high_key);
             u64 over = 0;                                         /* of the keys from hi on */
 #pragma unroll 1
             while (hi - lo > 1) {
                 const uint32_t d = max(1u, (hi - lo) / 4);
                 const uint32_t c0 = min(lo + d, hi), c1 = min(lo + 2 * d, hi), c2 = min(lo + 3 * d, hi);
                 Sum3 v{};
-#pragma unroll 1
-                for (int j = 0; j < e; ++j) {
-                    const uint32_t whole = wide(own[j]), key = whole >> kShift;
-                    if (key < c0 || key >= hi || !inside(whole)) continue;
-                    const u64 x = value(whole);
-                    v.w[0] += x;
-                    if (key >= c1) v.w[1] += x;
-                    if (key >= c2) v.w[2] += x;
-                }
+                each([&](K key, float x, int) {
+                    if (key < c0 || key >= hi) return;
+                    const u64 w = value(x);
+                    v.w[0] += w;
+                    if (key >= c1) v.w[1] += w;
+                    if (key >= c2) v.w[2] += w;
+                });
                 v = cl.sum(v);
                 const u64 have = *above + over;
                 if (c2 < hi && have + v.w[2] >= need) lo = c2;
@@ -740,7 +752,8 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         u64 above;
         if (by_k) {
             above = (u64)count_to(k_step);
-            cut = key_at(k_step, k_step + 1, 1u, (u64)k, &above, true);
+            edges(k_step + 1, k_step);
+            cut = key_at(s->edge[0], s->edge[1], count_to(k_step + 1) - count_to(k_step), (u64)k, &above, true);
             ties = (int)((u64)k - above);
         }
         if (by_p) {
@@ -768,17 +781,19 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
             const u64 tied = by_k ? (u64)ties * weight(cut) : 0;
 #pragma unroll 1
             for (;;) {
+                edges(to, from);
+                const uint32_t low_key = s->edge[0], high_key = s->edge[1], low_form = least_form(low_key), high_form = least_form(high_key);
+                const uint32_t over_cut = by_k ? least_form(cut) + 1 : 1u;
                 Sum3 v{};                                         /* over the cut; of those, in steps below from, below to */
-#pragma unroll 2
-                for (int j = 0; j < e; ++j) {
-                    const uint32_t key = wide(own[j]);
-                    if (by_k ? key <= cut : !key) continue;
-                    const u64 x = weight(key);
-                    const int b = bin_of(key);
-                    v.w[0] += x;
-                    if (b < from) v.w[1] += x;
-                    if (b < to) v.w[2] += x;
-                }
+                each([&](K key, float x, int) {
+                    if (by_k && key < over_cut) return;
+                    const u64 w = weigh.of(s->powers.of, x);
+                    v.w[0] += w;
+                    if (key >= low_form) {
+                        v.w[2] += w;
+                        if (key >= high_form) v.w[1] += w;
+                    }
+                });
                 v = cl.sum(v);
                 const u64 want = want_of(p, v.w[0] + tied);
                 above = v.w[0];
@@ -789,7 +804,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
                 }
                 if (want > v.w[1] && want <= v.w[2]) {
                     above = v.w[1];
-                    cut = key_at(from, to, by_k ? cut + 1 : 1u, want, &above, false);
+                    cut = key_at(by_k ? max(cut + 1, low_key) : low_key, high_key, count_to(to) - count_to(from), want, &above, false);
                     const u64 one = weight(cut);
                     ties = one ? (int)min((u64)V, (want - above + one - 1) / one) : V;
                     break;
@@ -805,8 +820,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     int tie_rank = 0;
     if (ties < V) {
         int n = 0, n_cta;
-#pragma unroll 1
-        for (int j = 0; j < e; ++j) n += wide(own[j]) == cut;
+        own([&](K key, float, int) { n += key == (K)(sizeof(K) == 2 ? cut >> 16 : cut); });
         tie_rank = scan(s->warp_n, n, &n_cta);
         if (tid == 0) s->mine.w[0] = (u64)n_cta;
         const Part* parts = cl.exchange();
@@ -814,16 +828,16 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         for (int r = 0; r < cl.rank; ++r) tie_rank += (int)parts[r].w[0];
     }
     int rank = tie_rank;
-    const auto kept = [&](uint32_t key) { return key >= cut && (key > cut || rank++ < ties) && key >= least_key; };
+    /* the least kept, and what is more than the cut, in the form of the keys */
+    const uint32_t least = max(max(least_form(cut), least_form(least_key)), 1u), over = least_form(cut) + 1;
+    const auto kept = [&](K key) { return key >= least && (key >= over || rank++ < ties); };
     u64 w = 0, w_cta;
     int n = 0;
-#pragma unroll 2
-    for (int j = 0; j < e; ++j) {
-        const uint32_t key = wide(own[j]);
-        if (!kept(key)) continue;
-        w += weight(key);
+    own([&](K key, float x, int) {
+        if (!kept(key)) return;
+        w += weigh.of(s->powers.of, x);
         ++n;
-    }
+    });
     n = __reduce_add_sync(0xffffffffu, n);
     if ((tid & 31) == 0) s->warp_n[tid >> 5] = n;
     u64 before = scan(s->warp_w, w, &w_cta);                      /* its barriers order the counts, too */
@@ -842,21 +856,26 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     const u64 point = point_of(u, sum);
     if (before <= point && point < before + w) {
         rank = tie_rank;
+        bool found = false;
 #pragma unroll 1
-        for (int j = 0; j < e; ++j) {
-            const uint32_t key = wide(own[j]);
-            if (!kept(key)) continue;
-            before += weight(key);
-            if (before <= point) continue;
-            answer(P, m, own_id + j, n_kept, logprob_of(R, key, sum));
-            break;
-        }
+        for (int i = tid * e; i < tid * e + e && !found; ++i)
+            word(i, [&](K key, float x, int id) {
+                if (found || !kept(key)) return;
+                before += weigh.of(s->powers.of, x);
+                if (before <= point) return;
+                answer(P, m, base + id, n_kept, logprob_of(R, wide(key), sum));
+                found = true;
+            });
     }
 }
 
 constexpr size_t kRowSmem = 220 * 1024;
-int each_of(int vocab, int size) { return ((vocab + kT * size - 1) / (kT * size)) | 1; }
-size_t row_smem(int vocab, int size, int ksz) { return sizeof(Shared) + 16 + (size_t)kT * each_of(vocab, size) * ksz; }
+/* words of keys a thread: an odd number, and 16 bytes for the shift to the logits' grid */
+int words_of(int vocab, int size, int ksz) {
+    const int bytes = (vocab + size - 1) / size * ksz + 16;
+    return (bytes + kT * 4 - 1) / (kT * 4) | 1;
+}
+size_t row_smem(int vocab, int size, int ksz) { return sizeof(Shared) + (size_t)kT * 4 * words_of(vocab, size, ksz); }
 
 template <typename K>
 int launch_row(const R3dNucleus& P, int size, cudaStream_t st) {
@@ -869,7 +888,7 @@ int launch_row(const R3dNucleus& P, int size, cudaStream_t st) {
             cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return RAD_E_DEVICE;
         set[dev].store(true, std::memory_order_relaxed);
     }
-    const int e = each_of(P.n_vocab, size);
+    const int e = words_of(P.n_vocab, size, (int)sizeof(K));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)P.rows * (unsigned)size); cfg.blockDim = dim3(kT); cfg.stream = st;
     cfg.dynamicSmemBytes = row_smem(P.n_vocab, size, (int)sizeof(K));
@@ -893,8 +912,8 @@ int launch_nucleus(const R3dNucleus& p, cudaStream_t st) {
      * takes 27 / 20 / 16 us on 4 / 8 / 16 CTAs; 64 rows 59 / 56 / 83, 256 rows with filters of their own 521 / 519 on
      * 4 / 8; 30 rows of 20000 52 / 16 / 18 us on 2 / 4 / 8) */
     int size = 1;
-    while (size < kMaxCluster && (row_smem(p.n_vocab, size, ksz) > kRowSmem || each_of(p.n_vocab, size) > 39 ||
-                                  ((long long)p.rows * size < 100 && each_of(p.n_vocab, size) > 9))) size *= 2;
+    const auto each = [&]() { return words_of(p.n_vocab, size, ksz) * (4 / ksz); };
+    while (size < kMaxCluster && (row_smem(p.n_vocab, size, ksz) > kRowSmem || each() > 39 || ((long long)p.rows * size < 100 && each() > 9))) size *= 2;
     if (row_smem(p.n_vocab, size, ksz) > kRowSmem) {
         k_nucleus_long<<<(unsigned)p.rows, 1024, 0, st>>>(P);
         return cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
