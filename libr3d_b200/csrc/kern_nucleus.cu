@@ -249,6 +249,7 @@ struct Shared {
     Part mine;
     double c, floor_y, drop;                                      /* log2(e) / T; min-p as an exponent, and in logits */
     Powers powers;
+    Weigh weigh;
     u64 warp_w[kWarps];
     int warp_n[kWarps];
     Sum3 sums[kWarps];
@@ -260,6 +261,12 @@ struct Shared {
     union { uint32_t tops[kGroups]; uint32_t hist[kBins]; };   /* the groups' largest keys; this CTA's histogram */
     uint32_t upto[kBins];                                         /* the cluster's, summed up to each step */
 };
+
+/* the kernel's shared memory: its state, then the keys. The calls name it themselves: a pointer handed on would be read as
+ * one to any memory */
+extern __shared__ __align__(16) uint8_t raw[];
+__device__ __forceinline__ Shared* shared() { return (Shared*)raw; }
+__device__ __forceinline__ const uint32_t* key_words() { return (const uint32_t*)(raw + sizeof(Shared)); }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ uint32_t peer_addr(const void* p, int rank) {
@@ -289,17 +296,17 @@ static_assert(offsetof(Shared, sel) % 16 == 0 && sizeof(Shared) % 16 == 0, "read
 static_assert(offsetof(Shared, parts) % 8 == 0 && offsetof(Shared, mine) % 8 == 0 && sizeof(Part) % 8 == 0, "sent by 8 bytes");
 /* the cluster, the same in every thread of it */
 struct Cluster {
-    Shared* s;
     int size, rank, turn;
 
     /* every CTA's `mine` to every CTA, and with it what the threads put before; parts are valid until the turn after next */
     __device__ __forceinline__ const Part* exchange() {
-        const Part* p = s->parts[turn];
-        send(s, size, rank, turn);
+        const Part* p = shared()->parts[turn];
+        send(size, rank, turn);
         turn ^= 1;
         return p;
     }
-    __device__ static __noinline__ void send(Shared* s, int size, int rank, int turn) {
+    __device__ static __noinline__ void send(int size, int rank, int turn) {
+        Shared* const s = shared();
         __syncthreads();
         constexpr int kWords = sizeof(Part) / 8;
         for (int i = threadIdx.x; i < size * kWords; i += kT)
@@ -308,14 +315,15 @@ struct Cluster {
     }
     /* sums over the cluster */
     __device__ __forceinline__ Sum3 sum(Sum3 v) {
-        block_sums(s, v.w[0], v.w[1], v.w[2]);
+        block_sums(v.w[0], v.w[1], v.w[2]);
         const Part* p = exchange();
         Sum3 all{};
 #pragma unroll 1
         for (int r = 0; r < size; ++r) { all.w[0] += p[r].w[0]; all.w[1] += p[r].w[1]; all.w[2] += p[r].w[2]; }
         return all;
     }
-    __device__ static __noinline__ void block_sums(Shared* s, u64 a, u64 b, u64 c) {
+    __device__ static __noinline__ void block_sums(u64 a, u64 b, u64 c) {
+        Shared* const s = shared();
         a = warp_sum(a); b = warp_sum(b); c = warp_sum(c);
         if ((threadIdx.x & 31) == 0) s->sums[threadIdx.x >> 5] = Sum3{{a, b, c}};
         __syncthreads();
@@ -329,7 +337,8 @@ struct Cluster {
 
 /* exclusive over the block's threads, in their order; *total over all of them */
 template <typename V>
-__device__ __noinline__ V scan(V* warps, V v, V* total) {
+__device__ __noinline__ V scan(V v, V* total) {
+    V* const warps = sizeof(V) == 8 ? (V*)shared()->warp_w : (V*)shared()->warp_n;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     V x = v;
 #pragma unroll 1
@@ -348,7 +357,9 @@ __device__ __noinline__ V scan(V* warps, V v, V* total) {
 /* For the i-th of n gathered tokens (i = the thread's place among groups of kT / n2 threads): how many stand before it
  * in the order, the sum of their values, and of those with a larger key. */
 struct Before { int n; u64 all, larger; };
-__device__ __noinline__ Before before_of(const u64* list, const u64* weight, int n, int i, int share) {
+__device__ __noinline__ Before before_of(int n, int i, int share) {
+    const u64* const list = shared()->list;
+    const u64* const weight = shared()->weight;
     const u64 a = i < n ? list[i] : ~0ull;
     Before r{0, 0, 0};
 #pragma unroll 4
@@ -378,6 +389,63 @@ template <typename K> __device__ __forceinline__ uint32_t wide(K k);
 template <> __device__ __forceinline__ uint32_t wide<uint32_t>(uint32_t k) { return k; }
 template <> __device__ __forceinline__ uint32_t wide<uint16_t>(uint16_t k) { return k & 0x8000u ? (uint32_t)k << 16 : k ? (uint32_t)k << 16 | 0xffffu : 0u; }
 
+/* f(key as it is kept, its value, its id in the CTA) of a word of keys; what is masked, or lies around the row, has key 0
+ * and is not a number */
+template <typename K, typename F>
+__device__ __forceinline__ void word_of(const uint32_t* words, int lead, int i, F f) {
+    const uint32_t w = words[i];
+    if (sizeof(K) == 2) {
+        uint32_t sign;                                            /* of both halves; the keys' map the other way round */
+        asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(sign) : "r"(w));
+        const uint32_t v = w ^ (~sign | 0x80008000u);
+        f((K)w, __uint_as_float(v << 16), 2 * i - lead);
+        f((K)(w >> 16), __uint_as_float(v & 0xffff0000u), 2 * i + 1 - lead);
+    } else f((K)w, val_of(w), i - lead);
+}
+template <typename K, typename F>
+__device__ __forceinline__ void each_of(const uint32_t* words, int lead, int e, F f) {
+    constexpr int kUnroll = sizeof(K) == 2 ? 2 : 4;
+#pragma unroll kUnroll
+    for (int i = threadIdx.x; i < kT * e; i += kT) word_of<K>(words, lead, i, f);
+}
+/* a thread's own words, by id: neighbouring ones, an odd number (banks of their own) */
+template <typename K, typename F>
+__device__ __forceinline__ void own_of(const uint32_t* words, int lead, int e, F f) {
+    constexpr int kUnroll = sizeof(K) == 2 ? 2 : 4;
+    const uint32_t* const mine = words + threadIdx.x * e;
+#pragma unroll kUnroll
+    for (int i = 0; i < e; ++i) word_of<K>(mine, lead, i, f);
+}
+/* The passes that weigh many are calls, for registers of their own: inside the kernel they took twice the time.
+ * Over this thread's words: the weights of the keys from `over` on (0: of all), of those from `high` and from `low` on. */
+template <typename K>
+__device__ __noinline__ Sum3 weigh_all(int e, uint32_t over, uint32_t high, uint32_t low) {
+    const Weigh weigh = shared()->weigh;
+    Sum3 v{};
+    each_of<K>(key_words(), 0, e, [&](K key, float x, int) {
+        if (key < over) return;
+        const u64 w = weigh.of(shared()->powers.of, x);
+        v.w[0] += w;
+        if (key >= low) {
+            v.w[2] += w;
+            if (key >= high) v.w[1] += w;
+        }
+    });
+    return v;
+}
+/* Of this thread's own words: how many keys are kept, and their weight. `rank`: of its first key `over` - 1 among those. */
+template <typename K>
+__device__ __noinline__ Sum weigh_kept(int e, uint32_t least, uint32_t over, int rank, int ties) {
+    const Weigh weigh = shared()->weigh;
+    Sum v{0, 0};
+    own_of<K>(key_words(), 0, e, [&](K key, float x, int) {
+        if (key < least || (key < over && rank++ >= ties)) return;
+        ++v.n;
+        v.w += weigh.of(shared()->powers.of, x);
+    });
+    return v;
+}
+
 /* key_of by the integer pipe alone: +0 folds -0; the keys of what is not masked lie next to each other */
 __device__ __forceinline__ uint32_t key_fast(uint32_t bits) {
     const int v = __float_as_int(__uint_as_float(bits) + 0.0f);
@@ -387,20 +455,19 @@ __device__ __forceinline__ uint32_t key_fast(uint32_t bits) {
 
 template <typename K>
 __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const int e) {
-    extern __shared__ __align__(16) uint8_t raw[];
-    Shared* const s = (Shared*)raw;
+    Shared* const s = shared();
     constexpr int kEach = 16 / (int)sizeof(K), kPer = 4 / (int)sizeof(K);     /* values of 16 bytes and of four, as logits and as keys */
     Cluster cl;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cl.size));
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cl.rank));
-    cl.s = s; cl.turn = 0;
+    cl.turn = 0;
     const int64_t m = blockIdx.x / cl.size;
     const int V = P.n_vocab, span = kT * e * kPer - kEach, base = cl.rank * span, tid = threadIdx.x;      /* this CTA's ids */
     /* the keys lie to the 16-byte grid as the logits do, which takes up to 16 bytes more than the ids' own */
     const K* const x = (const K*)P.logits + m * P.x_pitch + base;
     const int lead = (int)((uintptr_t)x & 15) / (int)sizeof(K);
     K* const keys = (K*)(raw + sizeof(Shared)) + lead;
-    const uint32_t* const words = (const uint32_t*)(raw + sizeof(Shared));
+    const uint32_t* const words = key_words();
     /* the peers' shared memory may be written once they have all begun: waited for below */
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
@@ -507,29 +574,11 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     Row R;
     R.c = s->c; R.mx = (double)val_of(best); R.inf = isinf(val_of(best)); R.S = P.shift;
     const bool by_k = k < live, by_p = p < 1.0f;
-    const Weigh weigh{R.mx, R.c * 128.0, val_of(best), R.S, R.inf};
-    const auto weight = [&](uint32_t key) { return weigh.of(s->powers.of, val_of(key)); };
-    /* f(key as it is kept, its value, its id in this CTA) of a word of keys; what is masked, or lies around the row, has key 0
-     * and is not a number */
-    const auto word = [&](int i, auto f) {
-        const uint32_t w = words[i];
-        if (sizeof(K) == 2) {
-            uint32_t sign;                                        /* of both halves; the keys' map the other way round */
-            asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(sign) : "r"(w));
-            const uint32_t v = w ^ (~sign | 0x80008000u);
-            f((K)w, __uint_as_float(v << 16), 2 * i - lead);
-            f((K)(w >> 16), __uint_as_float(v & 0xffff0000u), 2 * i + 1 - lead);
-        } else f((K)w, val_of(w), i - lead);
-    };
-    /* of all, in any order; and of this thread's, by id: threads own neighbouring words, an odd number each (banks of their own) */
-    const auto each = [&](auto f) {
-#pragma unroll 2
-        for (int i = tid; i < kT * e; i += kT) word(i, f);
-    };
-    const auto own = [&](auto f) {
-#pragma unroll 2
-        for (int i = tid * e; i < tid * e + e; ++i) word(i, f);
-    };
+    if (tid == 0) s->weigh = Weigh{R.mx, R.c * 128.0, val_of(best), R.S, R.inf};
+    __syncthreads();
+    const auto weight = [&](uint32_t key) { return s->weigh.of(s->powers.of, val_of(key)); };
+    const auto word = [&](int i, auto f) { word_of<K>(words, lead, i, f); };
+    const auto each = [&](auto f) { each_of<K>(words, lead, e, f); };     /* of all, in any order */
     /* the least kept form that is `key` or more: (a bf16 key stands for one of 2^16) */
     const auto least_form = [&](uint32_t key) -> uint32_t {
         if (sizeof(K) == 4) return key;
@@ -552,7 +601,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         const uint32_t low_form = max(least_form(from), 1u), range = least_form(to) - low_form;
         int n = 0, n_cta;
         each([&](K key, float, int) { n += key - low_form < range; });
-        int at = scan(s->warp_n, n, &n_cta);
+        int at = scan(n, &n_cta);
         if (tid == 0) {
             uint32_t first;
             asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(first) : "r"(peer_addr(&s->gathered, 0)), "r"(n_cta) : "memory");
@@ -606,19 +655,19 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
             __syncthreads();
             const int sh = share_of(n), i = tid / sh;
             const bool mine_too = i < n && tid % sh == 0;         /* one thread speaks for a token */
-            const Before b = before_of(s->list, s->weight, n, i, sh);
+            const Before b = before_of(n, i, sh);
             const u64 me = i < n ? s->list[i] : 0, w = i < n ? s->weight[i] : 0;
             const uint32_t key = (uint32_t)(me >> 32);
             u64 sum;
-            scan(s->warp_w, mine_too && b.n < k ? w : 0ull, &sum);
+            scan(mine_too && b.n < k ? w : 0ull, &sum);
             const u64 want = by_p ? want_of(p, sum) : ~0ull;
             const bool keep = mine_too && b.n < k && (b.n == 0 || (b.all < want && key >= least_key));
-            scan(s->warp_w, keep ? w : 0ull, &sum);
+            scan(keep ? w : 0ull, &sum);
             const int n_kept = __syncthreads_count(keep);
             /* by id, ascending: the low words are 0xffffffff - id, and what is not kept weighs nothing */
             if (mine_too) { s->list[i] = me << 32 | key; s->weight[i] = keep ? w : 0; }
             __syncthreads();
-            const u64 before = before_of(s->list, s->weight, n, i, sh).all, point = point_of(u, sum);
+            const u64 before = before_of(n, i, sh).all, point = point_of(u, sum);
             if (keep && before <= point && point < before + w)
                 answer(P, m, (int)(0xffffffffu - (uint32_t)me), n_kept, logprob_of(R, key, sum));
             return;
@@ -661,7 +710,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
             n_own += cnt[j]; est_own += est[j];
         }
         int dummy;
-        int upto = scan(s->warp_n, (int)n_own, &dummy);
+        int upto = scan((int)n_own, &dummy);
 #pragma unroll
         for (int j = 0; j < kBinsEach; ++j) {
             const int before = upto;
@@ -697,7 +746,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         /* the largest key c of the keys [low_key, high_key) such that above + the value of those >= c reaches `need`;
          * *above moves on to what lies over c. The `many` tokens are gathered and ranked, or the key is searched */
         const auto key_at = [&](uint32_t low_key, uint32_t high_key, int many, u64 need, u64* above, bool ones) {
-            const auto value = [&](float x) { return ones ? 1ull : weigh.of(s->powers.of, x); };
+            const auto value = [&](float x) { return ones ? 1ull : s->weigh.of(s->powers.of, x); };
             /* ranking takes as many steps as the square of their number over the CTAs: a thousand on 4, 512 on one */
             if (many <= kCap && many * many <= cl.size << 18) {
                 if (first_cta && tid == 0) s->gathered = 0;
@@ -713,7 +762,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
 #pragma unroll 1
                 for (int j = tid / sh; j - tid / sh < here; j += kT / sh) {
                     const int i = j < here ? cl.rank * here + j : n;
-                    const Before b = before_of(s->list, s->weight, n, i, sh);
+                    const Before b = before_of(n, i, sh);
                     if (i < n && tid % sh == 0 && *above + b.all < need && *above + b.all + s->weight[i] >= need) {
                         s->mine.key = s->list[i] >> 32;
                         s->mine.w[0] = *above + b.larger;
@@ -759,12 +808,12 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         if (by_p) {
             /* the window: where p of the middle weights ends, and up to two steps to either side if they hold few */
             float all;
-            float run = scan((float*)s->warp_n, est_own, &all);
+            float run = scan(est_own, &all);
             if (by_k) {                                           /* of the first k tokens */
                 float part = 0.0f;
 #pragma unroll
                 for (int j = 0; j < kBinsEach; ++j) if (kBinsEach * tid + j <= k_step) part += est[j];
-                scan((float*)s->warp_n, part, &all);
+                scan(part, &all);
             }
             if (tid == 0) s->pick = by_k ? k_step : kBins - 1;
             __syncthreads();
@@ -782,18 +831,9 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
 #pragma unroll 1
             for (;;) {
                 edges(to, from);
-                const uint32_t low_key = s->edge[0], high_key = s->edge[1], low_form = least_form(low_key), high_form = least_form(high_key);
-                const uint32_t over_cut = by_k ? least_form(cut) + 1 : 1u;
-                Sum3 v{};                                         /* over the cut; of those, in steps below from, below to */
-                each([&](K key, float x, int) {
-                    if (by_k && key < over_cut) return;
-                    const u64 w = weigh.of(s->powers.of, x);
-                    v.w[0] += w;
-                    if (key >= low_form) {
-                        v.w[2] += w;
-                        if (key >= high_form) v.w[1] += w;
-                    }
-                });
+                const uint32_t low_key = s->edge[0], high_key = s->edge[1];
+                /* over the cut; of those, in steps below from, below to */
+                Sum3 v = weigh_all<K>(e, by_k ? least_form(cut) + 1 : 0u, least_form(high_key), least_form(low_key));
                 v = cl.sum(v);
                 const u64 want = want_of(p, v.w[0] + tied);
                 above = v.w[0];
@@ -820,27 +860,22 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     int tie_rank = 0;
     if (ties < V) {
         int n = 0, n_cta;
-        own([&](K key, float, int) { n += key == (K)(sizeof(K) == 2 ? cut >> 16 : cut); });
-        tie_rank = scan(s->warp_n, n, &n_cta);
+        own_of<K>(words, lead, e, [&](K key, float, int) { n += key == (K)(sizeof(K) == 2 ? cut >> 16 : cut); });
+        tie_rank = scan(n, &n_cta);
         if (tid == 0) s->mine.w[0] = (u64)n_cta;
         const Part* parts = cl.exchange();
 #pragma unroll 1
         for (int r = 0; r < cl.rank; ++r) tie_rank += (int)parts[r].w[0];
     }
-    int rank = tie_rank;
     /* the least kept, and what is more than the cut, in the form of the keys */
     const uint32_t least = max(max(least_form(cut), least_form(least_key)), 1u), over = least_form(cut) + 1;
-    const auto kept = [&](K key) { return key >= least && (key >= over || rank++ < ties); };
-    u64 w = 0, w_cta;
-    int n = 0;
-    own([&](K key, float x, int) {
-        if (!kept(key)) return;
-        w += weigh.of(s->powers.of, x);
-        ++n;
-    });
+    const Sum mine = weigh_kept<K>(e, least, over, tie_rank, ties);
+    const u64 w = mine.w;
+    u64 w_cta;
+    int n = mine.n;
     n = __reduce_add_sync(0xffffffffu, n);
     if ((tid & 31) == 0) s->warp_n[tid >> 5] = n;
-    u64 before = scan(s->warp_w, w, &w_cta);                      /* its barriers order the counts, too */
+    u64 before = scan(w, &w_cta);                      /* its barriers order the counts, too */
     if (tid < 32) {
         n = __reduce_add_sync(0xffffffffu, tid < kWarps ? s->warp_n[tid] : 0);
         if (tid == 0) { s->mine.w[0] = w_cta; s->mine.w[1] = (u64)n; }
@@ -855,13 +890,13 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     }
     const u64 point = point_of(u, sum);
     if (before <= point && point < before + w) {
-        rank = tie_rank;
+        int rank = tie_rank;
         bool found = false;
 #pragma unroll 1
         for (int i = tid * e; i < tid * e + e && !found; ++i)
             word(i, [&](K key, float x, int id) {
-                if (found || !kept(key)) return;
-                before += weigh.of(s->powers.of, x);
+                if (found || key < least || (key < over && rank++ >= ties)) return;
+                before += s->weigh.of(s->powers.of, x);
                 if (before <= point) return;
                 answer(P, m, base + id, n_kept, logprob_of(R, wide(key), sum));
                 found = true;
