@@ -254,7 +254,6 @@ struct Shared {
     int warp_n[kWarps];
     Sum3 sums[kWarps];
     uint32_t my_tops[kT];
-    alignas(16) uint32_t sel[kT];                                 /* read by 16 bytes */
     int gathered, pick, from;
     uint32_t edge[2];
     u64 list[kCap], weight[kCap];                                 /* gathered tokens, key << 32 | ~id; their values */
@@ -292,7 +291,7 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
     return v;
 }
 
-static_assert(offsetof(Shared, sel) % 16 == 0 && sizeof(Shared) % 16 == 0, "read by 16 bytes");
+static_assert(sizeof(Shared) % 16 == 0, "the keys behind it are written by 16 bytes");
 static_assert(offsetof(Shared, parts) % 8 == 0 && offsetof(Shared, mine) % 8 == 0 && sizeof(Part) % 8 == 0, "sent by 8 bytes");
 /* the cluster, the same in every thread of it */
 struct Cluster {
@@ -354,27 +353,27 @@ __device__ __noinline__ V scan(V v, V* total) {
     return (warp ? before : (V)0) + x - v;
 }
 
-/* For the i-th of n gathered tokens (i = the thread's place among groups of kT / n2 threads): how many stand before it
- * in the order, the sum of their values, and of those with a larger key. */
-struct Before { int n; u64 all, larger; };
-__device__ __noinline__ Before before_of(int n, int i, int share) {
+/* For the i-th of n gathered tokens (i = the thread's place among groups of `share` threads): how many stand before it in
+ * the order, and the sum of their values. */
+__device__ __noinline__ int count_before(int n, int i, int share) {
+    const u64* const list = shared()->list;
+    const u64 a = i < n ? list[i] : ~0ull;
+    int r = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x % share; j < n; j += share) r += list[j] > a;
+#pragma unroll 1
+    for (int o = 1; o < share; o <<= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+    return r;
+}
+__device__ __noinline__ u64 sum_before(int n, int i, int share) {
     const u64* const list = shared()->list;
     const u64* const weight = shared()->weight;
     const u64 a = i < n ? list[i] : ~0ull;
-    Before r{0, 0, 0};
+    u64 r = 0;
 #pragma unroll 4
-    for (int j = threadIdx.x % share; j < n; j += share) {
-        const u64 o = list[j], v = o > a ? weight[j] : 0;
-        r.n += o > a;
-        r.all += v;
-        r.larger += (uint32_t)(o >> 32) > (uint32_t)(a >> 32) ? v : 0;
-    }
+    for (int j = threadIdx.x % share; j < n; j += share) r += list[j] > a ? weight[j] : 0;
 #pragma unroll 1
-    for (int o = 1; o < share; o <<= 1) {
-        r.n += __shfl_xor_sync(0xffffffffu, r.n, o);
-        r.all += __shfl_xor_sync(0xffffffffu, r.all, o);
-        r.larger += __shfl_xor_sync(0xffffffffu, r.larger, o);
-    }
+    for (int o = 1; o < share; o <<= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
     return r;
 }
 /* threads for each of n tokens, a power of two up to a warp */
@@ -622,54 +621,51 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     int sel = 128;                                                /* groups to rank: at least twice k, which lets through 1.4 k tokens */
     while (sel < 2 * k && sel <= kT) sel *= 2;
     if (by_k && sel <= kT) {
-        /* the k-th largest of the groups' keys, neighbours taken together down to `sel` groups */
-        const int of = mine_groups * cl.size / sel, share = min(kT / sel, 32);     /* threads a group */
-        if (tid < sel) {
-            uint32_t g = 0;
+        /* a bound that k groups reach, and at most an eighth more: neighbours are taken together down to `sel` groups, one a
+         * thread, and every step of the search is one barrier that counts */
+        const int of = mine_groups * cl.size / sel;
+        uint32_t g = 0;
+        if (tid < sel)
 #pragma unroll 1
             for (int j = 0; j < of; ++j) g = max(g, s->tops[tid * of + j]);
-            s->sel[tid] = g;
-        }
-        __syncthreads();
-        const uint32_t mine = tid / share < sel ? s->sel[tid / share] : 0u;
-        int larger = 0;
-#pragma unroll 1
-        for (int j = tid % share * 4; j < sel; j += share * 4) {
-            const uint4 o = *(const uint4*)&s->sel[j];
-            larger += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
-        }
-#pragma unroll 1
-        for (int o = 1; o < share; o <<= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
-        /* fewer than k groups lie above it: the least such key is the k-th largest */
-        uint32_t bound = __reduce_min_sync(0xffffffffu, larger < k && tid / share < sel ? mine : 0xffffffffu);
+        uint32_t bound = __reduce_min_sync(0xffffffffu, tid < sel ? g : best);      /* the least group: all reach it */
         if ((tid & 31) == 0) s->warp_n[tid >> 5] = (int)bound;
         __syncthreads();
-        bound = __reduce_min_sync(0xffffffffu, (tid & 31) < kWarps ? (uint32_t)s->warp_n[tid & 31] : 0xffffffffu);
+        bound = __reduce_min_sync(0xffffffffu, (tid & 31) < kWarps ? (uint32_t)s->warp_n[tid & 31] : best);
+        uint32_t past = best + 1;
+        for (int have = sel; have > k + k / 8 && past - bound > 1;) {
+            const uint32_t mid = bound + (past - bound) / 2;
+            const int n = __syncthreads_count(g >= mid);
+            if (n >= k) { bound = mid; have = n; } else past = mid;
+        }
         gather(1, bound, best + 1);
         meet();
         const int n = (int)peer_get(peer_addr(&s->gathered, 0));
         meet();                                                   /* all have read it */
         if (bound && n <= kT) {                                   /* a thread for each */
             if (!first_cta) return;
-            for (int i = tid; i < n; i += kT) s->weight[i] = weight((uint32_t)(s->list[i] >> 32));
+            /* in order, a thread each; what is kept is a first part */
+            int sh = share_of(n), i = tid / sh;
+            const int place = count_before(n, i, sh);
+            if (i < n && tid % sh == 0) s->list[kT + place] = s->list[i];
             __syncthreads();
-            const int sh = share_of(n), i = tid / sh;
-            const bool mine_too = i < n && tid % sh == 0;         /* one thread speaks for a token */
-            const Before b = before_of(n, i, sh);
-            const u64 me = i < n ? s->list[i] : 0, w = i < n ? s->weight[i] : 0;
-            const uint32_t key = (uint32_t)(me >> 32);
-            u64 sum;
-            scan(mine_too && b.n < k ? w : 0ull, &sum);
-            const u64 want = by_p ? want_of(p, sum) : ~0ull;
-            const bool keep = mine_too && b.n < k && (b.n == 0 || (b.all < want && key >= least_key));
-            scan(keep ? w : 0ull, &sum);
+            const u64 me = s->list[kT + tid];
+            uint32_t key = (uint32_t)(me >> 32);
+            const bool in = tid < min(n, k);
+            u64 w = in ? weight(key) : 0, sum;
+            const u64 before = scan(w, &sum), want = by_p ? want_of(p, sum) : ~0ull;
+            const bool keep = in && (tid == 0 || (before < want && key >= least_key));
+            /* by id, ascending: the low words are 0xffffffff - id */
+            s->list[tid] = me << 32 | key;
+            s->weight[tid] = w;
             const int n_kept = __syncthreads_count(keep);
-            /* by id, ascending: the low words are 0xffffffff - id, and what is not kept weighs nothing */
-            if (mine_too) { s->list[i] = me << 32 | key; s->weight[i] = keep ? w : 0; }
-            __syncthreads();
-            const u64 before = before_of(n, i, sh).all, point = point_of(u, sum);
-            if (keep && before <= point && point < before + w)
-                answer(P, m, (int)(0xffffffffu - (uint32_t)me), n_kept, logprob_of(R, key, sum));
+            scan(keep ? w : 0ull, &sum);
+            sh = share_of(n_kept); i = tid / sh;
+            const u64 run = sum_before(n_kept, i, sh), point = point_of(u, sum);
+            if (i < n_kept && tid % sh == 0 && run <= point && point < run + s->weight[i]) {
+                key = (uint32_t)s->list[i];
+                answer(P, m, (int)(0xffffffffu - (uint32_t)(s->list[i] >> 32)), n_kept, logprob_of(R, key, sum));
+            }
             return;
         }
     }
@@ -762,16 +758,17 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
 #pragma unroll 1
                 for (int j = tid / sh; j - tid / sh < here; j += kT / sh) {
                     const int i = j < here ? cl.rank * here + j : n;
-                    const Before b = before_of(n, i, sh);
-                    if (i < n && tid % sh == 0 && *above + b.all < need && *above + b.all + s->weight[i] >= need) {
-                        s->mine.key = s->list[i] >> 32;
-                        s->mine.w[0] = *above + b.larger;
-                    }
+                    const u64 run = *above + sum_before(n, i, sh);
+                    if (i < n && tid % sh == 0 && run < need && run + s->weight[i] >= need) s->mine.key = s->list[i] >> 32;
                 }
                 const Part* parts = cl.exchange();
                 uint32_t found = 0;
 #pragma unroll 1
-                for (int r = 0; r < cl.size; ++r) if (parts[r].key) { found = (uint32_t)parts[r].key; *above = parts[r].w[0]; }
+                for (int r = 0; r < cl.size; ++r) found = max(found, (uint32_t)parts[r].key);
+                u64 larger = 0, all;
+                for (int i = tid; i < n; i += kT) larger += (uint32_t)(s->list[i] >> 32) > found ? s->weight[i] : 0;
+                scan(larger, &all);
+                *above += all;
                 return found;
             }
             uint32_t lo = max(least_form(low_key), 1u), hi = least_form(high_key);
