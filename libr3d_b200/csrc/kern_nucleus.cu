@@ -452,15 +452,37 @@ __device__ __forceinline__ uint32_t key_fast(uint32_t bits) {
     return k - 0x00800000u <= 0xff000000u ? k : 0u;               /* from the least number to +inf */
 }
 
+/* The row of the q-th cluster, those that need every token's weight (top-p without a small top-k) first: they take three
+ * times as long, and begun in the last wave they end it alone. At most kT rows. */
+constexpr int kSmallK = 256;
+__device__ __forceinline__ int long_rows_first(const R3dNucleus& P, int q) {
+    Shared* const s = shared();
+    const int i = threadIdx.x, lane = i & 31;
+    bool heavy = false;
+    if (i < P.rows) {
+        const float p = P.top_p[i * P.p_pitch];
+        const int k = P.top_k ? P.top_k[i * P.k_pitch] : 0;
+        heavy = p < 1.0f && p > 0.0f && (k <= 0 || k > kSmallK) && !(P.temperature && P.temperature[i * P.t_pitch] <= 0.0f);
+    }
+    const uint32_t in_warp = __ballot_sync(0xffffffffu, heavy);
+    if (lane == 0) s->warp_n[i >> 5] = __popc(in_warp);
+    const int all = __syncthreads_count(heavy);
+    int before = __popc(in_warp & ((1u << lane) - 1u));
+    for (int w = 0; w < i >> 5; ++w) before += s->warp_n[w];
+    if (i < P.rows && (heavy ? before : all + i - before) == q) s->pick = i;
+    __syncthreads();
+    return s->pick;
+}
+
 template <typename K>
-__global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const int e) {
+__global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const int e, const int waves) {
     Shared* const s = shared();
     constexpr int kEach = 16 / (int)sizeof(K), kPer = 4 / (int)sizeof(K);     /* values of 16 bytes and of four, as logits and as keys */
     Cluster cl;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cl.size));
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cl.rank));
     cl.turn = 0;
-    const int64_t m = blockIdx.x / cl.size;
+    const int64_t m = waves ? long_rows_first(P, blockIdx.x / cl.size) : blockIdx.x / cl.size;
     const int V = P.n_vocab, span = kT * e * kPer - kEach, base = cl.rank * span, tid = threadIdx.x;      /* this CTA's ids */
     /* the keys lie to the 16-byte grid as the logits do, which takes up to 16 bytes more than the ids' own */
     const K* const x = (const K*)P.logits + m * P.x_pitch + base;
@@ -620,6 +642,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     /* ---- top-k of a few */
     int sel = 128;                                                /* groups to rank: at least twice k, which lets through 1.4 k tokens */
     while (sel < 2 * k && sel <= kT) sel *= 2;
+    static_assert(2 * kSmallK == kT, "what `sel` lets through");
     if (by_k && sel <= kT) {
         /* a bound that k groups reach, and at most an eighth more: neighbours are taken together down to `sel` groups, one a
          * thread, and every step of the search is one barrier that counts */
@@ -928,7 +951,10 @@ int launch_row(const R3dNucleus& P, int size, cudaStream_t st) {
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = (unsigned)size; at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, P, e) == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
+    int sms = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return RAD_E_DEVICE;
+    const int waves = P.top_p && P.rows <= kT && (long long)P.rows * size > 2 * sms;
+    return cudaLaunchKernelEx(&cfg, kernel, P, e, waves) == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
 }
 
 } /* namespace */
@@ -940,12 +966,15 @@ int launch_nucleus(const R3dNucleus& p, cudaStream_t st) {
     P.shift = 62 - bits < 50 ? 62 - bits : 50;
     count_launch();
     const int ksz = p.x_dtype == RAD_F32 ? 4 : 2;
-    /* CTAs a row: no more than 39 tokens a thread, and more where rows are few, down to nine (151936 tokens: one row
-     * takes 27 / 20 / 16 us on 4 / 8 / 16 CTAs; 64 rows 59 / 56 / 83, 256 rows with filters of their own 521 / 519 on
-     * 4 / 8; 30 rows of 20000 52 / 16 / 18 us on 2 / 4 / 8) */
+    /* CTAs a row: what lets two be on an SM (256 rows of 151936 bf16, settings of their own: 4 CTAs 163 us, 8 203 us; 256 of
+     * 32000: 1 73, 2 70, with top-k 50 for all 25 and 38 us), and more where they all are resident still, down to ten
+     * tokens a thread (1 x 151936, top-k 50: 2 / 4 / 8 / 16 CTAs 26 / 20 / 15.6 / 15.6 us, mixed 75 / 53 / 37 / 34; 30 rows of
+     * 65000 mixed: 2 / 4 / 8 / 16 58 / 41 / 37 / 47 us; 64 of 32000: 38 / 36 / 48 on 2 / 4 / 8); rows of more than 70 tokens
+     * a thread may take a second wave (64 x 151936 mixed: 4 CTAs 86 us, 8 76). */
     int size = 1;
     const auto each = [&]() { return words_of(p.n_vocab, size, ksz) * (4 / ksz); };
-    while (size < kMaxCluster && (row_smem(p.n_vocab, size, ksz) > kRowSmem || each() > 39 || ((long long)p.rows * size < 100 && each() > 9))) size *= 2;
+    const auto all = [&]() { return (long long)p.rows * size; };
+    while (size < kMaxCluster && (row_smem(p.n_vocab, size, ksz) > 112 * 1024 || (all() <= 150 && each() > 10) || (all() <= 256 && each() > 70))) size *= 2;
     if (row_smem(p.n_vocab, size, ksz) > kRowSmem) {
         k_nucleus_long<<<(unsigned)p.rows, 1024, 0, st>>>(P);
         return cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;

@@ -368,6 +368,24 @@ def test_sample_rows_whose_logits_lie_next_to_each_other(V):
     _check_sample(two, u, None, k, p)
 
 
+@pytest.mark.parametrize("M,V,dt", [(64, 151936, BF16), (300, 20001, F32), (512, 5003, BF16), (513, 5003, BF16), (700, 3001, F32)])
+def test_sample_rows_of_long_batches_keep_their_places(M, V, dt):
+    """batches of more than a wave: every row's answer is that of a call of its own rows"""
+    g = _rng(M + V)
+    x = (torch.randn(M, V, generator=g, device="cuda") * 3).to(dt)
+    x[5::7, 1:] = -math.inf
+    x[6::50] = math.nan
+    u, (t, k, p, low) = torch.rand(M, generator=g, device="cuda"), _planes(g, M)
+    kept, lp = torch.empty(M, dtype=torch.int32, device="cuda"), torch.empty(M, device="cuda")
+    token = ops.sample_nucleus(x, u, temperature=t, top_k=k, top_p=p, min_p=low, kept=kept, logprob=lp)
+    for at in range(0, M, 20):
+        few = slice(at, at + 20)
+        n, l = torch.empty_like(kept[few]), torch.empty_like(lp[few])
+        one = ops.sample_nucleus(x[few], u[few], temperature=t[few], top_k=k[few], top_p=p[few], min_p=low[few], kept=n, logprob=l)
+        assert torch.equal(one, token[few]) and torch.equal(n, kept[few]) and torch.equal(l, lp[few])
+    assert bool((token[6::50] == -1).all()) and bool((token[5::7][token[5::7] >= 0] == 0).all())
+
+
 def test_sample_temperatures_far_apart():
     g = _rng(77)
     M, V = 8, 20000
