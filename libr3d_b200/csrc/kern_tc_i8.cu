@@ -6,10 +6,11 @@
  * owns a token, whose channels lie next to each other in registers as they do in y, and the channel tile can be any
  * multiple of 16, which is what balances a wave over 148 SMs.
  *
- * k_i8_stream (M <= 128): bound by the weights' bytes. One CTA a channel tile, the channel tile chosen so that the
- *   tiles fill the device's slots (27648 channels: 288 tiles of 96 on 296 slots), a deep TMA ring; rows of the token
- *   tile past M are whatever shared memory holds, their lanes are never read. Where channels alone do not fill the
- *   device, the CTAs of a cluster split K and add their 32-bit sums through distributed shared memory.
+ * k_i8_stream (M <= 128, and more tokens on few channels): bound by the weights' bytes. One CTA a channel tile (and 128
+ *   tokens), the channel tile chosen so that the tiles fill the device's slots (27648 channels: 288 tiles of 96 on 296
+ *   slots), a deep TMA ring; rows of the token tile past M are whatever shared memory holds, their lanes are never read.
+ *   Where the tiles do not fill the device, the CTAs of a cluster split K and add their 32-bit sums through distributed
+ *   shared memory.
  *
  * k_i8_pair (M > 128): bound by the tensor pipe and by the operands' way from L2 into shared memory. CTA pairs
  *   (cta_group::2), 256 tokens x 512 channels a pair: 96 KiB of operands for 2 x 256 x 512 x 128 operations, two
@@ -388,7 +389,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
     }
 }
 
-/* ------------------------------------------------------------------ M <= 128: the weights' stream */
+/* ------------------------------------------------------------------ few tokens or few channels: the weights' stream */
 constexpr int kStreamThreads = 32 * 6;
 constexpr int kMaxShares = 8;                      /* a portable cluster */
 constexpr size_t kStreamSmem = 220 * 1024;
@@ -403,7 +404,8 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     __shared__ __align__(16) float sb_s[256];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int shares = P.shares, crank = shares > 1 ? (int)cluster_rank() : 0;
-    const int n0 = (int)(blockIdx.x / shares) * P.nt;
+    /* neighbours share a channel tile's weights in L2 */
+    const int job = (int)(blockIdx.x / shares), n0 = job / P.tok_tiles * P.nt, t0 = job % P.tok_tiles * 128, m = min(128, P.m - t0);
     const int it0 = (int)((int64_t)P.nk * crank / shares), nk = (int)((int64_t)P.nk * (crank + 1) / shares) - it0;
     const int ablock = P.mb * kStageK, stage = ablock + P.nt * kStageK;
     const uint32_t cols = P.nt <= 32 ? 32u : P.nt <= 64 ? 64u : P.nt <= 128 ? 128u : 256u;
@@ -434,7 +436,7 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 const int at = it0 + it;
                 mbar_expect_tx(&full[s], (uint32_t)stage);
                 tma_load_2d(st + ablock, &tmB, at * kStageK, n0, &full[s]);
-                tma_load_2d(st, &tmA, at * kStageK, 0, &full[s]);
+                tma_load_2d(st, &tmA, at * kStageK, t0, &full[s]);
                 if (++s == P.stages) { s = 0; ph ^= 1u; }
             }
         }
@@ -457,7 +459,7 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         }
         __syncwarp();
     } else {
-        for (int i = threadIdx.x - 64; i < P.m; i += 128) sa_s[i] = __ldg(P.as + (int64_t)i * P.as_pitch);
+        for (int i = threadIdx.x - 64; i < m; i += 128) sa_s[i] = __ldg(P.as + (int64_t)(t0 + i) * P.as_pitch);
         for (int i = threadIdx.x - 64; i < P.nt; i += 128) sb_s[i] = channel_scale(P, n0 + i);
     }
     /* the sums of the CTA's K share as [token][channel] words over the ring, whose stages are all consumed */
@@ -468,13 +470,13 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     if (warp >= 2 && ok) {
         const int q = warp & 3, t = q * 32 + lane;
         tc_fence_after();
-        if (q * 32 < P.m)
+        if (q * 32 < m)
             for (int c = 0; c < P.nt; c += 16) {
                 uint32_t v[16];
                 tmem_ld16u(tmem_base + ((uint32_t)(q * 32) << 16) + c, v);
                 tmem_ld_wait();
                 pin_u32<16>(v);
-                if (t < P.m)
+                if (t < m)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) *(uint4*)(sums + t * pitch + c + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             }
@@ -484,13 +486,13 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     if (ok) {
         /* four channels of a token a thread, all of them spread over the threads of the cluster; the peers' words of two
          * such items are requested together (one at a time: 1.5 us more at 128 tokens and five shares) */
-        const int quads = P.nt / 4, items = P.m * quads, step = kStreamThreads * shares;
+        const int quads = P.nt / 4, items = m * quads, step = kStreamThreads * shares;
         const auto finish = [&](int item, int4 v) {
             const int t = item / quads, c = 4 * (item - t * quads), live = P.n - n0 - c;
             const float sa = sa_s[t];
             const float4 sb = *(const float4*)(sb_s + c);
             const float y[4] = {scaled((uint32_t)v.x, sa, sb.x), scaled((uint32_t)v.y, sa, sb.y), scaled((uint32_t)v.z, sa, sb.z), scaled((uint32_t)v.w, sa, sb.w)};
-            const int64_t at = (int64_t)t * P.y_pitch + n0 + c;
+            const int64_t at = (int64_t)(t0 + t) * P.y_pitch + n0 + c;
             if (P.y_f32) {
                 float* const o = (float*)P.y + at;
                 if (P.y_quads && live >= 4) *(float4*)o = make_float4(y[0], y[1], y[2], y[3]);
@@ -650,12 +652,13 @@ int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     static bool set[kTcMaxDevices] = {};
     if (!allow_smem(k_i8_stream, kStreamSmem, set)) return RAD_E_DEVICE;
     I8Params P = params_of(p);
-    P.mb = (p.m + 7) / 8 * 8;
+    P.mb = p.m > 128 ? 128 : (p.m + 7) / 8 * 8;
+    P.tok_tiles = (p.m + 127) / 128;
     const int sms = tc_sm_count();
-    const int per_sm = P.mb <= 64 || p.n >= 160 * sms ? 2 : 1, slots = sms * per_sm;
+    const int per_sm = P.mb <= 64 || (p.m <= 128 && p.n >= 160 * sms) ? 2 : 1, slots = sms * per_sm;
     P.shares = 1;
     if (per_sm == 1) {
-        /* 65 tokens and more, fewer than 160 channels an SM: a CTA has an SM, and the channels of a tile and the K shares are
+        /* 65 tokens and more (fewer than 160 channels an SM up to 128): a CTA has an SM, and the channels of a tile and the K shares are
          * those with the lowest cost of a K block (its two operands' way into shared memory), of a tile's results, and of
          * adding the shares' sums, in nanoseconds, fitted to 540 measured forms of thirteen sizes (12288 channels, K = 4096,
          * 128 tokens: 128 tiles of 96 14.8 us, 192 channels in two shares 19.0 us; 5120, 13824: 4 shares of 160 channels
@@ -664,7 +667,7 @@ int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
         long best = -1;
         for (int nt = 48; nt <= 256; nt += 16)
             for (int sh = 1; sh <= kMaxShares && (sh == 1 || 5 * sh <= P.nk); ++sh) {
-                const long tiles = (p.n + nt - 1) / nt;
+                const long tiles = (p.n + nt - 1) / nt * P.tok_tiles;
                 if (sh > 1 && (tiles * sh > slots || tiles > resident_clusters(tc_device(), sh))) break;
                 const long cost = (tiles * sh + slots - 1) / slots * ((P.nk + sh - 1) / sh * (61 + 5L * (P.mb + nt) / 8) + (long)P.mb * nt / 5) +
                                   (sh > 1 ? (long)P.mb * nt / 20 : 0);
@@ -699,12 +702,12 @@ int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     P.y_quads = (((uintptr_t)p.y | (uintptr_t)(p.y_pitch * esz)) & (uintptr_t)(4 * esz - 1)) == 0;
     /* the MMA reads 128 token rows from wherever the token tile starts: the last stage's reach 16 KiB on */
     const size_t ring = (size_t)P.stages * stage + 128 * kStageK;
-    const size_t sums = (size_t)p.m * (P.nt + 4) * 4;
+    const size_t sums = (size_t)(p.m < 128 ? p.m : 128) * (P.nt + 4) * 4;
     const size_t smem = 1024 + (ring > sums ? ring : sums);
     if (smem > kStreamSmem) return RAD_E_UNSUPPORTED;
     CUtensorMap ta, tb;
     if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, P.mb) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt)) return RAD_E_UNSUPPORTED;
-    return launch(k_i8_stream, tiles * P.shares, kStreamThreads, smem, P.shares, st, ta, tb, P);
+    return launch(k_i8_stream, P.tok_tiles * tiles * P.shares, kStreamThreads, smem, P.shares, st, ta, tb, P);
 }
 
 } /* namespace */
@@ -712,7 +715,12 @@ int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
 bool tc_i8_ok(const R3dGemmI8& p) {
     return grid16(p.a, p.a_pitch) && grid16(p.b, p.b_pitch) && p.a_pitch >= p.k && p.b_pitch >= p.k && tc_have_encoder();
 }
-int tc_i8(const R3dGemmI8& p, cudaStream_t st) { return p.m <= 128 ? tc_i8_stream(p, st) : tc_i8_pair(p, st); }
+/* Above 128 tokens the streams, 128 tokens a CTA, where tiles of 256 tokens x 64 channels would not be enough for one and a half waves of pairs:
+ * they split K instead (191 x 576, K = 13568: 9.0 us instead of 26.3; 687 x 900, 10112: 14.5 and 22.2; 457 x 2304, 6272, 72
+ * tiles: 14.8 and 15.6; but 734 x 728, 1568: 7.8 and 6.7). With more tiles the pairs are faster (472 x 4800, 4096: 14.6 us,
+ * 16.1; 764 x 12464, 2016: 18.5, 38.3). */
+bool tc_i8_streams(const R3dGemmI8& p) { return p.m <= 128 || (long)((p.m + 255) / 256) * ((p.n + 63) / 64) * 2 <= tc_sm_count() / 2 * 3; }
+int tc_i8(const R3dGemmI8& p, cudaStream_t st) { return tc_i8_streams(p) ? tc_i8_stream(p, st) : tc_i8_pair(p, st); }
 
 int tc_i8_status() {
     int v = 0;

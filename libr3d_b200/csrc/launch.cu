@@ -346,7 +346,7 @@ extern "C" int r3d_b200_gemm_i8a8(const R3dGemmI8* q, void* stream) {
     if (!device_is_sm100()) return RAD_E_UNSUPPORTED;
     if (q->arm != R3D_ARM_AUTO && q->arm != R3D_ARM_EXACT && q->arm != R3D_ARM_TILE) return RAD_E_UNSUPPORTED;
     if (q->arm != R3D_ARM_EXACT && tc_i8_ok(*q)) {
-        debug_arm("i8a8", q->m <= 128 ? "tcgen05 weight stream" : "tcgen05 pair tiles", q->m);
+        debug_arm("i8a8", tc_i8_streams(*q) ? "tcgen05 weight stream" : "tcgen05 pair tiles", q->m);
         return tc_i8(*q, (cudaStream_t)stream);
     }
     if (q->arm == R3D_ARM_TILE) return RAD_E_UNSUPPORTED;

@@ -52,6 +52,7 @@ int launch_gemm_w2a8(const R3dW2A8& q, cudaStream_t st);
 int i8_tile(const R3dGemmI8& p, cudaStream_t st);
 /* ... and on tcgen05 (kern_tc_i8.cu): operands on the 16-byte grid */
 bool tc_i8_ok(const R3dGemmI8& p);
+bool tc_i8_streams(const R3dGemmI8& p);
 int  tc_i8(const R3dGemmI8& p, cudaStream_t st);
 int  tc_i8_status();
 int launch_token_i8(const R3dTokenI8& p, cudaStream_t st);

@@ -64,6 +64,13 @@ def test_gemm_tiles_and_shares_up_to_128_tokens(M, N, K):
     test_gemm_against_whole_numbers(M, N, K, F32)
 
 
+@pytest.mark.parametrize("M,N,K", [(129, 700, 4112), (191, 576, 13568), (257, 64, 13824), (300, 513, 8192), (687, 900, 1040), (1000, 1000, 400), (2000, 128, 528),
+                                   (300, 2304, 1024), (300, 2369, 1024), (5000, 64, 256), (640, 1001, 272)])
+def test_gemm_many_tokens_on_few_channels(M, N, K):
+    test_gemm_against_whole_numbers(M, N, K, BF16)
+    test_gemm_against_whole_numbers(M, N, K, F32)
+
+
 def test_gemm_extremes_stay_inside_32_bits():
     K = 131071
     a = torch.full((3, K), -128, dtype=torch.int8, device="cuda")
