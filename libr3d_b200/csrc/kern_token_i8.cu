@@ -118,6 +118,20 @@ template <typename T> struct Raw;
 template <> struct Raw<uint16_t> {
     uint32_t w[4];
     __device__ __forceinline__ void get(const uint16_t* p) { const uint4 v = *(const uint4*)p; w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+    /* from any element on: the 16-byte words that hold some of the eight, moved down by the elements in front */
+    __device__ __forceinline__ void get_off(const uint16_t* p) {
+        const uint4* const q = (const uint4*)((uintptr_t)p & ~(uintptr_t)15);
+        const uint4 a = q[0], b = q[1];
+        const int d = (int)((uintptr_t)p & 15) >> 1;
+        uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 6; ++i) v[i] = d & 4 ? v[i + 2] : v[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) v[i] = d & 2 ? v[i + 1] : v[i];
+        const uint32_t take = d & 1 ? 0x5432 : 0x3210;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __byte_perm(v[i], v[i + 1], take);
+    }
     __device__ __forceinline__ void put(uint16_t* p) const { *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]); }
     __device__ __forceinline__ f2 pair(int j) const { return two_of(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)); }
     __device__ __forceinline__ void set(int j, f2 v) {
@@ -149,6 +163,18 @@ template <> struct Raw<float> {
         const ulonglong2 a = *(const ulonglong2*)p, b = *(const ulonglong2*)(p + 4);
         v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
     }
+    __device__ __forceinline__ void get_off(const float* p) {
+        const uint4* const q = (const uint4*)((uintptr_t)p & ~(uintptr_t)15);
+        const uint4 a = q[0], b = q[1], c = q[2];
+        const int d = (int)((uintptr_t)p & 15) >> 2;
+        uint32_t w[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 10; ++i) w[i] = d & 2 ? w[i + 2] : w[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = d & 1 ? w[i + 1] : w[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = two_of(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+    }
     __device__ __forceinline__ void put(float* p) const { *(ulonglong2*)p = make_ulonglong2(v[0], v[1]); *(ulonglong2*)(p + 4) = make_ulonglong2(v[2], v[3]); }
     __device__ __forceinline__ f2 pair(int j) const { return v[j]; }
     __device__ __forceinline__ void set(int j, f2 x) { v[j] = x; }
@@ -171,11 +197,13 @@ template <> struct Raw<float> {
         }
     }
 };
-/* the chunk at value `at` of a row, which may reach over either end of it: by 16 bytes where `fast` */
-template <typename T>
-__device__ __forceinline__ Raw<T> load_chunk(const T* row, int at, int n, bool fast) {
+__device__ __forceinline__ bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+/* the chunk at value `at` of a row, which may reach over either end of it unless `in`: by 16 bytes where it lies on their grid,
+ * else (OFF) by those around it, or one value at a time */
+template <bool OFF, typename T>
+__device__ __forceinline__ Raw<T> load_chunk(const T* row, int at, int n, bool in, bool grid) {
     Raw<T> r;
-    if (fast) r.get(row + at); else r.scalars(row, at, n);
+    if (in && grid) r.get(row + at); else if (OFF && in) r.get_off(row + at); else r.scalars(row, at, n);
     return r;
 }
 template <typename T>
@@ -185,11 +213,10 @@ __device__ __forceinline__ void store_chunk(T* row, int at, int n, bool fast, co
     for (int j = 0; j < 4; ++j) r.set(j, h[j]);
     if (fast) r.put(row + at); else r.put_scalars(row, at, n);
 }
-__device__ __forceinline__ bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-/* The block walks rows gridDim apart. A row is cut into chunks of eight values on x's 16-byte grid, wherever the row
- * begins, C chunks a thread; what else lies on that grid (the residual of an odd width as well) is accessed by 16 bytes
- * too. GRID: every row of every operand begins on its grid and ends a chunk. While a row is reduced, the next one is on
+/* The block walks rows gridDim apart. A row is cut into chunks of eight values on the codes' 8-byte grid, wherever the row
+ * begins, C chunks a thread; what else lies on that grid is copied by 16 bytes, and what does not (the up half of an odd
+ * width) is read by the 16-byte words around it: one value at a time took 100 instead of 90 us for 8191 x 5125 gated, 25 instead of 17 for 6043 x 1291. GRID: every row of every operand begins on its grid and ends a chunk. While a row is reduced, the next one is on
  * its way into shared memory by cp.async, each thread's chunks to places of its own: no barrier, no registers.
  * Instructions, not bytes, bound the bf16 forms at first (46 a value): hence two values an instruction wherever there is
  * one, and the residual's sum in bf16 pairs. */
@@ -197,6 +224,7 @@ template <int KIND, typename T, int C, bool GRID>
 __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const TokenI8 P) {
     constexpr bool kTwo = KIND != kQuant;                         /* the residual, or the up half */
     constexpr int kPer = 8 * (int)sizeof(T);                      /* bytes of a chunk */
+    constexpr bool kOff = KIND == kSilu || KIND == kSigmoid;      /* the others' operands lie on one grid if their rows follow each other */
     extern __shared__ __align__(16) uint8_t slots[];
     __shared__ float part[2][32];
     const int n = P.n, threads = blockDim.x;
@@ -207,7 +235,7 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
     T* y = KIND == kRms ? (T*)P.res + (P.res ? row * P.r_pitch : 0) : const_cast<T*>(x) + n;
     const int64_t x_step = P.x_pitch * gridDim.x, y_step = KIND == kRms ? P.r_pitch * gridDim.x : x_step;
     uint8_t* const slot = slots + threadIdx.x * kPer;             /* chunk c of x: c * threads on; of y: C + c */
-    const auto lead = [&]() { return GRID ? 0 : -(int)(((uintptr_t)x & 15) / sizeof(T)); };
+    const auto lead = [&](int64_t r) { return GRID ? 0 : -(int)((uintptr_t)(P.q + r * P.q_pitch) & 7); };
     const auto whole = [&](int at) { return GRID ? at < n : at >= 0 && at + 8 <= n; };
     const auto copy = [&](int place, const T* from) {
 #pragma unroll
@@ -216,17 +244,17 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
                          ::"r"((uint32_t)__cvta_generic_to_shared(slot + place * threads * kPer) + b), "l"((const char*)from + b) : "memory");
     };
     const auto fetch = [&](int first) {
-        const bool y_grid = two && (GRID || on16(y + first));
+        const bool x_grid = GRID || on16(x + first), y_grid = two && (GRID || on16(y + first));
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int at = first + c * threads * 8;
             if (!whole(at)) continue;
-            copy(c, x + at);
+            if (x_grid) copy(c, x + at);
             if (kTwo && y_grid) copy(C + c, y + at);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    int first = lead() + (int)threadIdx.x * 8;
+    int first = lead(row) + (int)threadIdx.x * 8;
     fetch(first);
     /* a norm's two reductions lie a barrier apart each; the other kinds have one barrier a row, so that a warp may be a row
      * ahead of another that still reads: their rows take the two places by turns */
@@ -236,7 +264,7 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
         f2 ss = 0, bad = 0;
         float amax = 0.0f;
         const int here = first;                                   /* this row's; `first` moves on to the next below */
-        const bool y_grid = two && (GRID || on16(y + here));
+        const bool x_grid = GRID || on16(x + here), y_grid = two && (GRID || on16(y + here));
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -246,9 +274,9 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
             if (GRID && at >= n) continue;
             const bool in = whole(at);
             Raw<T> r, s;
-            if (in) r.get((const T*)(slot + c * threads * kPer)); else r.scalars(x, at, n);
+            if (in && x_grid) r.get((const T*)(slot + c * threads * kPer)); else r = load_chunk<kOff, T>(x, at, n, in, false);
             if (two) {
-                if (in && y_grid) s.get((const T*)(slot + (C + c) * threads * kPer)); else s.scalars((const T*)y, at, n);
+                if (in && y_grid) s.get((const T*)(slot + (C + c) * threads * kPer)); else s = load_chunk<kOff, T>(y, at, n, in, false);
                 if (KIND == kRms) {
                     r.add(s);
                     if (in && y_grid) r.put(y + at); else r.put_scalars(y, at, n);
@@ -268,7 +296,7 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
             for (int j = 0; j < 4; ++j) asm volatile("" : "+l"(h[c][j]));
         if (row + gridDim.x < rows) {
             x += x_step; y += y_step;
-            first = lead() + (int)threadIdx.x * 8;
+            first = lead(row + gridDim.x) + (int)threadIdx.x * 8;
             fetch(first);
         }
         if (KIND == kRms) {
@@ -282,13 +310,13 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
             for (int c = 0; c < C; ++c) {
                 const int at = here + c * threads * 8;
                 if (GRID && at >= n) continue;
-                const bool in = w_grid && whole(at);
+                const bool in = whole(at);
                 if (P.w_f32) {
-                    const Raw<float> w = load_chunk((const float*)P.w, at, n, in);
+                    const Raw<float> w = load_chunk<sizeof(T) == 4>((const float*)P.w, at, n, in, w_grid);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) h[c][j] = mul2(mul2(h[c][j], rs2), add2(w.pair(j), wadd2));
                 } else {
-                    const Raw<uint16_t> w = load_chunk((const uint16_t*)P.w, at, n, in);
+                    const Raw<uint16_t> w = load_chunk<sizeof(T) == 4>((const uint16_t*)P.w, at, n, in, w_grid);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) h[c][j] = mul2(mul2(h[c][j], rs2), add2(w.pair(j), wadd2));
                 }
@@ -315,7 +343,6 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
         if (threadIdx.x == 0) P.scale[row * P.s_pitch] = scale_of(amax);
         const f2 step2 = two_of(step, step), code2 = two_of(kCode, kCode);
         int8_t* const q = P.q + row * P.q_pitch;
-        const bool q_grid = GRID || ((uintptr_t)(q + here) & 7) == 0;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int at = here + c * threads * 8;
@@ -331,7 +358,7 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
                                    __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040), 0x5410);
                 if (step == 0.0f) w[j] = 0u;
             }
-            if (in && q_grid) *(uint2*)(q + at) = make_uint2(w[0], w[1]);
+            if (in) *(uint2*)(q + at) = make_uint2(w[0], w[1]);
             else
 #pragma unroll
                 for (int j = 0; j < 8; ++j) if ((unsigned)(at + j) < (unsigned)n) q[at + j] = (int8_t)(w[j >> 2] >> (8 * (j & 3)));
@@ -410,7 +437,7 @@ bool rows_on(const void* p, int64_t pitch, int esz, int grid) { return !p || (((
 
 template <int KIND, typename T, bool GRID>
 int launch_regs(const TokenI8& P, int rows, cudaStream_t st) {
-    const int most = P.n + (GRID ? 0 : 16 / (int)sizeof(T) - 1);  /* a row may begin anywhere inside its first 16 bytes */
+    const int most = P.n + (GRID ? 0 : 7);                        /* a row may begin anywhere inside its first chunk */
     /* Chunks a thread. Few rows: as many threads as the row has chunks (4 x 5120 norm: 2.6 us with one chunk a thread,
      * 3.0 with two, 3.7 with four). Many rows: fewer threads, whose barriers cost less (8192 x 5120 norm: 62 / 51 / 53 us;
      * 4099 x 5120 codes alone: 17.8 / 13.7 / 12.5 us; 8192 x 13824 gated: two 101, four 96 us; 16384 x 512 codes:
