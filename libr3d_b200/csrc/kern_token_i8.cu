@@ -216,7 +216,7 @@ __device__ __forceinline__ void store_chunk(T* row, int at, int n, bool fast, co
 
 /* The block walks rows gridDim apart. A row is cut into chunks of eight values on the codes' 8-byte grid, wherever the row
  * begins, C chunks a thread; what else lies on that grid is copied by 16 bytes, and what does not (the up half of an odd
- * width) is read by the 16-byte words around it: one value at a time took 100 instead of 90 us for 8191 x 5125 gated, 25 instead of 17 for 6043 x 1291. GRID: every row of every operand begins on its grid and ends a chunk. While a row is reduced, the next one is on
+ * width) is read by the 16-byte words around it: one value at a time took 100 instead of 67 us for 8191 x 5125 gated, 25 instead of 17 for 6043 x 1291. GRID: every row of every operand begins on its grid and ends a chunk. While a row is reduced, the next one is on
  * its way into shared memory by cp.async, each thread's chunks to places of its own: no barrier, no registers.
  * Instructions, not bytes, bound the bf16 forms at first (46 a value): hence two values an instruction wherever there is
  * one, and the residual's sum in bf16 pairs. */
@@ -440,10 +440,10 @@ int launch_regs(const TokenI8& P, int rows, cudaStream_t st) {
     const int most = P.n + (GRID ? 0 : 7);                        /* a row may begin anywhere inside its first chunk */
     /* Chunks a thread. Few rows: as many threads as the row has chunks (4 x 5120 norm: 2.6 us with one chunk a thread,
      * 3.0 with two, 3.7 with four). Many rows: fewer threads, whose barriers cost less (8192 x 5120 norm: 62 / 51 / 53 us;
-     * 4099 x 5120 codes alone: 17.8 / 13.7 / 12.5 us; 8192 x 13824 gated: two 101, four 96 us; 16384 x 512 codes:
+     * 4099 x 5120 codes alone: 17.8 / 13.7 / 12.5 us; 8192 x 13824 gated: two 101, four 96 us, but off the grid, 8191 x 5125, 67 and 88; 16384 x 512 codes:
      * 8.7 / 7.3 / 8.2 us). */
     int c = most <= 8192 ? 1 : most <= 16384 ? 2 : 4;
-    if (rows > 2 * 148 && c < 4) c = KIND != kRms && most > 4096 ? 4 : most > 256 ? 2 : 1;
+    if (rows > 2 * 148 && c < 4) c = KIND != kRms && most > 4096 && (GRID || KIND == kQuant) ? 4 : most > 256 ? 2 : 1;
     const int t = ((most + 8 * c - 1) / (8 * c) + 31) / 32 * 32;
     return c == 1 ? launch_rows<KIND, T, 1, GRID>(P, rows, t, st) : c == 2 ? launch_rows<KIND, T, 2, GRID>(P, rows, t, st)
                                                                              : launch_rows<KIND, T, 4, GRID>(P, rows, t, st);
