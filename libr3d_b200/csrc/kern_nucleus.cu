@@ -541,6 +541,8 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
                             } else u[c] = take(u[c], i + c);
                         }
                         *(uint4*)(keys + i) = w[j];
+                    } else if (i >= 0 && i >= here && i + kEach <= span) {
+                        *(uint4*)(keys + i) = make_uint4(0u, 0u, 0u, 0u);
                     } else {
 #pragma unroll 1
                         for (int c = 0; c < kEach; ++c) if (i + c >= 0 && i + c < span) take_one(i + c);

@@ -336,6 +336,7 @@ extern "C" int r3d_b200_gated_quant_fp8(const void* gu, int64_t gu_pitch, void* 
 /* what the int8 step's calls can be made of */
 static bool wide_type(int32_t dt) { return dt == RAD_F32 || dt == RAD_BF16; }
 static bool extent_ok(int32_t n) { return n > 0 && n <= 0x7ffffff; }
+static bool on_own_grid(const void* p, int32_t dt) { return ((uintptr_t)p & (dt == RAD_F32 ? 3u : 1u)) == 0; }
 
 /* gemm_nt_q @ i8a8. AUTO: the tcgen05 kernels where TMA can take the operands, else the dp4a tile kernel. */
 extern "C" int r3d_b200_gemm_i8a8(const R3dGemmI8* q, void* stream) {
@@ -343,6 +344,7 @@ extern "C" int r3d_b200_gemm_i8a8(const R3dGemmI8* q, void* stream) {
     if (!extent_ok(q->m) || !extent_ok(q->n) || !extent_ok(q->k) || q->k > 131071) return RAD_E_SHAPE;
     if (q->a_pitch < 0 || q->b_pitch < 0 || q->as_pitch < 0 || q->bs_pitch < 0 || (q->m > 1 && q->y_pitch < q->n)) return RAD_E_STRIDE;
     if (!wide_type(q->bs_dtype) || !wide_type(q->y_dtype)) return RAD_E_DTYPE;
+    if (!on_own_grid(q->a_scale, RAD_F32) || !on_own_grid(q->b_scale, q->bs_dtype) || !on_own_grid(q->y, q->y_dtype)) return RAD_E_STRIDE;
     if (!device_is_sm100()) return RAD_E_UNSUPPORTED;
     if (q->arm != R3D_ARM_AUTO && q->arm != R3D_ARM_EXACT && q->arm != R3D_ARM_TILE) return RAD_E_UNSUPPORTED;
     if (q->arm != R3D_ARM_EXACT && tc_i8_ok(*q)) {
@@ -360,6 +362,8 @@ extern "C" int r3d_b200_token_i8(const R3dTokenI8* q, void* stream) {
     if (norm ? !q->w : q->w || q->residual) return RAD_E_INVAL;
     if (!wide_type(q->x_dtype) || (norm && !wide_type(q->w_dtype)) || (q->out && !wide_type(q->out_dtype))) return RAD_E_DTYPE;
     if (!extent_ok(q->rows) || !extent_ok(q->n) || q->n > 0x3ffffff) return RAD_E_SHAPE;
+    if (!on_own_grid(q->x, q->x_dtype) || !on_own_grid(q->residual, q->x_dtype) || (norm && !on_own_grid(q->w, q->w_dtype)) ||
+        !on_own_grid(q->scale, RAD_F32) || !on_own_grid(q->out, q->out_dtype)) return RAD_E_STRIDE;
     if (q->x_pitch < 0 || (q->rows > 1 && (q->q_pitch < q->n || q->s_pitch < 1 || (q->residual && q->r_pitch < q->n) ||
                                            (q->out && q->out_pitch < q->n)))) return RAD_E_STRIDE;
     if (!device_is_sm100()) return RAD_E_UNSUPPORTED;
@@ -370,6 +374,10 @@ extern "C" int r3d_b200_sample_nucleus(const R3dNucleus* q, void* stream) {
     if (!q || !q->logits || !q->u || !q->token) return RAD_E_INVAL;
     if (!wide_type(q->x_dtype)) return RAD_E_DTYPE;
     if (!extent_ok(q->rows) || !extent_ok(q->n_vocab)) return RAD_E_SHAPE;
+    if (!on_own_grid(q->logits, q->x_dtype)) return RAD_E_STRIDE;
+    for (const void* p : {(const void*)q->u, (const void*)q->temperature, (const void*)q->top_k, (const void*)q->top_p, (const void*)q->min_p,
+                          (const void*)q->token, (const void*)q->logprob, (const void*)q->kept})
+        if (!on_own_grid(p, RAD_F32)) return RAD_E_STRIDE;        /* four bytes, all of them */
     if (q->x_pitch < 0 || q->u_pitch < 0 || q->t_pitch < 0 || q->k_pitch < 0 || q->p_pitch < 0 || q->mp_pitch < 0 ||
         (q->rows > 1 && (q->token_pitch < 1 || (q->logprob && q->lp_pitch < 1) || (q->kept && q->kept_pitch < 1)))) return RAD_E_STRIDE;
     if (!device_is_sm100()) return RAD_E_UNSUPPORTED;

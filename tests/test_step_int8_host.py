@@ -133,6 +133,8 @@ def _struct(which, **over):
     ("norm", dict(x_dtype=abi.RAD_F16), DTYPE), ("norm", dict(w_dtype=I8), DTYPE), ("norm", dict(out=Z, out_dtype=I8), DTYPE), ("norm", dict(rows=0), SHAPE),
     ("norm", dict(q_pitch=7), STRIDE), ("norm", dict(residual=Z, r_pitch=0), STRIDE), ("norm", dict(s_pitch=0), STRIDE), ("norm", dict(x_pitch=-8), STRIDE),
     ("sample", dict(token=None), INVAL), ("sample", dict(x_dtype=abi.RAD_F16), DTYPE), ("sample", dict(n_vocab=0), SHAPE), ("sample", dict(rows=-1), SHAPE),
+    ("gemm", dict(y=Z + 1), STRIDE), ("gemm", dict(a_scale=Z + 2), STRIDE), ("norm", dict(x=Z + 1), STRIDE), ("norm", dict(w=Z + 2), STRIDE),
+    ("norm", dict(scale=Z + 1), STRIDE), ("sample", dict(logits=Z + 2), STRIDE), ("sample", dict(top_k=Z + 2), STRIDE), ("sample", dict(u=Z + 1), STRIDE),
     ("sample", dict(token_pitch=0), STRIDE), ("sample", dict(u_pitch=-1), STRIDE), ("sample", dict(kept=Z, kept_pitch=0), STRIDE),
 ])
 def test_launch_layer_refusals(plug, kind, over, rc):
