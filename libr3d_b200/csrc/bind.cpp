@@ -132,6 +132,14 @@ PyObject* issue(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
 }
 
+at::Tensor rows_of(const at::Tensor& x, long long n, at::ScalarType type) {
+    int64_t size[RAD_MAX_RANK];
+    const int lead = (int)x.dim() - 1;
+    for (int d = 0; d < lead; ++d) size[d] = x.size(d);
+    size[lead] = n;
+    return at::empty(at::IntArrayRef(size, (size_t)(n < 0 ? lead : lead + 1)), x.options().dtype(type).requires_grad(false));
+}
+
 /* rows(x, n, type): a new tensor of x's leading dimensions and n columns (n < 0: no columns) on x's device.
  * type: 0 f32, 1 bf16, 2 int8, 3 int32 */
 PyObject* rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -142,13 +150,32 @@ PyObject* rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     static const at::ScalarType types[4] = {at::kFloat, at::kBFloat16, at::kChar, at::kInt};
     const at::Tensor& x = THPVariable_Unpack(args[0]);
     if (type < 0 || type > 3 || x.dim() < 1 || x.dim() > RAD_MAX_RANK) { PyErr_SetString(PyExc_ValueError, "1 to 8 dimensions are needed"); return nullptr; }
-    int64_t size[RAD_MAX_RANK];
-    const int lead = (int)x.dim() - 1;
-    for (int d = 0; d < lead; ++d) size[d] = x.size(d);
-    size[lead] = n;
     try {
-        return THPVariable_Wrap(at::empty(at::IntArrayRef(size, (size_t)(n < 0 ? lead : lead + 1)), x.options().dtype(types[type]).requires_grad(false)));
+        return THPVariable_Wrap(rows_of(x, n, types[type]));
     } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
+/* codes(x, n): new int8 codes [..., n] and f32 scales [..., 1] for x's rows */
+PyObject* codes(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 2 || !THPVariable_Check(args[0])) { PyErr_SetString(PyExc_TypeError, "codes(tensor, n)"); return nullptr; }
+    const long long n = PyLong_AsLongLong(args[1]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor& x = THPVariable_Unpack(args[0]);
+    if (n < 0 || x.dim() < 1 || x.dim() > RAD_MAX_RANK) { PyErr_SetString(PyExc_ValueError, "1 to 8 dimensions are needed"); return nullptr; }
+    PyObject* q = nullptr;
+    try {
+        q = THPVariable_Wrap(rows_of(x, n, at::kChar));
+        PyObject* s = q ? THPVariable_Wrap(rows_of(x, 1, at::kFloat)) : nullptr;
+        PyObject* both = s ? PyTuple_New(2) : nullptr;
+        if (!both) { Py_XDECREF(q); Py_XDECREF(s); return nullptr; }
+        PyTuple_SET_ITEM(both, 0, q);
+        PyTuple_SET_ITEM(both, 1, s);
+        return both;
+    } catch (const std::exception& e) {
+        Py_XDECREF(q);
         PyErr_SetString(PyExc_RuntimeError, e.what());
         return nullptr;
     }
@@ -156,6 +183,7 @@ PyObject* rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 PyMethodDef kMethods[] = {
     {"issue", (PyCFunction)(void (*)(void))issue, METH_FASTCALL, "one call of an op through its row"},
+    {"codes", (PyCFunction)(void (*)(void))codes, METH_FASTCALL, "new codes and scales for a tensor's rows"},
     {"rows", (PyCFunction)(void (*)(void))rows, METH_FASTCALL, "a new tensor of another's rows"},
     {nullptr, nullptr, 0, nullptr},
 };

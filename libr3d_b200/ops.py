@@ -334,8 +334,10 @@ def gemm_i8a8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
 
 
 def _codes_for(x: torch.Tensor, n: int, q: torch.Tensor | None, scale: torch.Tensor | None):
-    new = (_bind or _load_bind()).rows
-    return new(x, n, _I8) if q is None else q, new(x, 1, _F32) if scale is None else scale
+    bind = _bind or _load_bind()
+    if q is None and scale is None:
+        return bind.codes(x, n)
+    return bind.rows(x, n, _I8) if q is None else q, bind.rows(x, 1, _F32) if scale is None else scale
 
 
 def _act_name(op: str, x: torch.Tensor) -> str:
@@ -348,10 +350,10 @@ def quant_token_i8(x: torch.Tensor, q: torch.Tensor | None = None,
                    scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16/f32 activations [..., n] -> int8 codes [..., n] and one f32 scale a token [..., 1]:
     scale = max|x| / 127, q = rint(x * (127 / max|x|)); a row of zeros has scale 1."""
-    n = x.shape[-1]
+    n, size = x.shape[-1], x.numel()
     q, scale = _codes_for(x, n, q, scale)
-    if x.numel() or not n:
-        _run("quant_token_i8", (("M", x.numel() // max(n, 1)), ("n", n), ("dtype", _act_name("quant_token_i8", x))), x, q, scale)
+    if size or not n:
+        _run("quant_token_i8", (("M", size // max(n, 1)), ("n", n), ("dtype", _NAME_OF.get(x.dtype) or _act_name("quant_token_i8", x))), x, q, scale)
     return q, scale
 
 
