@@ -227,8 +227,9 @@ __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
  *     rounds through the cluster, and no work on the other tokens but reading them.
  *   - Top-p alone, or a k beyond that: a histogram of the distance to the largest logit gives the exact step of the k-th
  *     token, and for top-p a window of steps in which its end lies by the steps' middle weights; one pass of exact sums
- *     proves the window (or moves it). The tokens of the window are gathered and ranked, and the key and the number of
- *     ties at which the kept ones end goes back to all.
+ *     proves the window (or moves it). If it and what lies over it are a few tokens, they end like a top-k of as many; else
+ *     the tokens of the window are gathered and ranked, and the key and the number of ties at which the kept ones end go
+ *     back to all.
  *   - More tokens in a window than can be gathered (a flat row): the key is searched by exact sums, three probes a round.
  * The answer among the kept ones follows from running weights by id.
  * Latency bounds single rows: a round through the cluster is about a microsecond, and so is the first run through a few
@@ -641,6 +642,10 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
             });
     };
 
+    /* what the first CTA has gathered if that is all that can be kept, at most a thread each: how many tokens, how many of
+     * them top-k lets through, and the weight that top-p wants (0: of those) */
+    int few = -1, most = 0;
+    u64 want_few = 0;
     /* ---- top-k of a few */
     int sel = 128;                                                /* groups to rank: at least twice k, which lets through 1.4 k tokens */
     while (sel < 2 * k && sel <= kT) sel *= 2;
@@ -667,37 +672,15 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         meet();
         const int n = (int)peer_get(peer_addr(&s->gathered, 0));
         meet();                                                   /* all have read it */
-        if (bound && n <= kT) {                                   /* a thread for each */
-            if (!first_cta) return;
-            /* in order, a thread each; what is kept is a first part */
-            int sh = share_of(n), i = tid / sh;
-            const int place = count_before(n, i, sh);
-            if (i < n && tid % sh == 0) s->list[kT + place] = s->list[i];
-            __syncthreads();
-            const u64 me = s->list[kT + tid];
-            uint32_t key = (uint32_t)(me >> 32);
-            const bool in = tid < min(n, k);
-            u64 w = in ? weight(key) : 0, sum;
-            const u64 before = scan(w, &sum), want = by_p ? want_of(p, sum) : ~0ull;
-            const bool keep = in && (tid == 0 || (before < want && key >= least_key));
-            /* by id, ascending: the low words are 0xffffffff - id */
-            s->list[tid] = me << 32 | key;
-            s->weight[tid] = w;
-            const int n_kept = __syncthreads_count(keep);
-            scan(keep ? w : 0ull, &sum);
-            sh = share_of(n_kept); i = tid / sh;
-            const u64 run = sum_before(n_kept, i, sh), point = point_of(u, sum);
-            if (i < n_kept && tid % sh == 0 && run <= point && point < run + s->weight[i]) {
-                key = (uint32_t)s->list[i];
-                answer(P, m, (int)(0xffffffffu - (uint32_t)(s->list[i] >> 32)), n_kept, logprob_of(R, key, sum));
-            }
-            return;
+        if (bound && n <= kT) {
+            few = n;
+            most = k;
         }
     }
 
     uint32_t cut = 1;                                             /* kept: keys above cut, and the first `ties` equal to it */
     int ties = V;
-    if (by_k || by_p) {
+    if (few < 0 && (by_k || by_p)) {
         /* ---- histogram of the distance to the largest logit (key order and step order agree) */
         const float mx = val_of(best), inv = (float)((kBins - 1) / kRange * 1.4426950408889634) / t;
         const auto bin_of = [&](float x) {
@@ -864,6 +847,13 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
                     if (one) ties = (int)min((u64)ties, (want - above + one - 1) / one);
                     break;
                 }
+                if (!by_k && want <= v.w[2] && count_to(to) <= kT) {          /* it ends among a few */
+                    gather(1, low_key, best + 1);
+                    meet();
+                    few = most = count_to(to);
+                    want_few = want;
+                    break;
+                }
                 if (want > v.w[1] && want <= v.w[2]) {
                     above = v.w[1];
                     cut = key_at(by_k ? max(cut + 1, low_key) : low_key, high_key, count_to(to) - count_to(from), want, &above, false);
@@ -876,6 +866,34 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
                 else { from = to; to = min(to + width, kBins); }
             }
         }
+    }
+
+    if (few >= 0) {
+        if (!first_cta) return;
+        /* ---- in order, a thread each; what is kept is a first part */
+        const int n = few;
+        int sh = share_of(n), i = tid / sh;
+        const int place = count_before(n, i, sh);
+        if (i < n && tid % sh == 0) s->list[kT + place] = s->list[i];
+        __syncthreads();
+        const u64 me = s->list[kT + tid];
+        uint32_t key = (uint32_t)(me >> 32);
+        const bool in = tid < min(n, most);
+        u64 w = in ? weight(key) : 0, sum;
+        const u64 before = scan(w, &sum), want = want_few ? want_few : by_p ? want_of(p, sum) : ~0ull;
+        const bool keep = in && (tid == 0 || (before < want && key >= least_key));
+        /* by id, ascending: the low words are 0xffffffff - id */
+        s->list[tid] = me << 32 | key;
+        s->weight[tid] = w;
+        const int n_kept = __syncthreads_count(keep);
+        scan(keep ? w : 0ull, &sum);
+        sh = share_of(n_kept); i = tid / sh;
+        const u64 run = sum_before(n_kept, i, sh), point = point_of(u, sum);
+        if (i < n_kept && tid % sh == 0 && run <= point && point < run + s->weight[i]) {
+            key = (uint32_t)s->list[i];
+            answer(P, m, (int)(0xffffffffu - (uint32_t)(s->list[i] >> 32)), n_kept, logprob_of(R, key, sum));
+        }
+        return;
     }
 
     /* ---- the kept ones by id */
