@@ -219,11 +219,11 @@ __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
 }
 
 /* ------------------------------------------------------------------ a cluster a row
- * The row is read once, as ordered keys into the shared memory of the cluster's CTAs; a thread owns `e` neighbouring ids
- * (an odd number of words: its reads fall into banks of their own), so id order is the order of threads. What the CTAs
- * find out goes to all of them through distributed shared memory.
- *   - Top-k of a few: every one to eight threads know the largest key they read. The k-th largest of these is a bound that at
- *     least k tokens reach, and hardly more: they are gathered in the first CTA, which ranks them, cuts and sums. Two
+ * The row is read once, by 16 bytes, as ordered keys into the shared memory of the cluster's CTAs; for what goes by id a
+ * thread owns neighbouring words of keys, so id order is the order of threads. What the CTAs find out goes to all of them
+ * through distributed shared memory.
+ *   - Top-k of a few: every one to eight threads know the largest key they read. A bound that k of these reach, and hardly
+ *     more, is one that at least k tokens reach: these are gathered in the first CTA, which orders them, cuts and sums. Two
  *     rounds through the cluster, and no work on the other tokens but reading them.
  *   - Top-p alone, or a k beyond that: a histogram of the distance to the largest logit gives the exact step of the k-th
  *     token, and for top-p a window of steps in which its end lies by the steps' middle weights; one pass of exact sums
@@ -232,10 +232,11 @@ __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
  *     back to all.
  *   - More tokens in a window than can be gathered (a flat row): the key is searched by exact sums, three probes a round.
  * The answer among the kept ones follows from running weights by id.
- * Latency bounds single rows: a round through the cluster is about a microsecond, and so is the first run through a few
- * hundred instructions, which is why what is used more than once is a call here. Rows without top-k need the
- * exponential of every token. (An atomic add of 64 bits in shared memory takes ten times one of 32: a histogram of exact
- * weights cost 12 of 37 us.) */
+ * Latency bounds single rows (1 x 151936: top-k 50 13.5 us, top-p 28.6): a round through the cluster is about a
+ * microsecond, and so is the first run through a few hundred instructions, which is why what is used more than once is a
+ * call here. Batches are bound by instructions, half of the issue slots (64 x 151936 bf16, settings of their own: 64 us).
+ * Rows without top-k need the exponential of every token. (An atomic add of 64 bits in shared memory takes ten times one of
+ * 32: a histogram of exact weights cost 12 of 37 us.) */
 constexpr int kT = 512, kWarps = kT / 32;
 constexpr int kGroups = 1024;                                     /* of threads, in the cluster, at most */
 constexpr int kBins = 1024, kBinsEach = kBins / kT;
@@ -622,7 +623,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     }
     /* the tokens whose keys are `from` or more and below `to`, to the lists of the first `copies` CTAs, in any order */
     const auto gather = [&](int copies, uint32_t from, uint32_t to) {
-        const uint32_t low_form = max(least_form(from), 1u), range = least_form(to) - low_form;
+        const uint32_t low_form = max(least_form(from), 1u), range = max(least_form(to), low_form) - low_form;
         int n = 0, n_cta;
         each([&](K key, float, int) { n += key - low_form < range; });
         int at = scan(n, &n_cta);
@@ -647,7 +648,7 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
     int few = -1, most = 0;
     u64 want_few = 0;
     /* ---- top-k of a few */
-    int sel = 128;                                                /* groups to rank: at least twice k, which lets through 1.4 k tokens */
+    int sel = 128;                                                /* groups: at least twice k, which lets through 1.4 k tokens */
     while (sel < 2 * k && sel <= kT) sel *= 2;
     static_assert(2 * kSmallK == kT, "what `sel` lets through");
     if (by_k && sel <= kT) {

@@ -215,11 +215,12 @@ __device__ __forceinline__ void store_chunk(T* row, int at, int n, bool fast, co
 }
 
 /* The block walks rows gridDim apart. A row is cut into chunks of eight values on the codes' 8-byte grid, wherever the row
- * begins, C chunks a thread; what else lies on that grid is copied by 16 bytes, and what does not (the up half of an odd
- * width) is read by the 16-byte words around it: one value at a time took 100 instead of 67 us for 8191 x 5125 gated, 25 instead of 17 for 6043 x 1291. GRID: every row of every operand begins on its grid and ends a chunk. While a row is reduced, the next one is on
- * its way into shared memory by cp.async, each thread's chunks to places of its own: no barrier, no registers.
- * Instructions, not bytes, bound the bf16 forms at first (46 a value): hence two values an instruction wherever there is
- * one, and the residual's sum in bf16 pairs. */
+ * begins, C chunks a thread; what else lies on that grid is copied by 16 bytes, and the gated form's halves that do not (an
+ * odd width) are read by the 16-byte words around them: one value at a time took 100 instead of 67 us for 8191 x 5125, 25
+ * instead of 17 for 6043 x 1291. GRID: every row of every operand begins on its grid and ends a chunk. While a row is
+ * reduced, the next one is on its way into shared memory by cp.async, each thread's chunks to places of its own: no barrier,
+ * no registers. Instructions, not bytes, bound the bf16 forms at first (46 a value): hence two values an instruction wherever
+ * there is one, and the residual's sum in bf16 pairs. */
 template <int KIND, typename T, int C, bool GRID>
 __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const TokenI8 P) {
     constexpr bool kTwo = KIND != kQuant;                         /* the residual, or the up half */
