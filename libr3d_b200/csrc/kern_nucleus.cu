@@ -21,6 +21,8 @@
 
 namespace r3d {
 
+bool tc_pdl_on();                     /* kern_tc.cu: false under R3D_NO_PDL */
+
 namespace {
 
 using u64 = unsigned long long;
@@ -477,14 +479,17 @@ __device__ __forceinline__ int long_rows_first(const R3dNucleus& P, int q) {
 }
 
 template <typename K>
-__global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const int e, const int waves) {
+__global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const int e, const int early, const int reorder) {
+    /* the next kernel may begin to launch, unless CTAs of this one still wait for room; the previous one's results are there */
+    if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     Shared* const s = shared();
     constexpr int kEach = 16 / (int)sizeof(K), kPer = 4 / (int)sizeof(K);     /* values of 16 bytes and of four, as logits and as keys */
     Cluster cl;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cl.size));
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cl.rank));
     cl.turn = 0;
-    const int64_t m = waves ? long_rows_first(P, blockIdx.x / cl.size) : blockIdx.x / cl.size;
+    const int64_t m = reorder ? long_rows_first(P, blockIdx.x / cl.size) : blockIdx.x / cl.size;
     const int V = P.n_vocab, span = kT * e * kPer - kEach, base = cl.rank * span, tid = threadIdx.x;      /* this CTA's ids */
     /* the keys lie to the 16-byte grid as the logits do, which takes up to 16 bytes more than the ids' own */
     const K* const x = (const K*)P.logits + m * P.x_pitch + base;
@@ -968,14 +973,16 @@ int launch_row(const R3dNucleus& P, int size, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)P.rows * (unsigned)size); cfg.blockDim = dim3(kT); cfg.stream = st;
     cfg.dynamicSmemBytes = row_smem(P.n_vocab, size, (int)sizeof(K));
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)size; at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at; cfg.numAttrs = 1;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)size; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = tc_pdl_on() ? 2 : 1;
     int sms = 0;
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return RAD_E_DEVICE;
-    const int waves = P.top_p && P.rows <= kT && (long long)P.rows * size > 2 * sms;
-    return cudaLaunchKernelEx(&cfg, kernel, P, e, waves) == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
+    const int early = (long long)P.rows * size <= 2 * sms, reorder = !early && P.top_p && P.rows <= kT;
+    return cudaLaunchKernelEx(&cfg, kernel, P, e, early, reorder) == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
 }
 
 } /* namespace */

@@ -23,7 +23,27 @@
 
 namespace r3d {
 
+bool tc_pdl_on();                     /* kern_tc.cu: false under R3D_NO_PDL */
+
 namespace {
+
+/* the next kernel may begin to launch (`early`: a row a block; among many rows its blocks only took room, 8192 x 5120 norm 53.5
+ * instead of 51.3 us, while 3 x 6144 codes go from 2.2 to 1.8); the previous one's results are there, and all reads and writes
+ * come behind this */
+__device__ __forceinline__ void in_turn(bool early) {
+    if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... P, typename... A>
+cudaError_t launch_in_turn(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at; cfg.numAttrs = tc_pdl_on() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 enum { kQuant = 0, kSilu = 1, kSigmoid = 2, kRms = 3 };
 
@@ -228,6 +248,7 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
     constexpr bool kOff = KIND == kSilu || KIND == kSigmoid;      /* the others' operands lie on one grid if their rows follow each other */
     extern __shared__ __align__(16) uint8_t slots[];
     __shared__ float part[2][32];
+    in_turn(P.rows <= (int)gridDim.x);
     const int n = P.n, threads = blockDim.x;
     const bool two = kTwo && (KIND != kRms || P.res);
     const int64_t rows = P.rows;
@@ -375,6 +396,7 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
 template <int KIND, typename T>
 __global__ void __launch_bounds__(512) k_token_i8(const TokenI8 P) {
     __shared__ float part[2][32];
+    in_turn(false);
     const int64_t row = blockIdx.x;
     float rs = 0.0f;
     if (KIND == kRms) {
@@ -430,8 +452,7 @@ int launch_rows(const TokenI8& P, int rows, int threads, cudaStream_t st) {
         grid = (per > 0 ? per : 1) * sms;
         known.store(grid, std::memory_order_relaxed);
     }
-    kernel<<<(unsigned)(rows < grid ? rows : grid), threads, smem, st>>>(P);
-    return RAD_OK;
+    return launch_in_turn(kernel, (unsigned)(rows < grid ? rows : grid), (unsigned)threads, (size_t)smem, st, P) == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
 }
 
 bool rows_on(const void* p, int64_t pitch, int esz, int grid) { return !p || (((uintptr_t)p | (uintptr_t)(pitch * esz)) & (uintptr_t)(grid - 1)) == 0; }
@@ -457,7 +478,7 @@ int launch_type(const TokenI8& P, int rows, cudaStream_t st) {
     const bool grid = P.n % 8 == 0 && rows_on(P.x, P.x_pitch, esz, 16) && rows_on(P.res, P.r_pitch, esz, 16) && rows_on(P.w, 0, 1, 16) &&
                       rows_on(P.q, P.q_pitch, 1, 8);
     int rc = RAD_OK;
-    if (!fits_slots<KIND, T>(P)) k_token_i8<KIND, T><<<(unsigned)rows, 512, 0, st>>>(P);
+    if (!fits_slots<KIND, T>(P)) rc = launch_in_turn(k_token_i8<KIND, T>, (unsigned)rows, 512u, 0, st, P) == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
     else rc = grid ? launch_regs<KIND, T, true>(P, rows, st) : launch_regs<KIND, T, false>(P, rows, st);
     return rc != RAD_OK ? rc : cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
 }
