@@ -243,7 +243,7 @@ typedef struct R3dGemmI8 {
 int r3d_b200_gemm_i8a8(const R3dGemmI8* q, void* stream);
 
 /* One call of an int8 activation producer: h as `kind` says, then per token scale = max|h| / 127 and
- * q = rint(h * (127 / max|h|)); a row below 2^-100 has scale 1 and codes 0. h is held in f32. */
+ * q = rint(h * 127 / max|h|), halves to even; a row below 2^-100 has scale 1 and codes 0. h is held in f32. */
 enum { R3D_TOKEN_QUANT = 0, R3D_TOKEN_SILU = 1, R3D_TOKEN_SIGMOID = 2, R3D_TOKEN_RMSNORM = 3 };
 typedef struct R3dTokenI8 {
     const void* x;          /* [rows, n], [rows, 2n] for the gated kinds (gate half first); x_dtype RAD_BF16 or RAD_F32 */

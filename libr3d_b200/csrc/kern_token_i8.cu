@@ -4,7 +4,7 @@
  *   gated     h = silu(gate) * up, or sigmoid(gate) * up
  *   rmsnorm   r = x (+ residual, narrowed to the residual's type and stored back);
  *             h = (r * 1/sqrt(mean(r^2) + eps)) * (w + wadd)
- *   all       amax = max |h|; scale = amax / 127; code = rint(h * (127 / amax)).
+ *   all       amax = max |h|; scale = amax / 127; code = rint(h * 127 / amax), halves to even.
  *
  * h stays in f32 from the operands to the code: it is rounded once, to eight bits. A row of zeros (amax below
  * 2^-100, where 127 / amax would overflow) has scale 1 and codes 0; a NaN or an infinity in a row makes its scale
@@ -96,9 +96,17 @@ __device__ __forceinline__ float block_reduce(float v, float* part, F f) {
 /* 1.5 * 2^23: the low byte of fma(h, step, kCode) is the whole number nearest to h * step, ties to even */
 constexpr float kCode = 12582912.0f;
 
-/* a row of zeros, and one so small that 127 / amax is not a number of this type, has step 0: codes 0. So has a row
- * with a NaN or an infinity in it */
-__device__ __forceinline__ float step_of(float amax) { return amax < 0x1p-100f || !(amax < INFINITY) ? 0.0f : 127.0f / amax; }
+/* 127 / amax rounded up. h * step is then rounded once, to the whole number, and is never below the quotient it stands
+ * for, so that h = amax / 2, where that is 63.5 exactly, goes to the even 64 whatever amax is (rounded to nearest, the step
+ * of 66 of the 128 significands that amax has in bf16 is low, and their halves went to 63). Among quotients of two bf16
+ * numbers there is no other half, save where the step is exact (amax = 127 2^n), and what is not a half lies further from
+ * one than the step's error: the codes of bf16 rows are the quotients' own. A row of zeros, and one so small that 127 / amax is not a number of this type, has step 0: codes 0. So
+ * has a row with a NaN or an infinity in it. */
+__device__ __forceinline__ float step_of(float amax) {
+    if (amax < 0x1p-100f || !(amax < INFINITY)) return 0.0f;
+    const float q = 127.0f / amax;
+    return fmaf(q, amax, -127.0f) < 0.0f ? __uint_as_float(__float_as_uint(q) + 1u) : q;      /* the residual's sign is exact */
+}
 __device__ __forceinline__ float scale_of(float amax) { return amax < 0x1p-100f ? 1.0f : amax / 127.0f; }
 
 /* silu(g) * u or sigmoid(g) * u; the exponential and the quotient by the special-function unit, 2 ulp each */

@@ -349,7 +349,8 @@ def _act_name(op: str, x: torch.Tensor) -> str:
 def quant_token_i8(x: torch.Tensor, q: torch.Tensor | None = None,
                    scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16/f32 activations [..., n] -> int8 codes [..., n] and one f32 scale a token [..., 1]:
-    scale = max|x| / 127, q = rint(x * (127 / max|x|)); a row of zeros has scale 1."""
+    scale = max|x| / 127, q = x * 127 / max|x| to the nearest whole number, halves to even; a row whose values all lie
+    below 2^-100 has scale 1 and codes 0."""
     n, size = x.shape[-1], x.numel()
     q, scale = _codes_for(x, n, q, scale)
     if size or not n:
