@@ -478,6 +478,22 @@ __device__ __forceinline__ int long_rows_first(const R3dNucleus& P, int q) {
     return s->pick;
 }
 
+/* the least key with exponent_of(key) >= floor_y, the same in every lane: keys and exponents have one order, and `best`
+ * is one of them */
+__device__ __noinline__ uint32_t least_kept(Row R, uint32_t best, double floor_y) {
+    uint32_t lo = 0x00800000u, hi = best;                         /* from the least number on */
+#pragma unroll 1
+    while (lo < hi) {
+        const uint32_t step = (hi - lo + 31) / 32, at = lo + (threadIdx.x & 31) * step;
+        const uint32_t yes = __ballot_sync(0xffffffffu, at >= hi || exponent_of(R, at) >= floor_y);
+        if (!yes) { lo += 31 * step + 1; continue; }
+        const int first = __ffs(yes) - 1;                         /* the lane before says no, this one yes */
+        hi = min(hi, lo + first * step);
+        if (first) lo += (first - 1) * step + 1;
+    }
+    return hi;
+}
+
 template <typename K>
 __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const int e, const int early, const int reorder) {
     /* the next kernel may begin to launch, unless CTAs of this one still wait for room; the previous one's results are there */
@@ -615,16 +631,17 @@ __global__ void __launch_bounds__(kT, 2) k_nucleus_row(const R3dNucleus P, const
         const uint32_t h = key >> 16;
         return wide((K)h) >= key ? h : h + 1;
     };
-    /* the least key that min-p keeps: from the 32 next to where the bound falls (all keys, if it falls lower) */
+    /* the least key that min-p keeps: among the 32 next to where the bound falls, if it lies between two of them. Next to 0,
+     * where f32 numbers lie closer together than x - mx is known, they may all be on one side of it (and T without end
+     * keeps all keys): then it is searched, a warp looking at 32 keys a step. The largest logit is always kept. */
     uint32_t least_key = 1;
     if (low > 0.0f) {
         const double floor_y = s->floor_y;
         const uint32_t guess = R.inf || !(R.c > 0.0) ? best : key_of((float)fmax(R.mx + s->drop, -3.4e38));
         const uint32_t mine = max(min(guess, best), 32u) - 16 + (tid & 31);
-        const bool in = mine <= best && exponent_of(R, mine) >= floor_y;
-        least_key = __reduce_min_sync(0xffffffffu, in ? mine : 0xffffffffu);
-        if (least_key == max(min(guess, best), 32u) - 16) least_key = 1;          /* even the lowest looked at is kept: T without end */
-        if (R.inf) least_key = best;
+        const uint32_t yes = __ballot_sync(0xffffffffu, mine >= best || exponent_of(R, mine) >= floor_y);
+        least_key = min(best, mine - (tid & 31) + __ffs(yes) - 1);
+        if (!yes || (yes & 1u)) least_key = R.inf ? best : least_kept(R, best, floor_y);
     }
     /* the tokens whose keys are `from` or more and below `to`, to the lists of the first `copies` CTAs, in any order */
     const auto gather = [&](int copies, uint32_t from, uint32_t to) {
