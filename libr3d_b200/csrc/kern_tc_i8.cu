@@ -17,7 +17,8 @@
  *   thirds of what 256 x 256 tiles fetch. The 512 accumulator columns fill tensor memory, so its two halves run
  *   `kLag` K steps apart: while one half is drained, the other half's MMAs still run. Persistent, 74 pairs.
  *
- * Every wait is bounded; on expiry a status word is set and the CTA drains and leaves.
+ * Every wait is bounded; on expiry a status word is set, the copies on their way are waited for (again with a bound), and
+ * the CTA leaves without storing its tile, which no other share of it stores either.
  */
 #include <atomic>
 #include <cstdio>
@@ -395,11 +396,23 @@ constexpr int kMaxShares = 8;                      /* a portable cluster */
 constexpr size_t kStreamSmem = 220 * 1024;
 constexpr int kMaxStages = 16;                     /* 88 KiB of 7 KiB or 190 KiB of 15 KiB: 12 */
 
+/* a warp's wait ran out: the last copies into each stage land before the ring is given up, and all CTAs of the cluster are
+ * told (they began together, a second ago) */
+__device__ __forceinline__ void give_up(uint64_t* full, int issued, int stages, int* failed, int shares) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0)
+        for (int i = issued > stages ? issued - stages : 0; i < issued && mbar_wait(&full[i % stages], (i / stages) & 1, 84); ++i) { }
+    if (shares == 1) *(volatile int*)failed = 1;
+    else if (lane < shares)
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_u32(smem_u32(failed), (uint32_t)lane)), "r"(1) : "memory");
+}
+
 __global__ void __launch_bounds__(kStreamThreads, 2)
 k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const I8Params P) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
     __shared__ uint32_t tmem_slot;
+    __shared__ int issued, failed;                                /* K blocks asked for; a wait of this CTA or of a peer ran out */
     __shared__ float sa_s[128];
     __shared__ __align__(16) float sb_s[256];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -414,6 +427,7 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     if (threadIdx.x == 0) {
         for (int s = 0; s < P.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(&done, 1);
+        failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -429,8 +443,8 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 
     if (warp == 0) {
         if (elect_one()) {
-            int s = 0; uint32_t ph = 0;
-            for (int it = 0; it < nk; ++it) {
+            int s = 0, it = 0; uint32_t ph = 0;
+            for (; it < nk; ++it) {
                 if (!mbar_wait(&empty[s], ph ^ 1u, 81)) break;
                 uint8_t* const st = ring + s * stage;
                 const int at = it0 + it;
@@ -439,14 +453,15 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 tma_load_2d(st, &tmA, at * kStageK, t0, &full[s]);
                 if (++s == P.stages) { s = 0; ph ^= 1u; }
             }
+            issued = it;
         }
         __syncwarp();
     } else if (warp == 1) {
         if (elect_one()) {
             const uint32_t idesc = i8_idesc(128, P.nt);
             const uint64_t desc0 = smem_desc_sw128(smem_u32(ring));
-            int s = 0; uint32_t ph = 0;
-            for (int it = 0; it < nk; ++it) {
+            int s = 0, it = 0; uint32_t ph = 0;
+            for (; it < nk; ++it) {
                 if (!mbar_wait(&full[s], ph, 82)) break;
                 tc_fence_after();
                 const uint64_t a = desc0 + s * (stage >> 4), b = a + (ablock >> 4);
@@ -455,7 +470,7 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 umma_commit(&empty[s]);
                 if (++s == P.stages) { s = 0; ph ^= 1u; }
             }
-            umma_commit(&done);
+            if (it == nk) umma_commit(&done);                     /* else the wait for it runs out, too */
         }
         __syncwarp();
     } else {
@@ -463,8 +478,9 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         for (int i = threadIdx.x - 64; i < P.nt; i += 128) sb_s[i] = channel_scale(P, n0 + i);
     }
     /* the sums of the CTA's K share as [token][channel] words over the ring, whose stages are all consumed */
-    const bool ok = mbar_wait(&done, 0, 83);
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(&done, 0, 83));
     __syncthreads();
+    if (!ok) give_up(full, issued, P.stages, &failed, shares);
     const int pitch = P.nt + 4;                                   /* 16 bytes on: the lanes' rows fall into different banks */
     int* const sums = (int*)ring;
     if (warp >= 2 && ok) {
@@ -483,7 +499,7 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         tc_fence_before();
     }
     if (shares > 1) cluster_sync_all(); else __syncthreads();
-    if (ok) {
+    if (*(volatile int*)&failed == 0) {
         /* four channels of a token a thread, all of them spread over the threads of the cluster; the peers' words of two
          * such items are requested together (one at a time: 1.5 us more at 128 tokens and five shares) */
         const int quads = P.nt / 4, items = m * quads, step = kStreamThreads * shares;
@@ -651,6 +667,7 @@ int resident_clusters(int dev, int shares) {
 int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     static bool set[kTcMaxDevices] = {};
     if (!allow_smem(k_i8_stream, kStreamSmem, set)) return RAD_E_DEVICE;
+    static const int missing = getenv("R3D_TEST_I8_MISSING") ? 16 : 0;     /* a test's: boxes of fewer rows than are waited for */
     I8Params P = params_of(p);
     P.mb = p.m > 128 ? 128 : (p.m + 7) / 8 * 8;
     P.tok_tiles = (p.m + 127) / 128;
@@ -706,7 +723,7 @@ int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     const size_t smem = 1024 + (ring > sums ? ring : sums);
     if (smem > kStreamSmem) return RAD_E_UNSUPPORTED;
     CUtensorMap ta, tb;
-    if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, P.mb) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt)) return RAD_E_UNSUPPORTED;
+    if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, P.mb) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt - missing)) return RAD_E_UNSUPPORTED;
     return launch(k_i8_stream, P.tok_tiles * tiles * P.shares, kStreamThreads, smem, P.shares, st, ta, tb, P);
 }
 
