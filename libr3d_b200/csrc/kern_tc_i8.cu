@@ -235,8 +235,10 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
             asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(&tmB) : "memory");
             Ring<kSA> ra; Ring<kSB> rb;
-            const auto load = [&](uint64_t* full, uint64_t* empty, int s, uint32_t ph, int slot, const CUtensorMap* map, int rows, int x, int y) {
+            int na = 0, nb = 0;                                   /* loads issued */
+            const auto load = [&](uint64_t* full, uint64_t* empty, int s, uint32_t ph, int slot, const CUtensorMap* map, int rows, int x, int y, int& n) {
                 if (!mbar_wait(&empty[s], ph ^ 1u, 91)) return false;
+                ++n;
                 if (leader) mbar_expect_tx(&full[s], 2u * (uint32_t)rows * kStageK);
                 tma_load_2d_pair(smem_u32(smem + slot * kOpBytes), map, x, y, mapa_u32(smem_u32(&full[s]), 0u));
                 return true;
@@ -246,14 +248,19 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
                 const int t0 = J.t0 + (int)crank * kTokC, n0 = J.n0 + (int)crank * bc;
                 for (int it = 0; it < nk + (J.halves - 1) * kLag && alive; ++it) {     /* the order in which the MMAs read */
                     if (it < nk) {
-                        alive = load(full_a, empty_a, ra.s, ra.ph, ra.s, &tmA, kTokC, it * kStageK, t0); ra.next();
-                        alive = alive && load(full_b, empty_b, rb.s, rb.ph, kSA + rb.s, &tmB, bc, it * kStageK, n0); rb.next();
+                        alive = load(full_a, empty_a, ra.s, ra.ph, ra.s, &tmA, kTokC, it * kStageK, t0, na); ra.next();
+                        alive = alive && load(full_b, empty_b, rb.s, rb.ph, kSA + rb.s, &tmB, bc, it * kStageK, n0, nb); rb.next();
                     }
                     if (NH == 2 && J.halves == 2 && it >= kLag && alive) {
-                        alive = load(full_b, empty_b, rb.s, rb.ph, kSA + rb.s, &tmB, bc, (it - kLag) * kStageK, n0 + P.nt); rb.next();
+                        alive = load(full_b, empty_b, rb.s, rb.ph, kSA + rb.s, &tmB, bc, (it - kLag) * kStageK, n0 + P.nt, nb); rb.next();
                     }
                 }
             }
+            /* where a wait ran out, the last loads into each slot are still to land (both CTAs' count on the leader's barriers);
+             * else they have */
+            bool landed = leader;
+            for (int i = na > kSA ? na - kSA : 0; i < na && landed; ++i) landed = mbar_wait(&full_a[i % kSA], (i / kSA) & 1, 98);
+            for (int i = nb > kSB ? nb - kSB : 0; i < nb && landed; ++i) landed = mbar_wait(&full_b[i % kSB], (i / kSB) & 1, 99);
         }
     } else if (warp == 1) {
         /* ---------------- MMA issuer (the pair's leader only) ---------------- */
@@ -613,6 +620,12 @@ int run_pair(const I8Params& P, const CUtensorMap& ta, const CUtensorMap& tb, co
     return launch(k_i8_pair<NH>, 2 * P.workers, kPairThreads, kPairSmem, 1, st, ta, tb, ty, P);
 }
 
+/* a test's: operand boxes of fewer rows than are waited for */
+int missing_rows() {
+    static const int rows = getenv("R3D_TEST_I8_MISSING") ? 16 : 0;
+    return rows;
+}
+
 int tc_i8_pair(const R3dGemmI8& p, cudaStream_t st) {
     I8Params P = params_of(p);
     const int pairs = tc_sm_count() / 2;
@@ -639,7 +652,7 @@ int tc_i8_pair(const R3dGemmI8& p, cudaStream_t st) {
     P.tma_store = grid16(p.y, p.y_pitch * esz);
     CUtensorMap ta, tb, ty;
     memset(&ty, 0, sizeof ty);
-    if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, kTokC) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt / 2) ||
+    if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, kTokC) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt / 2 - missing_rows()) ||
         (P.tma_store && !rows_map(&ty, p.y, p.n, p.m, p.y_pitch * esz,
                                   P.y_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 128 / esz, 32)))
         return RAD_E_UNSUPPORTED;
@@ -667,7 +680,6 @@ int resident_clusters(int dev, int shares) {
 int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     static bool set[kTcMaxDevices] = {};
     if (!allow_smem(k_i8_stream, kStreamSmem, set)) return RAD_E_DEVICE;
-    static const int missing = getenv("R3D_TEST_I8_MISSING") ? 16 : 0;     /* a test's: boxes of fewer rows than are waited for */
     I8Params P = params_of(p);
     P.mb = p.m > 128 ? 128 : (p.m + 7) / 8 * 8;
     P.tok_tiles = (p.m + 127) / 128;
@@ -723,7 +735,7 @@ int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     const size_t smem = 1024 + (ring > sums ? ring : sums);
     if (smem > kStreamSmem) return RAD_E_UNSUPPORTED;
     CUtensorMap ta, tb;
-    if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, P.mb) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt - missing)) return RAD_E_UNSUPPORTED;
+    if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, P.mb) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt - missing_rows())) return RAD_E_UNSUPPORTED;
     return launch(k_i8_stream, P.tok_tiles * tiles * P.shares, kStreamThreads, smem, P.shares, st, ta, tb, P);
 }
 
