@@ -593,13 +593,14 @@ int launch(K kernel, int grid, int threads, size_t smem, int cluster, cudaStream
     return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
 }
 
+/* host threads may come here at once */
 template <typename K>
-bool allow_smem(K kernel, size_t smem, bool (&set)[kTcMaxDevices]) {
+bool allow_smem(K kernel, size_t smem, std::atomic<bool> (&set)[kTcMaxDevices]) {
     const int dev = tc_device();
     if (dev < 0) return false;
-    if (!set[dev]) {
+    if (!set[dev].load(std::memory_order_acquire)) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
-        set[dev] = true;
+        set[dev].store(true, std::memory_order_release);
     }
     return true;
 }
@@ -615,7 +616,7 @@ I8Params params_of(const R3dGemmI8& p) {
 
 template <int NH>
 int run_pair(const I8Params& P, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ty, cudaStream_t st) {
-    static bool set[kTcMaxDevices] = {};
+    static std::atomic<bool> set[kTcMaxDevices];
     if (!allow_smem(k_i8_pair<NH>, kPairSmem, set)) return RAD_E_DEVICE;
     return launch(k_i8_pair<NH>, 2 * P.workers, kPairThreads, kPairSmem, 1, st, ta, tb, ty, P);
 }
@@ -678,7 +679,7 @@ int resident_clusters(int dev, int shares) {
 }
 
 int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
-    static bool set[kTcMaxDevices] = {};
+    static std::atomic<bool> set[kTcMaxDevices];
     if (!allow_smem(k_i8_stream, kStreamSmem, set)) return RAD_E_DEVICE;
     I8Params P = params_of(p);
     P.mb = p.m > 128 ? 128 : (p.m + 7) / 8 * 8;
