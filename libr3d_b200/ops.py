@@ -35,6 +35,14 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _on_device(device: torch.device | None, launch) -> int:
+    """launch() with `device` as the current one (None: the current one as it is)."""
+    if device is None or device.index == torch.cuda.current_device():
+        return launch()
+    with torch.cuda.device(device):
+        return launch()
+
+
 def _desc(t: torch.Tensor | None, dtype: int, shape=None, stride=None) -> abi.RadTensor:
     if t is None:
         return tensor_desc(None, dtype, [])
@@ -44,6 +52,18 @@ def _desc(t: torch.Tensor | None, dtype: int, shape=None, stride=None) -> abi.Ra
 
 def _group_of(dtype: str, K: int) -> int:
     return {"fp8a8": 128, "i8a8": K}.get(dtype, 32)
+
+
+def _check_i8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, y: torch.Tensor) -> torch.device:
+    """The i8a8 band's operands are what they will be read as, on one device (which is returned)."""
+    wide = (torch.float32, torch.bfloat16)
+    for name, t, types in (("a", a, (torch.int8,)), ("a_scale", a_scale, (torch.float32,)), ("b", b, (torch.int8,)),
+                           ("b_scale", b_scale, wide), ("y", y, wide + (torch.uint16,))):
+        if t.dtype not in types:
+            raise TypeError(f"gemm_nt_q i8a8: {name} is {' or '.join(str(x) for x in types)}, got {t.dtype}")
+    if not a.is_cuda or any(t.device != a.device for t in (a_scale, b, b_scale, y)):
+        raise ValueError("gemm_nt_q i8a8: operands on one CUDA device are needed")
+    return a.device
 
 
 def _gemm_descs(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, y: torch.Tensor,
@@ -76,6 +96,7 @@ def gemm_nt_q(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     `row` forces a row by name; otherwise the band is resolved like the engine would.
     Returns the row that served the call; raises RowRefused on a nonzero status.
     """
+    device = _check_i8(a, a_scale, b, b_scale, y) if dtype == "i8a8" else None
     P = plugin()
     M = y.numel() // N
     if group is None:
@@ -89,7 +110,7 @@ def gemm_nt_q(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     else:
         r = next(x for x in P.rows() + P.ext_rows() if x.name == row)
     pack = ArgPack(_gemm_descs(a, a_scale, b, b_scale, y, dtype, K), query)
-    rc = P.launch_row(r, pack, _stream())
+    rc = _on_device(device, lambda: P.launch_row(r, pack, _stream()))
     if rc != abi.RAD_OK:
         raise RowRefused(r.name, rc)
     return r
@@ -415,6 +436,7 @@ class BoundGemm:
     def __init__(self, a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
                  b_scale: torch.Tensor, y: torch.Tensor, *, dtype: str, N: int, K: int,
                  row: str | None = None):
+        self._device = _check_i8(a, a_scale, b, b_scale, y) if dtype == "i8a8" else None
         P = plugin()
         M = y.numel() // N
         group = _group_of(dtype, K)
@@ -431,6 +453,6 @@ class BoundGemm:
         self._C = _C
 
     def issue(self) -> None:
-        rc = self._fn(self._argp, self._C.c_void_p(_stream()))
+        rc = _on_device(self._device, lambda: self._fn(self._argp, self._C.c_void_p(_stream())))
         if rc != abi.RAD_OK:
             raise RowRefused(self.row.name, rc)
