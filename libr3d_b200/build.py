@@ -2,14 +2,17 @@
 
     python -m libr3d_b200.build
 
-The shared object (and _bind.so, the Python side of its int8 step) lands next to this file so that it travels with the source tree; there
-is no JIT cache and no installed copy. Objects are rebuilt only when a source or header is
-newer. `-fmad=false`: the kernels spell every fused multiply-add they want, because a
-contracted mul+add is a different rounding than the arithmetic contract states.
+The shared object lands next to this file so that it travels with the source tree; there
+is no JIT cache and no installed copy. Building it needs nvcc alone. Where torch is installed,
+_bind.so (the Python side of the int8 step) is built beside it, and again after a change of
+torch. Objects are rebuilt only when a source or header is newer. `-fmad=false`: the kernels
+spell every fused multiply-add they want, because a contracted mul+add is a different rounding
+than the arithmetic contract states.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import subprocess
 import sys
@@ -21,6 +24,7 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "build"
 SO = PKG / "libr3d_b200.so"
 BIND = PKG / "_bind.so"
+BIND_FOR = OBJ / "bind_for.txt"                   # the torch that _bind.so was built against
 
 SOURCES = [
     "rows_table.cpp",
@@ -94,7 +98,6 @@ def build_plugin(verbose: bool = False, ptxas_info: bool = False) -> Path:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
-    build_bind()
     return SO
 
 
@@ -106,7 +109,8 @@ def build_bind() -> Path:
     from torch.utils import cpp_extension
 
     src = CSRC / "bind.cpp"
-    if _stale(BIND, [src, SO, *(ROOT / "include").glob("*.h")]):
+    against = f"torch {torch.__version__} {sys.implementation.cache_tag}"
+    if _stale(BIND, [src, SO, *(ROOT / "include").glob("*.h")]) or not BIND_FOR.exists() or BIND_FOR.read_text() != against:
         home = Path(torch.__file__).resolve().parent
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                *(f"-isystem{p}" for p in cpp_extension.include_paths("cuda")), f"-isystem{sysconfig.get_paths()['include']}",
@@ -117,9 +121,15 @@ def build_bind() -> Path:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("g++ failed on bind.cpp")
+        OBJ.mkdir(exist_ok=True)
+        BIND_FOR.write_text(against)
     return BIND
 
 
 if __name__ == "__main__":
     build_plugin(verbose="-v" in sys.argv, ptxas_info="--ptxas" in sys.argv)
     print(SO)
+    if importlib.util.find_spec("torch") is None:
+        sys.stderr.write("torch is not installed: _bind.so, which ops.py's int8 step goes through, is not built\n")
+    else:
+        print(build_bind())

@@ -8,6 +8,7 @@ current CUDA stream. Nothing is computed here.
 """
 from __future__ import annotations
 
+from pathlib import Path
 from typing import Any
 
 import torch
@@ -322,7 +323,9 @@ def _load_bind():
     try:
         from . import _bind as loaded
     except ImportError as e:
-        raise ImportError("libr3d_b200/_bind.so is not built: run `python -m libr3d_b200.build`") from e
+        built = Path(__file__).with_name("_bind.so").exists()
+        why = f"does not load with this torch ({e})" if built else "is not built"
+        raise ImportError(f"libr3d_b200/_bind.so {why}: run `python -m libr3d_b200.build`") from e
     _bind = loaded
     return loaded
 
