@@ -1,7 +1,7 @@
 /* bind.cpp -- the call path of ops.py's int8 step in C++: torch tensors to RadArgs, resolution, launch. What the
  * ctypes harness of plugin.py does for a row (operands by schema position, the row with the highest priority whose
  * constraints hold, its launch pointer on the current stream), at 6 to 7 us a call on the host, the launch included, instead
- * of 97: a decode step's kernels take 2 to 25 us each. Nothing is computed or remembered here.
+ * of 97: a decode step's kernels take 2 to 25 us each. Nothing is computed here, and nothing of a call is remembered.
  */
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cstring>
+#include <vector>
 #include "rad_abi.h"
 #include "r3d_b200.h"
 
@@ -45,15 +46,27 @@ bool holds(const RadConstraint& c, const RadParam* p, int n) {
     return false;
 }
 
+/* the loader's rows and behind them the extension rows. Both tables are fixed for the process, and walking the loader's by
+ * index takes 3 us: they are walked once */
+const std::vector<const RadKernelInfo*>& all_rows() {
+    static const std::vector<const RadKernelInfo*> all = [] {
+        std::vector<const RadKernelInfo*> v;
+        for (int i = 0; const RadKernelInfo* k = rad_kernel_at(i); ++i) v.push_back(k);
+        for (int i = 0; const RadKernelInfo* k = r3d_b200_ext_kernel_at(i); ++i) v.push_back(k);
+        return v;
+    }();
+    return all;
+}
+
+/* highest priority, the first declared among equals */
 const RadKernelInfo* resolve(const char* op, const RadParam* p, int n) {
     const RadKernelInfo* best = nullptr;
-    const auto consider = [&](const RadKernelInfo* k) {
-        if (strcmp(k->op, op) != 0 || (best && k->priority <= best->priority)) return;
-        for (int i = 0; i < k->n_constraints; ++i) if (!holds(k->constraints[i], p, n)) return;
-        best = k;
-    };
-    for (int i = 0; const RadKernelInfo* k = r3d_b200_ext_kernel_at(i); ++i) consider(k);
-    if (!best) for (int i = 0; const RadKernelInfo* k = rad_kernel_at(i); ++i) consider(k);
+    for (const RadKernelInfo* k : all_rows()) {
+        if (strcmp(k->op, op) != 0 || (best && k->priority <= best->priority)) continue;
+        bool fits = true;
+        for (int i = 0; i < k->n_constraints && fits; ++i) fits = holds(k->constraints[i], p, n);
+        if (fits) best = k;
+    }
     return best;
 }
 
