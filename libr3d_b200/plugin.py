@@ -87,6 +87,7 @@ class Plugin:
                 f"{path} is not built: run `python -m libr3d_b200.build` (nvcc, sm_100a). "
                 "There is no fallback implementation.")
         self.lib = C.CDLL(str(path))
+        self._ext: list[Row] | None = None
         L = self.lib
         L.rad_plugin_abi_version.restype = C.c_uint32
         L.rad_plugin_info.restype = C.POINTER(abi.RadPluginInfo)
@@ -161,8 +162,10 @@ class Plugin:
         return self._rows(self.lib.rad_kernel_count(), self.lib.rad_kernel_at)
 
     def ext_rows(self) -> list[Row]:
-        """The rows of ops the reference does not have."""
-        return self._rows(self.lib.r3d_b200_ext_kernel_count(), self.lib.r3d_b200_ext_kernel_at)
+        """The rows of ops the reference does not have (fixed for the process, read once)."""
+        if self._ext is None:
+            self._ext = self._rows(self.lib.r3d_b200_ext_kernel_count(), self.lib.r3d_b200_ext_kernel_at)
+        return list(self._ext)
 
     @staticmethod
     def _rows(count: int, at) -> list[Row]:
