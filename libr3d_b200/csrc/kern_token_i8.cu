@@ -70,6 +70,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {          /* keeps a
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float max_size_nan(float a, float b, float c) {      /* of their sizes */
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 /* two values an instruction */
 using f2 = unsigned long long;
 __device__ __forceinline__ f2 two_of(float a, float b) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
@@ -109,23 +114,39 @@ __device__ __forceinline__ float step_of(float amax) {
 }
 __device__ __forceinline__ float scale_of(float amax) { return amax < 0x1p-100f ? 1.0f : amax / 127.0f; }
 
-/* silu(g) * u or sigmoid(g) * u; the exponential and the quotient by the special-function unit, 2 ulp each */
-template <int KIND>
+/* silu(g) * u or sigmoid(g) * u; the exponential and the quotient by the special-function unit (2^-22 and 2^-23 of their
+ * results). An argument -g log2 e rounded to f32 would be off by up to 2^-25 of itself, and the exponential by 1.2 |g| units
+ * in the last place for it. So the exponential is of an argument that is known exactly, and what it lacks follows as a factor
+ * 1 + d. SHORT, g of eight bits: its product with the first 16 bits of log2 e is exact, d = -g ln 2 times the other bits
+ * (at most 5e-4 before the sigmoid is 0; d^2 / 2 is left out). Else the product's rounding error is found by a multiply-add
+ * (for g of eight bits, too, that took 5 % more for 8192 x 13824). Where d is infinite or not a number the exponential is 0
+ * or infinite and has to stay so: the factor is held on the side of 1 that it leaves there. */
+template <int KIND, bool SHORT>
 __device__ __forceinline__ f2 gate2(f2 g, f2 u) {
-    float e[2];
-    parts_of(mul2(g, two_of(-1.442695041f, -1.442695041f)), e);
+    const f2 one = two_of(1.0f, 1.0f);
+    const float log2e = SHORT ? 1.442687988f : 1.44269502f;       /* 47274 / 2^15; the nearest f32 */
+    const f2 t = mul2(g, two_of(-log2e, -log2e));
+    float e[2], f[2];
+    parts_of(t, e);
 #pragma unroll
     for (int i = 0; i < 2; ++i) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[i]));
-    parts_of(add2(two_of(e[0], e[1]), two_of(1.0f, 1.0f)), e);
+    if (SHORT) parts_of(fma2(g, two_of(-4.88849515e-6f, -4.88849515e-6f), one), f);
+    else {
+        const f2 d = fma2(g, two_of(1.92596299e-8f, 1.92596299e-8f), fma2(g, two_of(log2e, log2e), t));
+        parts_of(fma2(d, two_of(-0.693147182f, -0.693147182f), one), f);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) f[i] = SHORT ? fmaxf(f[i], 0.5f) : fminf(f[i], 2.0f);
+    parts_of(fma2(two_of(e[0], e[1]), two_of(f[0], f[1]), one), e);
 #pragma unroll
     for (int i = 0; i < 2; ++i) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e[i]));
     const f2 s = two_of(e[0], e[1]);
     return mul2(KIND == kSilu ? mul2(g, s) : s, u);
 }
-template <int KIND>
+template <int KIND, bool SHORT>
 __device__ __forceinline__ float gate(float g, float u) {
     float f[2];
-    parts_of(gate2<KIND>(two_of(g, 0.0f), two_of(u, 0.0f)), f);
+    parts_of(gate2<KIND, SHORT>(two_of(g, 0.0f), two_of(u, 0.0f)), f);
     return f[0];
 }
 
@@ -138,7 +159,7 @@ __device__ __forceinline__ float value_of(const TokenI8& P, int64_t row, int i, 
         const float w = P.w_f32 ? ((const float*)P.w)[i] : bf16_to_f32(((const uint16_t*)P.w)[i]);
         return v * rs * (w + P.wadd);
     }
-    return gate<KIND>(ld1(x + i), ld1(x + P.n + i));
+    return gate<KIND, sizeof(T) == 2>(ld1(x + i), ld1(x + P.n + i));
 }
 
 /* Eight neighbouring values as they lie in memory. */
@@ -291,7 +312,7 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
     int turn = 1;
     for (; row < rows; row += gridDim.x) {
         f2 h[C][4];
-        f2 ss = 0, bad = 0;
+        f2 ss = 0;
         float amax = 0.0f;
         const int here = first;                                   /* this row's; `first` moves on to the next below */
         const bool x_grid = GRID || on16(x + here), y_grid = two && (GRID || on16(y + here));
@@ -316,7 +337,7 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
             for (int j = 0; j < 4; ++j) {
                 h[c][j] = r.pair(j);
                 if (KIND == kRms) ss = fma2(h[c][j], h[c][j], ss);
-                else if (KIND != kQuant) h[c][j] = gate2<KIND>(h[c][j], s.pair(j));
+                else if (KIND != kQuant) h[c][j] = gate2<KIND, sizeof(T) == 2>(h[c][j], s.pair(j));
             }
         }
         /* the slots have been read once their values are in use */
@@ -352,21 +373,14 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
                 }
             }
         }
-        /* fmaxf drops a NaN: 0 * h keeps it */
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float f[2];
                 parts_of(h[c][j], f);
-                amax = fmaxf(fmaxf(amax, fabsf(f[0])), fabsf(f[1]));
-                bad = fma2(h[c][j], two_of(0.0f, 0.0f), bad);
+                amax = max_size_nan(amax, f[0], f[1]);
             }
-        {
-            float f[2];
-            parts_of(bad, f);
-            if (f[0] != 0.0f || f[1] != 0.0f) amax = amax < INFINITY ? NAN : amax;
-        }
         amax = block_reduce(amax, part[turn], max_nan);
         if (KIND != kRms) turn ^= 1;
         const float step = step_of(amax);
