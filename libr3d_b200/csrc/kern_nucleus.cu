@@ -22,6 +22,7 @@
 namespace r3d {
 
 bool tc_pdl_on();                     /* kern_tc.cu: false under R3D_NO_PDL */
+int tc_sm_count();
 
 namespace {
 
@@ -134,7 +135,9 @@ __device__ Sum block_sum(Sum v, Sum* part) {
     return s;
 }
 
-/* rows too long for a cluster's shared memory: one block a row, read again for each step of the searches */
+/* rows too long for a cluster's shared memory (16 CTAs hold 778 thousand f32 or 1.55 million bf16 tokens): one block a row,
+ * read again for each step of the searches, some hundred times: 3 x 900001 f32, top-k 50 and top-p, take 22 ms (1 x 1300000
+ * bf16, in a cluster, 27 us). */
 __global__ void __launch_bounds__(1024) k_nucleus_long(const R3dNucleus P) {
     __shared__ Sum part[32];
     const int64_t m = blockIdx.x;
@@ -996,9 +999,7 @@ int launch_row(const R3dNucleus& P, int size, cudaStream_t st) {
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at; cfg.numAttrs = tc_pdl_on() ? 2 : 1;
-    int sms = 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return RAD_E_DEVICE;
-    const int early = (long long)P.rows * size <= 2 * sms, reorder = !early && P.top_p && P.rows <= kT;
+    const int early = (long long)P.rows * size <= 2 * tc_sm_count(), reorder = !early && P.top_p && P.rows <= kT;
     return cudaLaunchKernelEx(&cfg, kernel, P, e, early, reorder) == cudaSuccess && cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;
 }
 
@@ -1011,15 +1012,20 @@ int launch_nucleus(const R3dNucleus& p, cudaStream_t st) {
     P.shift = 62 - bits < 50 ? 62 - bits : 50;
     count_launch();
     const int ksz = p.x_dtype == RAD_F32 ? 4 : 2;
-    /* CTAs a row: what lets two be on an SM (256 rows of 151936 bf16, settings of their own: 4 CTAs 163 us, 8 203 us; 256 of
-     * 32000: 1 73, 2 70, with top-k 50 for all 25 and 38 us), and more where they all are resident still, down to ten
-     * tokens a thread (1 x 151936, top-k 50: 2 / 4 / 8 / 16 CTAs 26 / 20 / 15.6 / 15.6 us, mixed 75 / 53 / 37 / 34; 30 rows of
-     * 65000 mixed: 2 / 4 / 8 / 16 58 / 41 / 37 / 47 us; 64 of 32000: 38 / 36 / 48 on 2 / 4 / 8); rows of more than 70 tokens
-     * a thread may take a second wave (64 x 151936 mixed: 4 CTAs 86 us, 8 76). */
+    /* CTAs a row: what lets two be on an SM, and more where they are all resident still (a few over the SM count share one),
+     * down to ten tokens a thread; rows of more than 70 tokens a thread may take a second wave. Measured, us, on 1 / 2 / 4 /
+     * 8 / 16 CTAs a row, the rule's in brackets. Settings of their own: 1 x 151936 f32 - / - / 49 / 35 / [28], 30 x 65000
+     * bf16 86 / 58 / 46 / [40] / 52, 64 x 32000 56 / 42 / [37] / 42 / 74, 64 x 151936 - / 132 / 93 / [63] / 90, 150 x 32000
+     * 67 / [53] / 58 / 86 / 168, 256 x 32000 [73] / 68 / 85 / 142 / 283, 256 x 151936 - / 141 / [130] / 180 / 318. Top-k 50 and
+     * top-p for all: 1 x 151936 f32 - / - / 19 / 15 / [13], 256 x 32000 [25] / 40 / 60 / 116 / 226. Which rows need every
+     * token's weight is known on the device alone: a batch of 64 x 151936 without such rows would be faster on fewer CTAs
+     * (- / 28 / 29 / [42] / 72). */
+    const int sms = tc_sm_count();
     int size = 1;
     const auto each = [&]() { return words_of(p.n_vocab, size, ksz) * (4 / ksz); };
     const auto all = [&]() { return (long long)p.rows * size; };
-    while (size < kMaxCluster && (row_smem(p.n_vocab, size, ksz) > 112 * 1024 || (all() <= 150 && each() > 10) || (all() <= 256 && each() > 70))) size *= 2;
+    while (size < kMaxCluster && (row_smem(p.n_vocab, size, ksz) > 112 * 1024 || (64 * all() <= 65 * sms && each() > 10) ||
+                                  (4 * all() <= 7 * sms && each() > 70))) size *= 2;
     if (row_smem(p.n_vocab, size, ksz) > kRowSmem) {
         k_nucleus_long<<<(unsigned)p.rows, 1024, 0, st>>>(P);
         return cudaGetLastError() == cudaSuccess ? RAD_OK : RAD_E_DEVICE;

@@ -24,6 +24,7 @@
 namespace r3d {
 
 bool tc_pdl_on();                     /* kern_tc.cu: false under R3D_NO_PDL */
+int tc_sm_count();
 
 namespace {
 
@@ -487,7 +488,7 @@ int launch_regs(const TokenI8& P, int rows, cudaStream_t st) {
      * 4099 x 5120 codes alone: 17.8 / 13.7 / 12.5 us; 8192 x 13824 gated: two 101, four 96 us, but off the grid, 8191 x 5125, 67 and 88; 16384 x 512 codes:
      * 8.7 / 7.3 / 8.2 us). */
     int c = most <= 8192 ? 1 : most <= 16384 ? 2 : 4;
-    if (rows > 2 * 148 && c < 4) c = KIND != kRms && most > 4096 && (GRID || KIND == kQuant) ? 4 : most > 256 ? 2 : 1;
+    if (rows > 2 * tc_sm_count() && c < 4) c = KIND != kRms && most > 4096 && (GRID || KIND == kQuant) ? 4 : most > 256 ? 2 : 1;
     const int t = ((most + 8 * c - 1) / (8 * c) + 31) / 32 * 32;
     return c == 1 ? launch_rows<KIND, T, 1, GRID>(P, rows, t, st) : c == 2 ? launch_rows<KIND, T, 2, GRID>(P, rows, t, st)
                                                                              : launch_rows<KIND, T, 4, GRID>(P, rows, t, st);
