@@ -227,8 +227,9 @@ int r3d_b200_gemm_fp8a8_gated(const R3dGemmQ* q, void* codes, int64_t q_pitch, f
  * Both apply the oracle's flush per 128 of K; exact, bit-identical to each other. */
 int r3d_b200_gemm_w2a8(const R3dW2A8* q, void* stream);
 
-/* Operands of one gemm_nt_q @ i8a8 call: y[m, n] = (float(sum_k a[m, k] b[n, k]) * a_scale[m]) * b_scale[n], the sum
- * exact in 32-bit integers, the result rounded once to y's type. Every arm gives the same bits. */
+/* Operands of one gemm_nt_q @ i8a8 call: y[m, n] = (sum_k a[m, k] b[n, k] * a_scale[m]) * b_scale[n], the sum
+ * exact in 32-bit integers. f32 results round once (twice where the sum is 2^24 or more), bf16 results are f32(f32(sum) *
+ * a_scale) * b_scale, narrowed. Every arm gives the same bits. */
 typedef struct R3dGemmI8 {
     const void*  a;         /* int8 codes [M, K] */
     const float* a_scale;   /* f32, one a token */

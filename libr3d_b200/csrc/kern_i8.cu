@@ -1,9 +1,10 @@
-/* kern_i8.cu -- gemm_nt_q @ i8a8, any shape and any alignment: y[m, n] = (float(sum_k a[m, k] b[n, k]) * sa[m]) * sb[n].
+/* kern_i8.cu -- gemm_nt_q @ i8a8, any shape and any alignment: y[m, n] = (sum_k a[m, k] b[n, k] * sa[m]) * sb[n].
  *
  * The sum is exact in 32-bit integers (K <= 131071), so its order is free and every arm of this band gives the same
  * bits. 64 tokens x 64 channels a block, 64 of K at a time in shared memory as four-byte words, dp4a; a thread owns
- * 4 x 4 outputs. Serves operands that TMA cannot take (rows off the 16-byte grid); arithmetic-bound far below the
- * tensor-core arms.
+ * 4 x 4 outputs. Serves operands that TMA cannot take (rows off the 16-byte grid). Bound by its own instructions, far
+ * below the tensor-core arms: with K = 5121 instead of 5120, 16 x 27648 takes 369 us for 24, 128 x 5120 321 for 11.4, 2048 x
+ * 5120 1830 for 39; 1 x 4096, K = 4097, 204 for 6.6. Rows padded to 16 bytes keep a caller off it.
  */
 #include "r3d_kernels.h"
 #include "r3d_numerics.cuh"
@@ -57,9 +58,8 @@ __global__ void __launch_bounds__(256) k_i8_tile(const R3dGemmI8 P, const int a_
             if (n >= P.n) continue;
             const int64_t at = (int64_t)n * P.bs_pitch;
             const float t = P.bs_dtype == RAD_F32 ? ((const float*)P.b_scale)[at] : bf16_to_f32(((const uint16_t*)P.b_scale)[at]);
-            const float y = __fmul_rn(__fmul_rn((float)acc[i][j], s), t);
-            if (P.y_dtype == RAD_F32) ((float*)P.y)[(int64_t)m * P.y_pitch + n] = y;
-            else ((uint16_t*)P.y)[(int64_t)m * P.y_pitch + n] = f32_to_bf16(y);
+            if (P.y_dtype == RAD_F32) ((float*)P.y)[(int64_t)m * P.y_pitch + n] = scaled_once(acc[i][j], s, t);
+            else ((uint16_t*)P.y)[(int64_t)m * P.y_pitch + n] = f32_to_bf16(__fmul_rn(__fmul_rn((float)acc[i][j], s), t));
         }
     }
 }

@@ -1,6 +1,9 @@
 /* kern_tc_i8.cu -- gemm_nt_q @ i8a8 on the tensor core (tcgen05 kind::i8, 32-bit integer accumulators in tensor
- * memory): y[m, n] = (float(sum_k a[m, k] b[n, k]) * sa[m]) * sb[n]. The sum over the whole of K is one exact
- * accumulation, so the result does not depend on tiles, splits or order, and the scales are two multiplies at the end.
+ * memory): y[m, n] = (sum_k a[m, k] b[n, k] * sa[m]) * sb[n]. The sum over the whole of K is one exact
+ * accumulation, so the result does not depend on tiles, splits or order. An f32 result carries the first product's rounding
+ * error on (scaled_once: 2 more operations a value, 8192 x 5120 x 5120 178 -> 179 us, 8192 x 8192 x 512 63 -> 65; with the
+ * low bits of sums beyond 2^24, too, 184 and 69). A bf16 result is two f32 products, then narrowed: one in 195 thousand is
+ * not the bf16 number next to the exact value.
  *
  * Tokens lie on the MMA's M axis (tensor-memory lanes), channels on its N axis (columns): a thread of the epilogue
  * owns a token, whose channels lie next to each other in registers as they do in y, and the channel tile can be any
@@ -355,8 +358,8 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float4 w = *(const float4*)(sb + c + 4 * j);
-                        row[j ^ (lane & 7)] = make_uint4(__float_as_uint(scaled(r[4 * j], sa, w.x)), __float_as_uint(scaled(r[4 * j + 1], sa, w.y)),
-                                                         __float_as_uint(scaled(r[4 * j + 2], sa, w.z)), __float_as_uint(scaled(r[4 * j + 3], sa, w.w)));
+                        row[j ^ (lane & 7)] = make_uint4(__float_as_uint(scaled_once((int)r[4 * j], sa, w.x)), __float_as_uint(scaled_once((int)r[4 * j + 1], sa, w.y)),
+                                                         __float_as_uint(scaled_once((int)r[4 * j + 2], sa, w.z)), __float_as_uint(scaled_once((int)r[4 * j + 3], sa, w.w)));
                     }
                 } else {
 #pragma unroll
@@ -514,15 +517,16 @@ k_i8_stream(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             const int t = item / quads, c = 4 * (item - t * quads), live = P.n - n0 - c;
             const float sa = sa_s[t];
             const float4 sb = *(const float4*)(sb_s + c);
-            const float y[4] = {scaled((uint32_t)v.x, sa, sb.x), scaled((uint32_t)v.y, sa, sb.y), scaled((uint32_t)v.z, sa, sb.z), scaled((uint32_t)v.w, sa, sb.w)};
             const int64_t at = (int64_t)(t0 + t) * P.y_pitch + n0 + c;
             if (P.y_f32) {
+                const float y[4] = {scaled_once(v.x, sa, sb.x), scaled_once(v.y, sa, sb.y), scaled_once(v.z, sa, sb.z), scaled_once(v.w, sa, sb.w)};
                 float* const o = (float*)P.y + at;
                 if (P.y_quads && live >= 4) *(float4*)o = make_float4(y[0], y[1], y[2], y[3]);
                 else
 #pragma unroll
                     for (int j = 0; j < 4; ++j) if (j < live) o[j] = y[j];
             } else {
+                const float y[4] = {scaled((uint32_t)v.x, sa, sb.x), scaled((uint32_t)v.y, sa, sb.y), scaled((uint32_t)v.z, sa, sb.z), scaled((uint32_t)v.w, sa, sb.w)};
                 uint16_t* const o = (uint16_t*)P.y + at;
                 if (P.y_quads && live >= 4) *(uint2*)o = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
                 else
@@ -690,9 +694,11 @@ int tc_i8_stream(const R3dGemmI8& p, cudaStream_t st) {
     if (per_sm == 1) {
         /* 65 tokens and more (fewer than 160 channels an SM up to 128): a CTA has an SM, and the channels of a tile and the K shares are
          * those with the lowest cost of a K block (its two operands' way into shared memory), of a tile's results, and of
-         * adding the shares' sums, in nanoseconds, fitted to 540 measured forms of thirteen sizes (12288 channels, K = 4096,
-         * 128 tokens: 128 tiles of 96 14.8 us, 192 channels in two shares 19.0 us; 5120, 13824: 4 shares of 160 channels
-         * 18.6 us, 2 of 80 18.8, 4 of 192 19.9). Beyond 160 channels an SM two CTAs, one's results under the other's loads
+         * adding the shares' sums. A ranking, not a time: launch, ring fill and drain, some 6 us, are the same for all
+         * forms and left out (12288 channels, K = 4096, 128 tokens: cost 8.9, measured 14.6 us). Fitted to 540 forms of
+         * thirteen sizes; against all forms of six sizes measured since, the choice is within 4 % of the best for five
+         * (77 x 5119 x 13808 18.8 and 18.3 us, 128 x 5120 x 13824 18.7 and 18.7, 191 x 576 x 13568 8.9 and 8.6) and 11 % off
+         * for one (457 x 2304 x 6272 14.5 us, 64 channels in one share 13.1). Beyond 160 channels an SM two CTAs, one's results under the other's loads
          * (27648, 5120, 128 tokens: 29.2 us, one CTA of 192 channels 31.4; 20480, 4096: 20.0 us and, with one, 19.7). */
         long best = -1;
         for (int nt = 48; nt <= 256; nt += 16)

@@ -109,6 +109,14 @@ R3D_HD int e2m1_x2(uint8_t n) {
     return (n & 8) ? -mag : mag;
 }
 
+/* An exact int8 product's sum times its token's and its channel's scale: rounded once to f32 where the sum is below 2^24 (as
+ * long as sum * sa is a normal number), and before that to its 24 bits where it is not. The first product goes on with its
+ * rounding error. An infinite scale gives NaN. */
+__device__ __forceinline__ float scaled_once(int sum, float sa, float sb) {
+    const float f = (float)sum, p = __fmul_rn(f, sa);
+    return __fmaf_rn(p, sb, __fmul_rn(__fmaf_rn(f, sa, -p), sb));
+}
+
 /* E8M0 -> f32 (src/r3d_mxfp4_q8x.h:29-37): 2^(x-127); 0xFF is NaN; 0x00 is the f32
  * subnormal 2^-127, not zero. */
 R3D_HD float e8m0_to_f32(uint8_t x) {

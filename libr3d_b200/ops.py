@@ -345,7 +345,9 @@ def gemm_i8a8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
               y: torch.Tensor | None = None, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """y[..., N] = (sum_k a[..., k] * b[n, k]) * a_scale[...] * b_scale[n]: int8 codes [..., K] and [N, K], one f32
     scale a token ([...] or [..., 1]) and one f32 or bf16 scale a channel ([N] or [N, 1]). The sum is exact (K at
-    most 131071), the result is rounded once, to `out_dtype` (bf16 or f32), or to y's type where y is given."""
+    most 131071). The result is of `out_dtype` (bf16 or f32), or of y's type where y is given: f32 rounds once (twice
+    where the sum is 2^24 or more), bf16 narrows the two products in f32. Rows off the 16-byte grid (K not a multiple of
+    16) are served by a kernel some 10 to 50 times slower."""
     N, K = b.shape
     if y is None:
         if out_dtype not in _KIND_OF:
