@@ -7,14 +7,16 @@
  *   all       amax = max |h|; scale = amax / 127; code = rint(h * 127 / amax), halves to even.
  *
  * h stays in f32 from the operands to the code: it is rounded once, to eight bits. A row of zeros (amax below
- * 2^-100, where 127 / amax would overflow) has scale 1 and codes 0; a NaN or an infinity in a row makes its scale
+ * 2^-100, before 127 / amax comes near the end of f32) has scale 1 and codes 0; a NaN or an infinity in a row makes its scale
  * NaN or infinite, so it reaches the product's output, and the codes of what cannot be scaled are 0.
  *
  * Bound by memory: x is read once (rmsnorm also reads and writes the residual), one byte a value is written. So a
- * block owns a row and keeps h in registers between the reduction and the codes: k_token_i8_regs, eight values a
- * thread and chunk, by 16-byte loads where every operand's rows lie on the 16-byte grid (codes: 8), else one value at
- * a time, neighbouring threads next to each other. Rows of more than 32760 values, or of f32 values and two streams beyond
- * 27648, which the shared memory does not hold, are read again for each step.
+ * block walks rows and keeps a row's h in registers between the reduction and the codes: k_token_i8_regs, chunks of eight
+ * values on the codes' 8-byte grid. Each operand whose chunks lie on the 16-byte grid is copied ahead by cp.async, whatever
+ * the others do; gated halves off it, and a norm's w off it beside f32 rows, are read by the 16-byte words around them, a
+ * row's ends (and the other operands off the grid) one value at a time. The sum of a norm's squares follows the chunks and
+ * the threads, so its last bit depends on how many rows a call has and on where they begin. Rows of more than 32760 values,
+ * or of f32 values and two streams beyond 27648, which the shared memory does not hold, are read again for each step.
  */
 #include <atomic>
 #include <cmath>
