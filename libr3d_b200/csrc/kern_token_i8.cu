@@ -101,20 +101,43 @@ __device__ __forceinline__ float block_reduce(float v, float* part, F f) {
     return v;
 }
 
-/* 1.5 * 2^23: the low byte of fma(h, step, kCode) is the whole number nearest to h * step, ties to even */
+/* The code of h is the low byte of h * step + kCode, kCode = 1.5 * 2^23: the whole number next to it, halves to even.
+ * A row of zeros, and one so small that 127 / amax is not a number of this type, has step 0: codes 0. So has a row with a NaN
+ * or an infinity in it.
+ * h of eight bits (bf16 rows as they are): step is 127 / amax rounded up, and the sum rounds once. h * step is never below the
+ * quotient it stands for, so that h = amax / 2, where that is 63.5 exactly, goes to the even 64 whatever amax is (rounded to
+ * nearest, the step of 66 of the 128 significands that amax has in bf16 is low, and their halves went to 63). Among quotients
+ * of two bf16 numbers there is no other half, save where the step is exact (amax = 127 2^n), and what is not a half lies
+ * further from one than the step's error: the codes are the quotients' own.
+ * Other h: quotients lie anywhere, so the step goes on with what its rounding left, and h * step is off by its own rounding
+ * alone, a quarter of what the step rounded up leaves on average; halves stay halves. (8192 x 5120 norm: 14 codes of a
+ * million are not the 64-bit quotient's, with the step rounded up 25, 16 by plain f32 operations.) Not for the gated
+ * product, whose own roundings are ten times the step's (8192 x 13824 101 us instead of 97). */
 constexpr float kCode = 12582912.0f;
 
-/* 127 / amax rounded up. h * step is then rounded once, to the whole number, and is never below the quotient it stands
- * for, so that h = amax / 2, where that is 63.5 exactly, goes to the even 64 whatever amax is (rounded to nearest, the step
- * of 66 of the 128 significands that amax has in bf16 is low, and their halves went to 63). Among quotients of two bf16
- * numbers there is no other half, save where the step is exact (amax = 127 2^n), and what is not a half lies further from
- * one than the step's error: the codes of bf16 rows are the quotients' own. A row of zeros, and one so small that 127 / amax is not a number of this type, has step 0: codes 0. So
- * has a row with a NaN or an infinity in it. */
-__device__ __forceinline__ float step_of(float amax) {
-    if (amax < 0x1p-100f || !(amax < INFINITY)) return 0.0f;
-    const float q = 127.0f / amax;
-    return fmaf(q, amax, -127.0f) < 0.0f ? __uint_as_float(__float_as_uint(q) + 1u) : q;      /* the residual's sign is exact */
-}
+__device__ __forceinline__ bool has_step(float amax) { return amax >= 0x1p-100f && amax < INFINITY; }
+template <int KIND, typename T> constexpr bool kShortStep = KIND != kRms && (KIND != kQuant || sizeof(T) == 2);
+template <bool SHORT> struct Step;
+template <> struct Step<true> {
+    float s;
+    __device__ __forceinline__ explicit Step(float amax) : s(0.0f) {
+        if (!has_step(amax)) return;
+        s = 127.0f / amax;
+        if (fmaf(s, amax, -127.0f) < 0.0f) s = __uint_as_float(__float_as_uint(s) + 1u);      /* the residual's sign is exact */
+    }
+    __device__ __forceinline__ f2 codes(f2 h) const { return fma2(h, two_of(s, s), two_of(kCode, kCode)); }
+};
+template <> struct Step<false> {
+    float s, rest;
+    __device__ __forceinline__ explicit Step(float amax) : s(0.0f), rest(0.0f) {
+        if (!has_step(amax)) return;
+        s = 127.0f / amax;
+        rest = fmaf(-s, amax, 127.0f) * (s * (1.0f / 127.0f));
+    }
+    __device__ __forceinline__ f2 codes(f2 h) const {
+        return add2(fma2(h, two_of(s, s), mul2(h, two_of(rest, rest))), two_of(kCode, kCode));
+    }
+};
 __device__ __forceinline__ float scale_of(float amax) { return amax < 0x1p-100f ? 1.0f : amax / 127.0f; }
 
 /* silu(g) * u or sigmoid(g) * u; the exponential and the quotient by the special-function unit (2^-22 and 2^-23 of their
@@ -386,9 +409,8 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
             }
         amax = block_reduce(amax, part[turn], max_nan);
         if (KIND != kRms) turn ^= 1;
-        const float step = step_of(amax);
+        const Step<kShortStep<KIND, T>> step(amax);
         if (threadIdx.x == 0) P.scale[row * P.s_pitch] = scale_of(amax);
-        const f2 step2 = two_of(step, step), code2 = two_of(kCode, kCode);
         int8_t* const q = P.q + row * P.q_pitch;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -399,11 +421,11 @@ __global__ void __launch_bounds__(1024, C == 4 ? 1 : 2) k_token_i8_regs(const To
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 float f[4];
-                parts_of(fma2(h[c][2 * j], step2, code2), f);
-                parts_of(fma2(h[c][2 * j + 1], step2, code2), f + 2);
+                parts_of(step.codes(h[c][2 * j]), f);
+                parts_of(step.codes(h[c][2 * j + 1]), f + 2);
                 w[j] = __byte_perm(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040),
                                    __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040), 0x5410);
-                if (step == 0.0f) w[j] = 0u;
+                if (step.s == 0.0f) w[j] = 0u;
             }
             if (in) *(uint2*)(q + at) = make_uint2(w[0], w[1]);
             else
@@ -439,11 +461,13 @@ __global__ void __launch_bounds__(512) k_token_i8(const TokenI8 P) {
     float amax = 0.0f;
     for (int i = threadIdx.x; i < P.n; i += blockDim.x) amax = max_nan(amax, fabsf(value_of<KIND, T>(P, row, i, rs)));
     amax = block_reduce(amax, part[1], max_nan);
-    const float step = step_of(amax);
+    const Step<kShortStep<KIND, T>> step(amax);
     if (threadIdx.x == 0) P.scale[row * P.s_pitch] = scale_of(amax);
     for (int i = threadIdx.x; i < P.n; i += blockDim.x) {
         const float h = value_of<KIND, T>(P, row, i, rs);
-        P.q[row * P.q_pitch + i] = step == 0.0f ? (int8_t)0 : (int8_t)(__float_as_uint(fmaf(h, step, kCode)) & 0xffu);
+        float f[2];
+        parts_of(step.codes(two_of(h, 0.0f)), f);
+        P.q[row * P.q_pitch + i] = step.s == 0.0f ? (int8_t)0 : (int8_t)(__float_as_uint(f[0]) & 0xffu);
         if (P.ob) {
             if (P.ob_f32) ((float*)P.ob)[row * P.ob_pitch + i] = h;
             else ((uint16_t*)P.ob)[row * P.ob_pitch + i] = f32_to_bf16(h);

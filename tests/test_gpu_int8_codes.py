@@ -51,3 +51,15 @@ def test_halves_of_the_norm_and_of_the_gated_form(n):
     gate = torch.linspace(-3, 3, 128, device="cuda")[:, None].expand(128, n).to(BF16)
     q, _ = ops.gated_quant_token_i8(torch.cat([gate, x], 1), act="sigmoid")
     assert torch.equal(q[sure], torch.where(x != 0, code, 0)[sure])
+
+
+@pytest.mark.parametrize("n", [5120, 1201, 40000])
+def test_codes_of_f32_rows_lie_within_one_rounding_of_the_quotient(n):
+    """quotients of f32 numbers lie anywhere: what decides between two codes is the quotient rounded to f32, off by at most
+    half a step of the numbers below 128, 2^-18, and its factor's two parts, off by 2^-40 of it"""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    for M in (20_000_000 // n, 40):
+        x = torch.randn(M, n, generator=g, device="cuda") * 2.0 ** torch.randint(-40, 40, (M, 1), generator=g, device="cuda")
+        q, _ = ops.quant_token_i8(x)
+        ratio = x.double() * 127 / x.double().abs().amax(-1, keepdim=True)
+        assert bool(((q.double() - ratio).abs() <= 0.5 + 2.0 ** -18 + 127 * 2.0 ** -40).all())
