@@ -47,7 +47,7 @@ struct I8Params {
     int tok_tiles, ch_tiles, workers, group;
     int whole, split, jobs;                        /* pair: jobs below `whole` are tiles, those above halves of one if `split` */
     int mb, stages, shares;                        /* stream: token rows of a box, ring, K shares */
-    int tma_store, y_quads;                        /* y on the 16-byte grid; y's rows on that of four elements */
+    int tma_store, y_quads;                        /* pair: y's rows on the 16-byte grid (2: not their ends); stream: on that of four elements */
 };
 
 /* kind::i8: s32 accumulators (2 at bit 4), a and b signed (1 at bits 7 and 10), N >> 3 at bit 17, M >> 4 at bit 24 */
@@ -333,6 +333,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
             tc_fence_after();
             aph ^= 1u;
             const bool live = tw < P.m;                           /* the warp has tokens at all */
+            const bool tma = P.tma_store == 1 || (P.tma_store == 2 && n0 + P.nt <= P.n);
             uint32_t bufs[2][32];
             if (live) tmem_ld32(ta, bufs[0]);
 #pragma unroll 1
@@ -372,7 +373,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
                 }
                 if ((c + 32) % cols && c + 32 < P.nt) continue;
                 const int cb = c / cols * cols, have = min(c + 32 - cb, P.n - n0 - cb);   /* channels staged and inside y */
-                if (P.tma_store) {
+                if (tma) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0 && have > 0) {
@@ -654,7 +655,8 @@ int tc_i8_pair(const R3dGemmI8& p, cudaStream_t st) {
     P.workers = P.jobs < pairs ? P.jobs : pairs;
     P.group = 16;
     const int esz = P.y_f32 ? 4 : 2;
-    P.tma_store = grid16(p.y, p.y_pitch * esz);
+    /* a box is clipped to whole 16 bytes: where y's rows end inside one, the tiles at their end are stored by words */
+    P.tma_store = !grid16(p.y, p.y_pitch * esz) ? 0 : (int64_t)p.n * esz % 16 == 0 ? 1 : 2;
     CUtensorMap ta, tb, ty;
     memset(&ty, 0, sizeof ty);
     if (!codes_map(&ta, p.a, p.k, p.m, p.a_pitch, kTokC) || !codes_map(&tb, p.b, p.k, p.n, p.b_pitch, P.nt / 2 - missing_rows()) ||
