@@ -421,7 +421,8 @@ def sample_nucleus(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.
     shortest first part that holds p of what top_k left (p >= 1: all), min_p those at least min_p times as likely as
     the first; the first always stays. The answer is the first kept id, ascending, at which the running share of the
     kept probability exceeds u. temperature <= 0 is greedy. Every parameter is a plane with one value a row (f32
-    but for top_k), or None. -inf and NaN logits are masked; a row with nothing left reports -1.
+    but for top_k), or None. -inf and NaN logits are masked; a row with nothing left reports -1. A token
+    less than some 2^-45 times as likely as the first has no share.
     `logprob` (f32) receives the log of the token's share of what was kept, `kept` (int32) how many tokens were."""
     V = logits.shape[-1]
     if token is None:
