@@ -6,7 +6,9 @@
  * device-resident blob are copied to the host once, on first sight of that pointer, and remembered
  * (weights are immortal for the life of the engine). That first call synchronises; later calls do
  * not. The engine may still put another blob at the same address (a reload, a caching allocator):
- * callers re-read once before they refuse on a remembered header, and r3d_b200_forget_head drops one. */
+ * callers re-read once before they refuse on a remembered header, and r3d_b200_forget_head drops one. A blob in the host's
+ * memory costs a copy, not a synchronisation: its header is read at every call and not remembered, so that another
+ * blob at its address is never taken for it. */
 #include <vector>
 #include <cuda_runtime.h>
 #include "entry_util.h"
@@ -23,11 +25,14 @@ struct HeadView {
 };
 std::vector<HeadView*>& seen_heads() { static std::vector<HeadView*> v; return v; }
 
-bool read_head(HeadView* v) {
+cudaMemoryType memory_of(const void* p) {
     cudaPointerAttributes at{};
-    const bool have = cudaPointerGetAttributes(&at, v->blob) == cudaSuccess;
-    if (!have) (void)cudaGetLastError();
-    if (have && at.type == cudaMemoryTypeDevice) {
+    if (cudaPointerGetAttributes(&at, p) == cudaSuccess) return at.type;
+    (void)cudaGetLastError();
+    return cudaMemoryTypeUnregistered;
+}
+bool read_head(HeadView* v) {
+    if (memory_of(v->blob) == cudaMemoryTypeDevice) {
         if (cudaMemcpy(v->head, v->blob, sizeof v->head, cudaMemcpyDeviceToHost) != cudaSuccess) {
             (void)cudaGetLastError();
             return false;
@@ -42,6 +47,12 @@ bool read_head(HeadView* v) {
 const unsigned char* planes_head_of(const void* blob, bool* cached) {
     for (const HeadView* v : seen_heads()) if (v->blob == blob) { *cached = true; return v->head; }
     *cached = false;
+    const cudaMemoryType type = memory_of(blob);
+    if (type != cudaMemoryTypeDevice && type != cudaMemoryTypeManaged) {
+        static thread_local HeadView here;                        /* until this thread's next call */
+        memcpy(here.head, blob, sizeof here.head);
+        return here.head;
+    }
     HeadView* v = new HeadView;
     v->blob = blob;
     if (!read_head(v)) { delete v; return nullptr; }
