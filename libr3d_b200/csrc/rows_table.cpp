@@ -409,7 +409,7 @@ const RadKernelInfo kExtRows[] = {
         "int8 a + f32 a_scale [M], int8 b + f32/bf16 b_scale [N], bf16/f32 y; a_sum and b_ref refused",
         kPrioPlain, kCI8, r3d_rad_gemm_nt_q_i8),
     ROW("quant_token_i8_act", "quant_token_i8", "band",
-        "per-token symmetric int8 quantisation, one block a row",
+        "per-token symmetric int8 quantisation, a block walks rows",
         "f32/bf16 input, any width", "activation in, int8 codes and f32 scales out",
         kPrioPlain, kCBand, r3d_rad_quant_token_i8),
     ROW("gated_quant_token_i8_act", "gated_quant_token_i8", "band",
